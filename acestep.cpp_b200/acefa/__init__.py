@@ -11,12 +11,13 @@ an sm_100 GPU every call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
 import torch
 
-GGML_F32, GGML_F16, GGML_Q8_0, GGML_BF16 = 0, 1, 8, 30
+GGML_F32, GGML_F16, GGML_Q8_0, GGML_I8, GGML_I32, GGML_BF16 = 0, 1, 8, 24, 26, 30
 PREC_DEFAULT, PREC_F32 = 0, 10
 
 OK = 0
@@ -51,6 +52,12 @@ EXPORTED_SYMBOLS = (
     "acefa_flash_attn_ext_fused",
     "acefa_kv_prologue",
     "acefa_cfg_logit_combine",
+    "acefa_kv8_store",
+    "acefa_kv8_load",
+    "acefa_kv8_attn",
+    "acefa_kv8_attn_workspace_bytes",
+    "acefa_kv8_evict",
+    "acefa_flash_attn_packed",
 )
 
 MAX_MIRRORS = 7
@@ -59,6 +66,9 @@ PEER_HANDLE_BYTES = 64
 # mask rules (acefa_mask_gen)
 MASK_CAUSAL, MASK_WINDOW, MASK_PADDING = 1, 2, 3
 MASK_GEN_MAX_BATCH = 32
+
+# 8-bit block-scaled KV cache (acefa_kv8_cache)
+KV8_BLOCK, KV8_MAX_SETS, KV8_MAX_ROWS = 64, 1024, 64
 
 
 class MaskGen(ctypes.Structure):
@@ -141,6 +151,11 @@ class Tensor(ctypes.Structure):
     ]
 
 
+class Kv8CacheC(ctypes.Structure):
+    """acefa_kv8_cache."""
+    _fields_ = [("k", Tensor), ("v", Tensor), ("k_scale", Tensor), ("v_scale", Tensor)]
+
+
 _lib = None
 
 
@@ -195,6 +210,22 @@ def load_library(path: str | None = None):
                                             ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
                                             ctypes.c_void_p, ctypes.c_void_p]
     lib.acefa_cfg_logit_combine.restype = ctypes.c_int
+    C = ctypes.POINTER(Kv8CacheC)
+    lib.acefa_kv8_store.argtypes = [C, T, T, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    lib.acefa_kv8_store.restype = ctypes.c_int
+    lib.acefa_kv8_load.argtypes = [C, ctypes.c_void_p, T, T, ctypes.c_void_p]
+    lib.acefa_kv8_load.restype = ctypes.c_int
+    lib.acefa_kv8_attn.argtypes = [T, C, ctypes.c_void_p, T, ctypes.c_float, T, ctypes.c_void_p, ctypes.c_void_p,
+                                   ctypes.c_size_t]
+    lib.acefa_kv8_attn.restype = ctypes.c_int
+    lib.acefa_kv8_attn_workspace_bytes.argtypes = [T, C, T]
+    lib.acefa_kv8_attn_workspace_bytes.restype = ctypes.c_size_t
+    lib.acefa_kv8_evict.argtypes = [C, T, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, C, T, T, ctypes.c_void_p,
+                                    ctypes.c_void_p]
+    lib.acefa_kv8_evict.restype = ctypes.c_int
+    lib.acefa_flash_attn_packed.argtypes = [T, T, T, T, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+                                            ctypes.c_int, ctypes.c_float, ctypes.c_void_p]
+    lib.acefa_flash_attn_packed.restype = ctypes.c_int
     lib.acefa_peer_export.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint64)]
     lib.acefa_peer_export.restype = ctypes.c_int
     lib.acefa_peer_import.argtypes = [ctypes.c_void_p, ctypes.c_uint64, ctypes.POINTER(ctypes.c_void_p)]
@@ -215,6 +246,10 @@ def _ggml_type(t: torch.Tensor, gtype: int | None) -> int:
         return GGML_F16
     if t.dtype == torch.bfloat16:
         return GGML_BF16
+    if t.dtype == torch.int8:
+        return GGML_I8
+    if t.dtype == torch.int32:
+        return GGML_I32
     raise TypeError(f"no ggml type for {t.dtype}; pass gtype=GGML_Q8_0 for uint8 Q8_0 blocks")
 
 
@@ -467,6 +502,211 @@ def cfg_logit_combine(cond: torch.Tensor, uncond: torch.Tensor | None, eos_idx: 
     if st != OK:
         raise AcefaError(st, "acefa_cfg_logit_combine")
     return out
+
+
+# --------------------------------------------------------------------------
+# A KV cache in 8 bits with a scale per 64 tokens and head, and packed prompts.
+# Every class below describes its operands once; calling it launches.
+
+class _Call:
+    """An entry with its operands: keeps the tensors alive, runs on their device,
+    on the stream given or that device's current one."""
+
+    def _bind(self, what, tensors, *args):
+        dev = tensors[0].device
+        for t in tensors:
+            if t.device != dev:
+                raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        self._what, self._keep, self._args, self._device = what, tensors, args, dev
+        self._fn = getattr(load_library(), what)
+
+    def _launch(self, stream):
+        # a CUDA tensor's device always has an index; CPU tensors reach the ABI only in its argument checks
+        index = self._device.index if self._device.type == "cuda" else None
+        if stream is None:
+            stream = torch.cuda.current_stream(index) if index is not None else None
+        elif index is not None and stream.device.index != index:
+            raise ValueError(f"{self._what}: a stream of {stream.device} for tensors on {self._device}")
+        handle = ctypes.c_void_p(stream.cuda_stream if stream is not None else 0)
+        if index is None or index == torch.cuda.current_device():
+            st = self._fn(*self._args[0], handle, *self._args[1])
+        else:
+            with torch.cuda.device(index):
+                st = self._fn(*self._args[0], handle, *self._args[1])
+        if st != OK:
+            raise AcefaError(st, self._what)
+
+
+def _int32(t, n, what):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 tensor of {n}")
+    return ctypes.c_void_p(t.data_ptr())
+
+
+class Kv8Cache:
+    """acefa_kv8_cache: k, v (sets, Hkv, n_max, D) int8, k_scale, v_scale (sets, Hkv, ceil(n_max / 64)) f32."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        for t, dtype, dim in ((k, torch.int8, 4), (v, torch.int8, 4), (k_scale, torch.float32, 3),
+                              (v_scale, torch.float32, 3)):
+            if t.dtype != dtype or t.dim() != dim:
+                raise ValueError("Kv8Cache: int8 k, v of 4 dims and f32 k_scale, v_scale of 3")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.c = Kv8CacheC(describe(k), describe(v), describe(k_scale), describe(v_scale))
+
+    @classmethod
+    def empty(cls, n_max, n_kv_heads, n_sets, head_dim, device="cuda"):
+        shape, blocks = (n_sets, n_kv_heads, n_max, head_dim), -(-n_max // KV8_BLOCK)
+        k, v = (torch.empty(shape, dtype=torch.int8, device=device) for _ in range(2))
+        ks, vs = (torch.empty((n_sets, n_kv_heads, blocks), device=device) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+    def sets(self, lo, hi):
+        """Sets lo .. hi - 1 of this cache (a view)."""
+        return Kv8Cache(self.k[lo:hi], self.v[lo:hi], self.k_scale[lo:hi], self.v_scale[lo:hi])
+
+    @property
+    def tensors(self):
+        return (self.k, self.v, self.k_scale, self.v_scale)
+
+
+class Kv8Store(_Call):
+    """acefa_kv8_store: the sets' new rows k_new, v_new (Hkv, rows, D) f32 / f16 / bf16, any strides over
+    heads and rows, go to cache rows pos[s] .. of each set; cu_rows (sets + 1) int32 says which rows are whose
+    (None: the same number each)."""
+
+    def __init__(self, cache, k_new, v_new, pos, cu_rows=None):
+        n = cache.k.shape[0]
+        self.tk, self.tv = describe(k_new), describe(v_new)
+        cu = _int32(cu_rows, n + 1, "cu_rows") if cu_rows is not None else None
+        self._bind("acefa_kv8_store", (*cache.tensors, k_new, v_new, pos) + ((cu_rows,) if cu_rows is not None else ()),
+                   (ctypes.byref(cache.c), _ref(self.tk), _ref(self.tv), cu, _int32(pos, n, "pos")), ())
+        self.cache = cache
+
+    def __call__(self, stream=None):
+        self._launch(stream)
+        return self.cache
+
+
+class Kv8Load(_Call):
+    """acefa_kv8_load: rows 0 .. n - 1 of every set as values in k_dst, v_dst (sets, Hkv, n, D) f32 / f16 /
+    bf16; rows at or past lens[s] become zeros."""
+
+    def __init__(self, cache, lens, k_dst, v_dst):
+        self.tk, self.tv = describe(k_dst), describe(v_dst)
+        self._bind("acefa_kv8_load", (*cache.tensors, lens, k_dst, v_dst),
+                   (ctypes.byref(cache.c), _int32(lens, cache.k.shape[0], "lens"), _ref(self.tk), _ref(self.tv)), ())
+        self.cache, self.out = cache, (k_dst, v_dst)
+
+    def __call__(self, stream=None):
+        self._launch(stream)
+        return self.out
+
+
+class Kv8Attn(_Call):
+    """acefa_kv8_attn: q (sets, Hq, n_q, D) over the first lens[s] rows of each set; returns out (sets, n_q, Hq, D),
+    of q's type unless given.  weight (sets, Hkv, n_max) f32 or None: grows by each row's attention weight."""
+
+    def __init__(self, q, cache, lens, scale=None, weight=None, out=None):
+        if out is None:
+            B, Hq, n_q, D = q.shape
+            out = torch.empty((B, n_q, Hq, D), dtype=q.dtype, device=q.device)
+        self.out, self.cache, self.weight = out, cache, weight
+        self.tq, self.td, self.tw = describe(q), describe(out), describe(weight)
+        with torch.cuda.device(q.device.index if q.is_cuda else -1):  # sized for the tensors' device
+            n = int(load_library().acefa_kv8_attn_workspace_bytes(_ref(self.tq), ctypes.byref(cache.c), _ref(self.tw)))
+        self.workspace = torch.empty(max(n, 256), dtype=torch.uint8, device=q.device)
+        keep = (*cache.tensors, q, lens, out, self.workspace) + ((weight,) if weight is not None else ())
+        self._bind("acefa_kv8_attn", keep,
+                   (_ref(self.tq), ctypes.byref(cache.c), _int32(lens, cache.k.shape[0], "lens"), _ref(self.td),
+                    ctypes.c_float(float(scale) if scale is not None else q.shape[-1] ** -0.5), _ref(self.tw)),
+                   (ctypes.c_void_p(self.workspace.data_ptr()), ctypes.c_size_t(n)))
+
+    def __call__(self, stream=None):
+        self._launch(stream)
+        return self.out
+
+
+class Kv8Evict(_Call):
+    """acefa_kv8_evict: kept.shape[2] rows of each (set, head) of cache move to out, the first n_first, the last
+    n_recent and the largest of weight (sets, Hkv, n_max) f32.  kept (sets, Hkv, keep) int32, lens_out (sets) int32
+    and weight_out (sets, Hkv, keep) f32 or None are written."""
+
+    def __init__(self, cache, weight, lens, out, kept, lens_out, weight_out=None, n_first=0, n_recent=0):
+        n = cache.k.shape[0]
+        self.tw, self.tk, self.to = describe(weight), describe(kept), describe(weight_out)
+        keep = (*cache.tensors, weight, lens, *out.tensors, kept, lens_out)
+        self._bind("acefa_kv8_evict", keep + ((weight_out,) if weight_out is not None else ()),
+                   (ctypes.byref(cache.c), _ref(self.tw), _int32(lens, n, "lens"), int(n_first), int(n_recent),
+                    ctypes.byref(out.c), _ref(self.tk), _ref(self.to), _int32(lens_out, n, "lens_out")), ())
+        self.cache, self.out, self.kept = cache, out, kept
+
+    def __call__(self, stream=None):
+        self._launch(stream)
+        return self.out
+
+
+class PackedAttn(_Call):
+    """acefa_flash_attn_packed: q (Hq, rows, D), k, v (Hkv, rows_kv, D) f16 or bf16, sequences behind one another at
+    the offsets cu_q, cu_k (n_seq + 1) int32 (cu_k None: cu_q).  mask: 0, MASK_CAUSAL or MASK_WINDOW with window.
+    Returns out (rows, Hq, D), of q's type unless given (or f32)."""
+
+    def __init__(self, q, k, v, cu_q, cu_k=None, mask=0, window=0, scale=None, out=None):
+        if out is None:
+            out = torch.empty((q.shape[1], q.shape[0], q.shape[2]), dtype=q.dtype, device=q.device)
+        self.out = out
+        n = cu_q.shape[0] - 1
+        self.tq, self.tk, self.tv, self.td = describe(q), describe(k), describe(v), describe(out)
+        keep = (q, k, v, out, cu_q) + ((cu_k,) if cu_k is not None else ())
+        self._bind("acefa_flash_attn_packed", keep,
+                   (_ref(self.tq), _ref(self.tk), _ref(self.tv), _ref(self.td), _int32(cu_q, n + 1, "cu_q"),
+                    _int32(cu_k, n + 1, "cu_k") if cu_k is not None else None, n, int(mask), int(window),
+                    ctypes.c_float(float(scale) if scale is not None else q.shape[-1] ** -0.5)), ())
+
+    def __call__(self, stream=None):
+        self._launch(stream)
+        return self.out
+
+
+def _on(stream):
+    """Allocations and launches of a call made for one use belong to the stream given."""
+    return torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext()
+
+
+def kv8_store(cache, k_new, v_new, pos, cu_rows=None, stream=None):
+    return Kv8Store(cache, k_new, v_new, pos, cu_rows)(stream)
+
+
+def kv8_load(cache, lens, n=None, dtype=torch.float32, stream=None):
+    """k, v (sets, Hkv, n, D) of the cache's first n rows (default: all), zeros past lens."""
+    B, H, n_max, D = cache.k.shape
+    shape = (B, H, n if n is not None else n_max, D)
+    with _on(stream):
+        k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+        return Kv8Load(cache, lens, k, v)(stream)
+
+
+def kv8_attn(q, cache, lens, scale=None, weight=None, out=None, stream=None):
+    with _on(stream):
+        return Kv8Attn(q, cache, lens, scale=scale, weight=weight, out=out)(stream)
+
+
+def kv8_evict(cache, weight, lens, keep, n_first=0, n_recent=0, stream=None):
+    """Returns (cache of keep rows, kept, lens, weights) of the rows that stay."""
+    B, H, _, D = cache.k.shape
+    with _on(stream):
+        out = Kv8Cache.empty(keep, H, B, D, device=cache.k.device)
+        kept = torch.empty((B, H, keep), dtype=torch.int32, device=cache.k.device)
+        weight_out = torch.empty((B, H, keep), device=cache.k.device)
+        lens_out = torch.empty(B, dtype=torch.int32, device=cache.k.device)
+        Kv8Evict(cache, weight, lens, out, kept, lens_out, weight_out=weight_out, n_first=n_first,
+                 n_recent=n_recent)(stream)
+    return out, kept, lens_out, weight_out
+
+
+def flash_attn_packed(q, k, v, cu_q, cu_k=None, mask=0, window=0, scale=None, out=None, stream=None):
+    with _on(stream):
+        return PackedAttn(q, k, v, cu_q, cu_k, mask=mask, window=window, scale=scale, out=out)(stream)
 
 
 # input preparation helpers (torch ops; not on the attention path)

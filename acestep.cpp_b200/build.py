@@ -19,8 +19,9 @@ OUT = os.path.join(HERE, "libacefa.so")
 BUILD = os.path.join(HERE, "_build")
 
 SOURCES = ["fa_api.cu", "fa_decode.cu", "fa_dense.cu", "fa_noalloc.cu", "fa_peer.cu", "fa_prologue.cu",
-           "cfg_combine.cu"]
-HEADERS = ["fa_internal.h", "ptx.cuh", "q8.cuh", "rope_norm.cuh"]
+           "cfg_combine.cu", "fa_packed.cu", "kv8_api.cu",
+           "kv8_cache.cu", "kv8_attn.cu", "kv8_evict.cu"]
+HEADERS = ["fa_internal.h", "ptx.cuh", "q8.cuh", "rope_norm.cuh", "kv8_internal.h"]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -68,10 +68,6 @@ int dev_info(DevInfo **out) {
 }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no -lcuda).
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 EncodeTiledFn encode_fn() {
     static const EncodeTiledFn fn = [] {  // thread-safe one-time lookup
         void                           *p = nullptr;
@@ -424,6 +420,27 @@ bool encode_o_map(CUtensorMap *map, const acefa_tensor *d, int D, int G, int n_m
 }
 
 }  // namespace
+
+int device_ctx(DeviceCtx *ctx) {
+    DevInfo  *di = nullptr;
+    const int rc = dev_info(&di);
+    if (rc == ACEFA_OK) {
+        ctx->sm_count      = di->sm_count;
+        ctx->dev_err       = di->err_ptr;
+        ctx->wait_limit_ns = wait_limit_ns();
+    }
+    return rc;
+}
+
+void note_launches(int launches, int path) {
+    t_last_launches = launches;
+    if (path) {
+        t_last_path = path;
+    }
+}
+
+EncodeTiledFn tensor_map_encoder() { return encode_fn(); }
+
 }  // namespace acefa
 
 using namespace acefa;

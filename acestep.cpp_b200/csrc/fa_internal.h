@@ -221,6 +221,22 @@ size_t workspace_bytes_within(const acefa_tensor *q, const acefa_tensor *k, cons
 int kv_prologue_launch(const acefa_tensor *k_src, const acefa_tensor *v_src, const acefa_tensor *k_dst,
                        const acefa_tensor *v_dst, const RopeNorm &kp, int sm_count, cudaStream_t stream);
 
+// ------------------------------------------------------------------ host services of fa_api.cu
+struct DeviceCtx {
+    int      sm_count;
+    int     *dev_err;        // the device error word (DEVERR_*)
+    uint64_t wait_limit_ns;  // bound of every device-side wait
+};
+// The current device, checked to be sm_100: ACEFA_OK, _ERR_CUDA or _ERR_DEVICE.
+int device_ctx(DeviceCtx *ctx);
+// What acefa_last_launch_count() and, for path != 0, acefa_last_path() report.
+void note_launches(int launches, int path);
+// cuTensorMapEncodeTiled, or nullptr.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn tensor_map_encoder();
+
 // ------------------------------------------------------------------ CFG logit combine
 // Launch for arguments validated by acefa_cfg_logit_combine (fa_api.cu).
 int cfg_combine_launch(const float *cond, const float *uncond, int64_t row_stride, int n, int eos_idx,

@@ -1,0 +1,702 @@
+// kv8_attn.cu -- attention of a few query rows per KV head over the 8-bit
+// block-scaled cache (acefa_kv8_attn): split over the keys, merged by a second
+// launch, which also adds up the attention weights of each key.
+//
+// Mathematics.  With K = kd * k8 and V = vd * v8 (one kd, vd per 64 keys),
+//   s_rj = scale * kd_j * (q_r . k8_j),   p_rj = exp(s_rj - m_r),
+//   o_r  = sum_j vd_j p_rj v8_j / sum_j p_rj.
+// k8 and v8 are integers below 128, exact in F16.  q_r (scaled by a power of
+// two into F16's range) and p_rj are split into two F16 numbers each, which
+// together keep 22 bits, so that the F16 tensor-core products with F32 sums
+// lose nothing beside F32 arithmetic; the scales multiply in F32: kd on the
+// finished score, vd on the 16-key partial product of V.
+//
+// Work.  The (set, KV head, row block) units' 64-key tiles, numbered one after
+// another over all sets' actual lengths, are cut into equal runs, one per CTA:
+// ragged batches balance as well as even ones, and the grid depends on shapes
+// only.  A CTA's four warps take 16 keys of every tile each and never wait for
+// one another inside a unit.  Each thread copies (cp.async) exactly the bytes
+// that its MMA fragments need into its own shared-memory slots, several chunks
+// ahead, so the stream needs no barrier; the dims and keys of a fragment are
+// assigned such that these bytes are 16-B pieces of rows (dims are summed over
+// in any order, and V's dims are only named at the end).
+// Products run transposed (keys or dims are the MMA's M, the rows its N = 8):
+// S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
+// operand layout by four movmatrix.  The running maximum moves only when a
+// score exceeds it by more than 2^8 (a warp vote), as in the other kernels.
+#include "kv8_internal.h"
+#include "ptx.cuh"
+
+namespace acefa {
+namespace {
+
+constexpr int   kWarps   = 4;
+constexpr int   kThreads = 32 * kWarps;
+constexpr int   kChunk   = 16;  // keys of one warp and tile
+constexpr float kSlack   = 8.0f;
+static_assert(kWarps * kChunk == kKv8Block, "a tile is one block of the cache");
+
+// ring stages of a warp: bytes of one chunk = 2 * 16 * D plus one 4-byte
+// scale of K and V per lane
+template <int HD>
+constexpr int stage_bytes() {
+    return 2 * kChunk * HD + 256;
+}
+constexpr int kStages = 4;
+template <int HD, int NT>
+constexpr int merge_floats() {
+    return kWarps * 8 * NT * (HD + 4) + kWarps * 8 * NT * 2;
+}
+template <int HD, int NT>
+constexpr int attn_smem_bytes() {
+    return kWarps * kStages * stage_bytes<HD>() + 4 * merge_floats<HD, NT>() + 4 * (kKv8MaxSets + 4);
+}
+constexpr int ctas_per_sm(int HD, int NT) { return HD == 128 && NT == 2 ? 2 : 2; }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds_v4(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds_v2(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+// 8x8 b16 matrix spread over the warp (row = lane / 4, two columns each), transposed
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Two bytes of `biased` (int8 + 128, picked by sel) as f16: 0x6400 | b is
+// 1024 + b, and subtracting 1152 leaves the int8 value exactly.
+__device__ __forceinline__ uint32_t i8x2_f16(uint32_t biased, uint32_t sel) {
+    const uint32_t t = __byte_perm(biased, 0x64646464u, sel);
+    const __half2  v = __hsub2(*reinterpret_cast<const __half2 *>(&t), __half2half2(__ushort_as_half(0x6480u)));
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+// x = hi + lo as two f16 pairs, hi the rounded value
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2  f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi              = *reinterpret_cast<const uint32_t *>(&h);
+    lo              = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+__device__ __forceinline__ float load1(const char *p, int type, int e) {
+    return type == ACEFA_TYPE_F32   ? reinterpret_cast<const float *>(p)[e]
+           : type == ACEFA_TYPE_F16 ? __half2float(reinterpret_cast<const __half *>(p)[e])
+                                    : __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[e]);
+}
+__device__ __forceinline__ void store1(char *p, int type, int e, float x) {
+    if (type == ACEFA_TYPE_F32) {
+        reinterpret_cast<float *>(p)[e] = x;
+    } else if (type == ACEFA_TYPE_F16) {
+        reinterpret_cast<__half *>(p)[e] = __float2half_rn(x);
+    } else {
+        reinterpret_cast<__nv_bfloat16 *>(p)[e] = __float2bfloat16_rn(x);
+    }
+}
+
+// base[b] = 64-key tiles of the sets before b, b = 0 .. B (the last is the
+// total per head and row block).  All threads; ends with a barrier.
+__device__ __forceinline__ void tile_table(int *base, const int32_t *len, int B, int n_max) {
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+        int acc = 0;
+        for (int b0 = 0; b0 < B; b0 += 32) {
+            int v = b0 + lane < B ? (clamp_len(__ldg(len + b0 + lane), n_max) + kKv8Block - 1) / kKv8Block : 0;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, off);
+                v += lane >= off ? u : 0;
+            }
+            if (b0 + lane < B) {
+                base[b0 + lane + 1] = acc + v;
+            }
+            acc += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) {
+            base[0] = 0;
+        }
+    }
+    __syncthreads();
+}
+
+// Run of tiles of CTA c of C: [T * c / C, T * (c + 1) / C).  C <= T, so no run
+// is empty and the CTAs that meet a unit are consecutive.
+__device__ __forceinline__ int run_start(int T, int C, int c) { return (int) ((int64_t) T * c / C); }
+// the CTA whose run holds tile x
+__device__ __forceinline__ int cta_of(int T, int C, int x) { return (int) ((((int64_t) x + 1) * C - 1) / T); }
+
+// A position in the sequence of tiles.
+struct Walk {
+    int     b, ub, t, nt, len;  // set, unit of the set, tile of the unit, its tiles, the set's length
+    int64_t off_k, off_v;       // byte offsets of (head, set) in k and v
+    const float *ks, *vs;       // its scales
+};
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
+    kv8_attn_kernel(const __grid_constant__ Kv8AttnParams P) {
+    constexpr int R    = 8 * NT;
+    constexpr int KS   = HD / 16;             // k-steps of S, m-tiles of O
+    constexpr int kSt  = stage_bytes<HD>();
+    constexpr int kOut = HD + 4;              // floats between merged rows
+    extern __shared__ __align__(16) uint8_t smem[];
+    float *s_o    = reinterpret_cast<float *>(smem + kWarps * kStages * kSt);  // [warp][R][kOut]
+    float *s_ml   = s_o + kWarps * R * kOut;                                   // [warp][R][2]
+    int   *s_base = reinterpret_cast<int *>(s_ml + kWarps * R * 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, c = lane & 3;
+    const int HU = P.c.Hkv * P.n_rb;  // units of a set
+
+    pdl_wait_primary();
+    tile_table(s_base, P.len, P.c.B, P.c.n_max);
+    const int T = s_base[P.c.B] * HU;
+    const int C = min((int) gridDim.x, T);
+    pdl_launch_dependents();
+    if ((int) blockIdx.x >= C) {
+        return;
+    }
+    const int x0 = run_start(T, C, blockIdx.x), n_my = run_start(T, C, blockIdx.x + 1) - x0;
+
+    auto enter_unit = [&](Walk &w) {
+        const int hk = w.ub / P.n_rb;
+        w.off_k      = (int64_t) hk * P.c.k.nb2 + (int64_t) w.b * P.c.k.nb3;
+        w.off_v      = (int64_t) hk * P.c.v.nb2 + (int64_t) w.b * P.c.v.nb3;
+        w.ks         = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.k.scale) +
+                                               hk * P.c.k.s_nb2 + w.b * P.c.k.s_nb3);
+        w.vs         = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.v.scale) +
+                                               hk * P.c.v.s_nb2 + w.b * P.c.v.s_nb3);
+    };
+    auto enter_set = [&](Walk &w) {
+        w.nt  = s_base[w.b + 1] - s_base[w.b];
+        w.len = clamp_len(__ldg(P.len + w.b), P.c.n_max);
+    };
+    auto advance = [&](Walk &w) {  // true: a new unit
+        if (++w.t < w.nt) {
+            return false;
+        }
+        w.t = 0;
+        if (++w.ub == HU) {
+            w.ub = 0;
+            do {
+                ++w.b;
+            } while (w.b < P.c.B && s_base[w.b + 1] == s_base[w.b]);
+            if (w.b == P.c.B) {
+                return true;
+            }
+            enter_set(w);
+        }
+        enter_unit(w);
+        return true;
+    };
+    Walk at;
+    {
+        int lo = 0, hi = P.c.B;  // the set whose tiles hold x0: base[lo] * HU <= x0 < base[lo + 1] * HU
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_base[mid] * HU <= x0) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        at.b = lo;
+        enter_set(at);
+        const int off = x0 - s_base[lo] * HU;
+        at.ub         = off / at.nt;
+        at.t          = off % at.nt;
+        enter_unit(at);
+    }
+    Walk ahead = at;
+
+    const uint32_t ring = smem_u32(smem) + (uint32_t) (warp * kStages * kSt);
+    // Copies this thread's part of a chunk.  K: rows g and g + 8, 16-B pieces c
+    // (and 4 + c) of each.  V: HD / 8 dims from g * HD / 8 of rows 2c, 2c + 1, 2c + 8,
+    // 2c + 9.  Rows past the length repeat the last one (they get no weight).
+    auto issue = [&](int st) {
+        const int j0 = ahead.t * kKv8Block + warp * kChunk;
+        if (j0 < ahead.len) {
+            const uint32_t d    = ring + (uint32_t) (st * kSt) + (uint32_t) lane * 16;
+            const int      last = ahead.len - 1;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int8_t *p = P.c.k.q + ahead.off_k + (int64_t) min(j0 + g + 8 * r, last) * P.c.k.nb1 + 16 * c;
+#pragma unroll
+                for (int e = 0; e < HD / 64; ++e) {
+                    cp16(d + (uint32_t) ((r * (HD / 64) + e) * 512), p + 64 * e);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int     j = j0 + 2 * c + (r & 1) + 8 * (r >> 1);
+                const int8_t *p = P.c.v.q + ahead.off_v + (int64_t) min(j, last) * P.c.v.nb1 + (HD / 8) * g;
+                if constexpr (HD == 128) {
+                    cp16(d + (uint32_t) (2048 + r * 512), p);
+                } else {
+                    cp8(ring + (uint32_t) (st * kSt + 1024 + r * 256 + lane * 8), p);
+                }
+            }
+            const uint32_t sc = ring + (uint32_t) (st * kSt + 2 * kChunk * HD + lane * 4);
+            cp4(sc, ahead.ks + ahead.t);
+            cp4(sc + 128, ahead.vs + ahead.t);
+        }
+    };
+
+    // ---- rows of the current unit
+    uint32_t qh[NT][KS][2], ql[NT][KS][2];  // Q^T operand, high and low halves
+    float    mul[NT][2];                    // log2-unit score per unit of accumulator, rows 2c and 2c + 1
+    int      lim[NT][2];                    // keys those rows see
+    float    acc_o[NT][KS][4];
+    float    m[NT][2], l[NT][2];
+    auto load_rows = [&]() {
+        const int hk = at.ub / P.n_rb, rb = at.ub % P.n_rb;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int   row = rb * R + nt * 8 + g;
+            float       x[KS][4];
+            float       top = 0.0f;
+            const bool  on  = row < P.rows;
+            const char *p   = P.q.data;
+            if (on) {
+                p += (int64_t) (row / P.G) * P.q.nb1 + (int64_t) (hk * P.G + row % P.G) * P.q.nb2 +
+                     (int64_t) at.b * P.q.nb3;
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                // word ks of this thread's K pieces: dims 64 * (ks / 4) + 16 * c + 4 * (ks % 4) ..
+                const int d = 64 * (ks >> 2) + 16 * c + 4 * (ks & 3);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[ks][e] = on ? load1(p, P.q.type, d + e) : 0.0f;
+                    top      = fmaxf(top, fabsf(x[ks][e]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // 2^k brings the row's largest value into [2^13, 2^14): far below
+            // F16's largest, and small values keep their bits in the low half
+            const int ex = (int) (__float_as_uint(top) >> 23);
+            const int k  = top > 0.0f && ex < 255 ? min(140 - ex, 126) : 0;
+            const float f = __uint_as_float((uint32_t) (127 + k) << 23);
+            const float u = P.scale_log2 * __uint_as_float((uint32_t) (127 - k) << 23);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                split2(x[ks][0] * f, x[ks][1] * f, qh[nt][ks][0], ql[nt][ks][0]);
+                split2(x[ks][2] * f, x[ks][3] * f, qh[nt][ks][1], ql[nt][ks][1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mul[nt][e]    = __shfl_sync(0xffffffffu, u, (2 * c + e) * 4);
+                const int rr  = rb * R + nt * 8 + 2 * c + e;
+                lim[nt][e]    = rr < P.rows ? at.len - (P.n_q - 1 - rr / P.G) : 0;
+                m[nt][e]      = -INFINITY;
+                l[nt][e]      = 0.0f;
+            }
+#pragma unroll
+            for (int t = 0; t < KS; ++t) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc_o[nt][t][e] = 0.0f;
+                }
+            }
+        }
+    };
+
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (i < n_my) {
+            issue(i);
+            advance(ahead);
+        }
+        cp_commit();
+    }
+    load_rows();
+
+#pragma unroll 1
+    for (int i = 0; i < n_my; ++i) {
+        if (i + kStages - 1 < n_my) {
+            issue((i + kStages - 1) % kStages);
+            advance(ahead);
+        }
+        cp_commit();
+        cp_wait<kStages - 1>();
+        const int j0 = at.t * kKv8Block + warp * kChunk;
+        if (j0 < at.len) {  // uniform over the warp
+            const uint32_t d  = ring + (uint32_t) ((i % kStages) * kSt);
+            const uint32_t dl = d + (uint32_t) lane * 16;
+            const float    kd = lds_f32(d + 2 * kChunk * HD + lane * 4);
+            const float    vd = lds_f32(d + 2 * kChunk * HD + 128 + lane * 4);
+            // ---- S^T = K Q^T
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[nt][e] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int e4 = 0; e4 < HD / 64; ++e4) {
+                const uint4    wa    = lds_v4(dl + (uint32_t) (e4 * 512));
+                const uint4    wb    = lds_v4(dl + (uint32_t) ((HD / 64 + e4) * 512));
+                const uint32_t va[4] = {wa.x, wa.y, wa.z, wa.w}, vb[4] = {wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t ba = va[e] ^ 0x80808080u, bb = vb[e] ^ 0x80808080u;
+                    const uint32_t a[4] = {i8x2_f16(ba, 0x4140u), i8x2_f16(bb, 0x4140u), i8x2_f16(ba, 0x4342u),
+                                           i8x2_f16(bb, 0x4342u)};
+                    const int      ks   = 4 * e4 + e;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16816<false>(s[nt], a, qh[nt][ks][0], qh[nt][ks][1]);
+                        mma_16816<false>(s[nt], a, ql[nt][ks][0], ql[nt][ks][1]);
+                    }
+                }
+            }
+            // ---- scores in log2 units, masked; s[nt]: (key g, rows 2c 2c+1), (key g + 8, same rows)
+            bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = j0 + g + 8 * (e >> 1);
+                    const float v = s[nt][e] * (mul[nt][e & 1] * kd);
+                    s[nt][e]      = j < lim[nt][e & 1] ? v : -INFINITY;
+                    grow |= s[nt][e] > m[nt][e & 1] + kSlack;
+                }
+            }
+            if (P.scores) {
+                float *sp = P.scores + ((int64_t) (at.b * HU + at.ub) * P.c.n_max + j0) * P.score_stride;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (nt * 8 + 2 * c < P.score_stride && j0 + g + 8 * e < at.len) {
+                            *reinterpret_cast<float2 *>(sp + (int64_t) (g + 8 * e) * P.score_stride + nt * 8 + 2 * c) =
+                                make_float2(s[nt][2 * e], s[nt][2 * e + 1]);
+                        }
+                    }
+                }
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(s[nt][e], s[nt][2 + e]);
+                        top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float mn = fmaxf(m[nt][e], top);
+                        const float f  = mn == -INFINITY ? 1.0f : exp2f(m[nt][e] - mn);
+                        m[nt][e]       = mn;
+                        l[nt][e] *= f;
+#pragma unroll
+                        for (int t = 0; t < KS; ++t) {
+                            acc_o[nt][t][e] *= f;
+                            acc_o[nt][t][2 + e] *= f;
+                        }
+                    }
+                }
+            }
+            // ---- P, its operand halves
+            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mu = m[nt][e & 1];
+                    p[e]           = exp2f(s[nt][e] - (mu == -INFINITY ? 0.0f : mu));
+                    l[nt][e & 1] += p[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t hi, lo;
+                    split2(p[2 * e], p[2 * e + 1], hi, lo);
+                    ph[nt][e] = movmatrix_trans(hi);
+                    pl[nt][e] = movmatrix_trans(lo);
+                }
+            }
+            // ---- O^T += vd * V^T P^T.  m-tile t: dims g * HD / 8 + 2t (row g) and + 2t + 1 (row g + 8)
+            uint32_t v[4][HD / 32];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (HD == 128) {
+                    const uint4 w = lds_v4(dl + (uint32_t) (2048 + r * 512));
+                    v[r][0] = w.x, v[r][1] = w.y, v[r][2] = w.z, v[r][3] = w.w;
+                } else {
+                    const uint2 w = lds_v2(d + (uint32_t) (1024 + r * 256 + lane * 8));
+                    v[r][0] = w.x, v[r][1] = w.y;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < KS; ++t) {
+                const uint32_t sel = (t & 1) ? 0x7362u : 0x5140u;
+                const uint32_t z0  = __byte_perm(v[0][t >> 1], v[1][t >> 1], sel) ^ 0x80808080u;
+                const uint32_t z1  = __byte_perm(v[2][t >> 1], v[3][t >> 1], sel) ^ 0x80808080u;
+                const uint32_t a[4] = {i8x2_f16(z0, 0x4140u), i8x2_f16(z0, 0x4342u), i8x2_f16(z1, 0x4140u),
+                                       i8x2_f16(z1, 0x4342u)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_16816<false>(o, a, ph[nt][0], ph[nt][1]);
+                    mma_16816<false>(o, a, pl[nt][0], pl[nt][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        acc_o[nt][t][e] = fmaf(o[e], vd, acc_o[nt][t][e]);
+                    }
+                }
+            }
+        }
+        // ---- end of the unit (or of this CTA's run): merge the warps' results
+        const int  unit = at.b * HU + at.ub;
+        const int  rb   = at.ub % P.n_rb;
+        const bool next = advance(at);
+        if (next || i + 1 == n_my) {
+            __syncthreads();  // the previous merge has been read
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float sum = l[nt][e];
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                    const int row = nt * 8 + 2 * c + e;
+                    if (g == 0) {
+                        s_ml[(warp * R + row) * 2]     = m[nt][e];
+                        s_ml[(warp * R + row) * 2 + 1] = sum;
+                    }
+                    // element e of the accumulators is dim 2t of row 2c + e, element 2 + e dim 2t + 1
+                    float *o = s_o + (warp * R + row) * kOut + g * (HD / 8);
+#pragma unroll
+                    for (int t = 0; t < KS; t += 2) {
+                        *reinterpret_cast<float4 *>(o + 2 * t) = make_float4(
+                            acc_o[nt][t][e], acc_o[nt][t][2 + e], acc_o[nt][t + 1][e], acc_o[nt][t + 1][2 + e]);
+                    }
+                }
+            }
+            __syncthreads();
+            const int n_row = min(R, P.rows - rb * R);
+            float    *slot  = P.part + (int64_t) (blockIdx.x + unit) * (R * (HD + 2));
+            for (int x = threadIdx.x; x < n_row * (HD / 4); x += kThreads) {
+                const int row = x / (HD / 4), d4 = x % (HD / 4);
+                float     mw[kWarps], M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    mw[w] = s_ml[(w * R + row) * 2];
+                    M     = fmaxf(M, mw[w]);
+                }
+                const float Mu = M == -INFINITY ? 0.0f : M;
+                float       L  = 0.0f;
+                float4      o  = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float  f = exp2f(mw[w] - Mu);
+                    const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * R + row) * kOut + 4 * d4);
+                    L += s_ml[(w * R + row) * 2 + 1] * f;
+                    o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+                }
+                *reinterpret_cast<float4 *>(slot + row * HD + 4 * d4) = o;
+                if (d4 == 0) {
+                    slot[R * HD + row]     = M;
+                    slot[R * HD + R + row] = L;
+                }
+            }
+            if (i + 1 < n_my) {
+                load_rows();
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The second launch.  CTAs below n_out finish one row each: O = sum of the
+// partials, each times 2^(m - M), over their summed l.  The others add the
+// weights of 1024 keys of a (set, KV head): p = 2^(s - M) / L summed over the
+// head's rows, whose M and L come from the same partials.  Every sum has a
+// fixed order, so results do not depend on scheduling.
+constexpr int kSumThreads = 128;
+constexpr int kSumKeys    = 1024;
+
+template <int HD>
+__global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_constant__ Kv8AttnParams P, int R,
+                                                                   int n_out, int key_chunks) {
+    __shared__ int    s_base[kKv8MaxSets + 4];
+    __shared__ float  s_lse[ACEFA_KV8_MAX_ROWS];
+    __shared__ float4 s_o[4][HD / 4];
+    const int slot_f = R * (HD + 2);
+    const int HU     = P.c.Hkv * P.n_rb;
+    pdl_wait_primary();
+    tile_table(s_base, P.len, P.c.B, P.c.n_max);
+    const int T = s_base[P.c.B] * HU, C = min(P.n_cta, T);
+    // the CTAs of the split kernel that met a unit: slots (c + unit), c0 <= c <= c1
+    auto range_of = [&](int b, int ub, int &c0, int &c1) {
+        const int nt = s_base[b + 1] - s_base[b];
+        const int a  = s_base[b] * HU + ub * nt;
+        c0 = nt ? cta_of(T, C, a) : 0;
+        c1 = nt ? cta_of(T, C, a + nt - 1) : -1;
+    };
+    if ((int) blockIdx.x < n_out) {
+        const int row = blockIdx.x % P.rows, bh = blockIdx.x / P.rows;
+        const int hk = bh % P.c.Hkv, b = bh / P.c.Hkv;
+        const int ub = hk * P.n_rb + row / R, r = row % R;
+        int       c0, c1;
+        range_of(b, ub, c0, c1);
+        const float *base = P.part + (int64_t) (b * HU + ub) * slot_f;
+        float        M    = -INFINITY;
+        for (int k = c0; k <= c1; ++k) {
+            M = fmaxf(M, __ldcg(base + (int64_t) k * slot_f + R * HD + r));
+        }
+        const float Mu = M == -INFINITY ? 0.0f : M;
+        const int   w = threadIdx.x / (HD / 4), d4 = threadIdx.x % (HD / 4);
+        constexpr int W = kSumThreads / (HD / 4);  // slots summed side by side
+        float4      o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float       L = 0.0f;
+#pragma unroll 4
+        for (int k = c0 + w; k <= c1; k += W) {
+            const float *sl = base + (int64_t) k * slot_f;
+            const float  f  = exp2f(__ldcg(sl + R * HD + r) - Mu);
+            const float4 v  = __ldcg(reinterpret_cast<const float4 *>(sl + r * HD) + d4);
+            L = fmaf(__ldcg(sl + R * HD + R + r), f, L);
+            o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+        }
+        __shared__ float s_l[8];
+        for (int half = W / 2; half; half >>= 1) {
+            if (w >= half && w < 2 * half) {
+                s_o[w - half][d4] = o;
+                if (d4 == 0) {
+                    s_l[w - half] = L;
+                }
+            }
+            __syncthreads();
+            if (w < half) {
+                const float4 v = s_o[w][d4];
+                o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+                L += s_l[w];
+            }
+            __syncthreads();
+        }
+        if (w == 0) {
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            char *p = P.dst.data + (int64_t) (hk * P.G + row % P.G) * P.dst.nb1 + (int64_t) (row / P.G) * P.dst.nb2 +
+                      (int64_t) b * P.dst.nb3;
+            store1(p, P.dst.type, 4 * d4, o.x * inv);
+            store1(p, P.dst.type, 4 * d4 + 1, o.y * inv);
+            store1(p, P.dst.type, 4 * d4 + 2, o.z * inv);
+            store1(p, P.dst.type, 4 * d4 + 3, o.w * inv);
+        }
+        return;
+    }
+    const int x = (int) blockIdx.x - n_out;
+    const int bh = x / key_chunks, j0 = x % key_chunks * kSumKeys;
+    const int hk = bh % P.c.Hkv, b = bh / P.c.Hkv;
+    const int len = clamp_len(__ldg(P.len + b), P.c.n_max);
+    if (j0 >= len) {
+        return;
+    }
+    for (int row = threadIdx.x; row < P.rows; row += kSumThreads) {
+        const int ub = hk * P.n_rb + row / R, r = row % R;
+        int       c0, c1;
+        range_of(b, ub, c0, c1);
+        const float *base = P.part + (int64_t) (b * HU + ub) * slot_f + R * HD + r;
+        float        M    = -INFINITY;
+        for (int k = c0; k <= c1; ++k) {
+            M = fmaxf(M, __ldcg(base + (int64_t) k * slot_f));
+        }
+        const float Mu = M == -INFINITY ? 0.0f : M;
+        float       L  = 0.0f;
+        for (int k = c0; k <= c1; ++k) {
+            L = fmaf(__ldcg(base + (int64_t) k * slot_f + R), exp2f(__ldcg(base + (int64_t) k * slot_f) - Mu), L);
+        }
+        s_lse[row] = L == 0.0f ? INFINITY : Mu + log2f(L);  // an empty row weighs nothing
+    }
+    __syncthreads();
+    float *wp = reinterpret_cast<float *>(P.weight + (int64_t) hk * P.w_nb2 + (int64_t) b * P.w_nb3);
+    for (int j = j0 + threadIdx.x; j < min(len, j0 + kSumKeys); j += kSumThreads) {
+        float sum = 0.0f;
+        for (int rb = 0; rb < P.n_rb; ++rb) {
+            const float *sp =
+                P.scores + ((int64_t) (b * HU + hk * P.n_rb + rb) * P.c.n_max + j) * P.score_stride;
+            const int n_row = min(R, P.rows - rb * R);
+            for (int r = 0; r < n_row; ++r) {
+                sum += exp2f(__ldcg(sp + r) - s_lse[rb * R + r]);
+            }
+        }
+        wp[j] += sum;
+    }
+}
+
+template <int HD, int NT>
+cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
+    constexpr int          smem = attn_smem_bytes<HD, NT>();
+    static thread_local int configured = -1;
+    int                     dev        = 0;
+    cudaGetDevice(&dev);
+    if (configured != dev) {
+        cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        configured = dev;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim            = dim3((unsigned) p.n_cta);
+    cfg.blockDim           = dim3(kThreads);
+    cfg.dynamicSmemBytes   = smem;
+    cfg.stream             = s;
+    cfg.attrs              = attr;
+    cfg.numAttrs           = 1;
+    cudaError_t e          = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT>, p);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    const int n_out      = p.c.B * p.c.Hkv * p.rows;
+    const int key_chunks = (p.c.n_max + kSumKeys - 1) / kSumKeys;
+    cfg.gridDim          = dim3((unsigned) (n_out + (p.weight ? p.c.B * p.c.Hkv * key_chunks : 0)));
+    cfg.blockDim         = dim3(kSumThreads);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, kv8_attn_sum_kernel<HD>, p, 8 * NT, n_out, key_chunks);
+}
+
+}  // namespace
+
+int kv8_attn_ctas_per_sm(int D, int unit_rows) { return ctas_per_sm(D, unit_rows / 8); }
+
+cudaError_t launch_kv8_attn(const Kv8AttnParams &p, cudaStream_t s) {
+    const bool wide = kv8_unit_rows(p.rows) == 16;
+    return p.c.D == 128 ? (wide ? launch<128, 2>(p, s) : launch<128, 1>(p, s))
+                        : (wide ? launch<64, 2>(p, s) : launch<64, 1>(p, s));
+}
+
+}  // namespace acefa

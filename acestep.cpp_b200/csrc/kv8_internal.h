@@ -1,0 +1,207 @@
+// kv8_internal.h -- parameter blocks and device helpers shared by the kernels
+// of the 8-bit block-scaled KV cache (acefa_kv8_*).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fa_internal.h"
+
+namespace acefa {
+
+constexpr int kKv8Block   = ACEFA_KV8_BLOCK;     // tokens that share a scale
+constexpr int kKv8MaxSets = ACEFA_KV8_MAX_SETS;  // sets of a cache
+
+// One of K and V of a cache, after validation.  Strides in bytes.
+struct Kv8Side {
+    int8_t *q;      // rows of D values
+    float  *scale;  // one per block
+    int64_t nb1, nb2, nb3;    // row, head, set
+    int64_t s_nb2, s_nb3;     // scales: head, set (blocks are contiguous)
+};
+struct Kv8Dev {
+    Kv8Side k, v;
+    int     D, n_max, Hkv, B;
+};
+
+// An F32 / F16 / BF16 tensor [D, rows, H, B] read or written by the kernels.
+struct Kv8Rows {
+    char   *data;
+    int64_t nb1, nb2, nb3;
+    int     type;
+};
+
+struct Kv8StoreParams {
+    Kv8Dev         c;
+    Kv8Rows        k_new, v_new;  // nb3 unused
+    int64_t        rows;          // rows of k_new
+    const int32_t *cu;            // or nullptr: rows / B each
+    const int32_t *pos;
+    int           *dev_err;
+};
+struct Kv8LoadParams {
+    Kv8Dev         c;
+    Kv8Rows        k, v;
+    int            n;  // rows of the destination
+    const int32_t *len;
+};
+struct Kv8AttnParams {
+    Kv8Dev         c;
+    Kv8Rows        q, dst;  // q: nb1 = query, nb2 = head; dst: nb1 = head, nb2 = query
+    const int32_t *len;
+    char          *weight;  // F32 [n_max, Hkv, B] or nullptr
+    int64_t        w_nb2, w_nb3;
+    int            n_q, G, rows;  // rows = G * n_q per kv head
+    int            n_rb;          // row blocks per (set, kv head)
+    int            n_cta;         // CTAs of the split kernel
+    float          scale_log2;    // scale * log2(e)
+    float         *part;          // partial results, one slot per (CTA, unit) that meet
+    float         *scores;        // [unit][n_max][score_stride] log2-unit scores, with weights only
+    int            score_stride;
+};
+struct Kv8EvictParams {
+    Kv8Dev         c, out;
+    const char    *weight;  // F32 [n_max, Hkv, B]
+    int64_t        w_nb2, w_nb3;
+    const int32_t *len;
+    int            n_first, n_recent, keep;
+    char          *kept;  // I32 [keep, Hkv, B]
+    int64_t        k_nb2, k_nb3;
+    char          *weight_out;  // F32 or nullptr
+    int64_t        wo_nb2, wo_nb3;
+    int32_t       *len_out;
+};
+
+cudaError_t launch_kv8_store(const Kv8StoreParams &p, cudaStream_t s);
+cudaError_t launch_kv8_load(const Kv8LoadParams &p, cudaStream_t s);
+cudaError_t launch_kv8_attn(const Kv8AttnParams &p, cudaStream_t s);
+cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s);
+
+// Rows of a unit of the attention kernel (8 or 16) and the CTAs that it may
+// keep resident on one SM; functions of the operands alone.
+inline int kv8_unit_rows(int rows) { return rows <= 8 ? 8 : 16; }
+int        kv8_attn_ctas_per_sm(int D, int unit_rows);
+inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows * (D + 2); }
+
+// ------------------------------------------------------------------ device helpers
+#ifdef __CUDACC__
+
+// Finds item x among the items of n segments, count(i) of segment i in their
+// order.  The whole warp calls it with the same arguments and gets the same
+// answer: the segment and the item's number in it, or false behind the last.
+template <class F>
+__device__ __forceinline__ bool find_item(int n, int64_t x, F count, int &seg, int &item) {
+    const int lane = threadIdx.x & 31;
+    int64_t   acc  = 0;
+    for (int base = 0; base < n; base += 32) {
+        const int mine = base + lane < n ? count(base + lane) : 0;
+        int64_t   incl = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, incl, off);
+            incl += lane >= off ? v : 0;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, x < acc + incl);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            seg         = base + l;
+            item        = (int) (x - acc - __shfl_sync(0xffffffffu, incl - mine, l));
+            return true;
+        }
+        acc += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return false;
+}
+
+__device__ __forceinline__ int clamp_len(int len, int n_max) { return len < 0 ? 0 : (len > n_max ? n_max : len); }
+
+// max that keeps a NaN of either side
+__device__ __forceinline__ float max_nan(float a, float b) { return a != a || b != b ? NAN : fmaxf(a, b); }
+
+// x / d rounded to the nearest integer, ties to even, as if the quotient were
+// exact, clamped to 127.  Rounding is monotonic, so rounding the F32 quotient
+// t can only differ where t landed on a half-integer h; there the sign of
+// x - h * d (one FMA: h * d is exact inside it) says on which side of h the
+// true quotient lies.  d > 0 and finite; the result is 0 for d == 0.
+__device__ __forceinline__ int quant_rne(float x, float d) {
+    const float t = __fdiv_rn(x, d);
+    float       q = rintf(t);
+    if (fabsf(t - truncf(t)) == 0.5f) {
+        const float r = fmaf(-t, d, x);
+        if (r != 0.0f) {
+            q = r > 0.0f ? ceilf(t) : floorf(t);
+        }
+    }
+    q = fminf(fmaxf(q, -127.0f), 127.0f);
+    return d > 0.0f ? __float2int_rn(q) : 0;  // NaN converts to 0
+}
+
+// q * d_old / d_new rounded once to the nearest integer, ties to even, for
+// |q| <= 127 and d_old <= d_new, with ratio = d_old / d_new in F32.  The F32
+// product is off by at most 127 * 2^-23 < 2^-15; within that of a half-integer
+// the quotient is formed in F64, where q * d_old is exact and the division
+// rounds correctly (a tie is then a tie, and nothing else is within 2^-40 of one).
+__device__ __forceinline__ int requant_rne(int q, float d_old, float d_new, float ratio) {
+    const float t = (float) q * ratio;
+    const float r = rintf(t);
+    if (fabsf(fabsf(t - r) - 0.5f) <= 3.0517578125e-5f) {
+        return (int) rint(__ddiv_rn((double) q * (double) d_old, (double) d_new));
+    }
+    return __float2int_rn(r);
+}
+
+// Four int8 values of a 32-bit word moved from scale d_old to d_new.
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float d_old, float d_new, float ratio) {
+    uint32_t o = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int q = (int) (int8_t) (w >> (8 * e));
+        o |= (uint32_t) (requant_rne(q, d_old, d_new, ratio) & 0xFF) << (8 * e);
+    }
+    return o;
+}
+
+// Four consecutive values of a row of type T at element e0, as F32.
+template <class T>
+__device__ __forceinline__ float4 load4(const char *row, int e0, bool vec) {
+    const T *p = reinterpret_cast<const T *>(row) + e0;
+    if constexpr (sizeof(T) == 4) {
+        return vec ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(p[0], p[1], p[2], p[3]);
+    } else {
+        alignas(8) T v[4];
+        if (vec) {
+            *reinterpret_cast<uint2 *>(v) = __ldcs(reinterpret_cast<const uint2 *>(p));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = p[e];
+            }
+        }
+        return make_float4((float) v[0], (float) v[1], (float) v[2], (float) v[3]);
+    }
+}
+template <class T>
+__device__ __forceinline__ void store4(char *row, int e0, float4 x, bool vec) {
+    T *p = reinterpret_cast<T *>(row) + e0;
+    if constexpr (sizeof(T) == 4) {
+        if (vec) {
+            __stcs(reinterpret_cast<float4 *>(p), x);
+        } else {
+            p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
+        }
+    } else {
+        alignas(8) T v[4] = {(T) x.x, (T) x.y, (T) x.z, (T) x.w};
+        if (vec) {
+            __stcs(reinterpret_cast<uint2 *>(p), *reinterpret_cast<uint2 *>(v));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = v[e];
+            }
+        }
+    }
+}
+
+#endif  // __CUDACC__
+
+}  // namespace acefa

@@ -43,6 +43,8 @@ typedef enum acefa_type {
     ACEFA_TYPE_F32  = 0,
     ACEFA_TYPE_F16  = 1,
     ACEFA_TYPE_Q8_0 = 8,
+    ACEFA_TYPE_I8   = 24,
+    ACEFA_TYPE_I32  = 26,
     ACEFA_TYPE_BF16 = 30,
 } acefa_type;
 
@@ -316,6 +318,141 @@ ACEFA_API int acefa_cfg_logit_combine(const float *cond, const float *uncond, in
                                       int eos_idx, int code_offset, int code_count, float cfg_scale,
                                       float *compact, void *stream);
 
+/* ------------------------------------------------------------------------
+ * A KV cache held in 8 bits with one scale per block of 64 tokens and head.
+ * No counterpart in the reference, whose cache is F16 (src/qwen3-lm.h:228-229);
+ * it takes the place of one layer's F16 K and V ([D, n_max, Hkv, n_sets]) at
+ * a little over half the bytes.  Row j of (head h, set s) stands for the values
+ *   k[d, j, h, s] * k_scale[j / 64, h, s]         (each product rounded to F32)
+ * and likewise for v.  k, v: I8 [D, n_max, Hkv, Bk], D 64 or 128, nb[0] == 1,
+ * data and nb[1..3] multiples of 16 bytes; k_scale, v_scale: F32
+ * [ceil(n_max / 64), Hkv, Bk], nb[0] == 4.  1 <= Bk <= ACEFA_KV8_MAX_SETS,
+ * Hkv <= 4096.  A cache needs no initialisation: rows at or past a set's
+ * length are never read as values.
+ *
+ * Every array of lengths, positions or offsets below is device memory that the
+ * kernels read, so a captured CUDA graph replays with new lengths.  The
+ * entries launch on `stream` only, allocate nothing and never synchronise.
+ */
+#define ACEFA_KV8_BLOCK    64
+#define ACEFA_KV8_MAX_SETS 1024
+typedef struct acefa_kv8_cache {
+    acefa_tensor k, v;             /* I8  [D, n_max, Hkv, Bk] */
+    acefa_tensor k_scale, v_scale; /* F32 [ceil(n_max / 64), Hkv, Bk] */
+} acefa_kv8_cache;
+
+/*
+ * Stores new rows: a decode step's one row per set, or whole prompts.
+ *   k_new, v_new  [D, rows, Hkv, 1], both F32, F16 or BF16, nb[0] = the element
+ *                 size: the sets' new rows behind one another
+ *   cu_rows       int32 [Bk + 1], device: set s's rows are cu_rows[s] ..
+ *                 cu_rows[s + 1] - 1; NULL: rows / Bk rows for every set
+ *   pos           int32 [Bk], device: the cache row of set s's first new row;
+ *                 its length becomes pos[s] + its number of new rows
+ * A block's scale is d = amax / 127 (F32 division) of its new rows, and where
+ * rows before pos[s] stay in the block not below the scale they have.  New
+ * values become x / d rounded to the nearest integer, ties to even (0 where
+ * d is 0); where d grew, the rows that stay are rounded again: q * d_old / d.
+ * Both quotients are rounded once, exactly.  A NaN or an infinity among the
+ * new rows makes their block's scale NaN.  Rows of the last block behind the
+ * new length are left as they are.  A set whose rows are no rows of the
+ * cache or of k_new (a negative pos, an end past n_max, offsets that
+ * decrease or leave [0, rows]) is left unwritten and raises device error 5
+ * (acefa_device_error()).  k_new and v_new must not overlap the cache.
+ */
+ACEFA_API int acefa_kv8_store(const acefa_kv8_cache *cache, const acefa_tensor *k_new, const acefa_tensor *v_new,
+                              const int32_t *cu_rows, const int32_t *pos, void *stream);
+
+/*
+ * Reads the cache back as values: k_dst, v_dst [D, n, Hkv, Bk], n <= n_max,
+ * both F32, F16 or BF16, nb[0] = the element size, receive rows 0 .. n - 1 of
+ * every set; rows at or past len[s] (int32 [Bk], device) become zeros.
+ * E.g. a cached prefix for a dense attention call, or a cache to be saved.
+ */
+ACEFA_API int acefa_kv8_load(const acefa_kv8_cache *cache, const int32_t *len, const acefa_tensor *k_dst,
+                             const acefa_tensor *v_dst, void *stream);
+
+/*
+ * Attention of a few new tokens per set over the cache (a decode step, or a
+ * handful of drafted tokens), after their rows were stored.
+ *   q       [D, n_q, Hq, Bk] F32, F16 or BF16, nb[0] = the element size;
+ *           Hq % Hkv == 0 and n_q * Hq / Hkv <= ACEFA_KV8_MAX_ROWS (longer
+ *           prompts: acefa_flash_attn_packed on their own K and V)
+ *   len     int32 [Bk], device: rows in each set, the new ones included
+ *           (values outside [0, n_max] count as the nearer bound)
+ *   dst     [D, Hq, n_q, Bk] F32, F16 or BF16, nb[0] = the element size
+ *   weight  F32 [n_max, Hkv, Bk], nb[0] == 4, or NULL
+ * Query i sees rows j < len - (n_q - 1 - i) of its set.  dst = softmax(scale *
+ * q k^T) v; a query that sees nothing gives 0.  With `weight`, weight[j, h, s]
+ * grows by the softmax weights of row j summed over the n_q * Hq / Hkv
+ * queries of its head -- what acefa_kv8_evict goes by; rows at or past
+ * len[s] are left alone.  Q, the weights and the sums are held in F32
+ * precision throughout: the cache's rounding is the only one in 8 bits.
+ * Results do not depend on the order in which the GPU runs the blocks.
+ * workspace: acefa_kv8_attn_workspace_bytes(), 256-B aligned, no
+ * initialisation; a function of shapes and the device only.  Calls that may
+ * overlap on the GPU need a workspace each.
+ */
+#define ACEFA_KV8_MAX_ROWS 64
+ACEFA_API int acefa_kv8_attn(const acefa_tensor *q, const acefa_kv8_cache *cache, const int32_t *len,
+                             const acefa_tensor *dst, float scale, const acefa_tensor *weight, void *stream,
+                             void *workspace, size_t workspace_bytes);
+/* 0 for operands that acefa_kv8_attn refuses, or without a device. */
+ACEFA_API size_t acefa_kv8_attn_workspace_bytes(const acefa_tensor *q, const acefa_kv8_cache *cache,
+                                                const acefa_tensor *weight);
+
+/*
+ * Eviction: each (head, set) of `cache` keeps `keep` = kept->ne[0] of its rows
+ * in `out`, in their order.
+ *   weight      F32 [n_max, Hkv, Bk]: accumulated attention weights
+ *   len         int32 [Bk], device: rows in each set
+ *   n_first, n_recent  the first and the last rows that are kept whatever
+ *               their weight (n_first + n_recent <= keep)
+ *   out         the smaller cache, keep <= its n_max, same D, Hkv and Bk; must
+ *               not overlap `cache`
+ *   kept        I32 [keep, Hkv, Bk], nb[0] == 4: the kept rows, ascending
+ *   weight_out  F32 [keep, Hkv, Bk], nb[0] == 4, or NULL: their weights
+ *   len_out     int32 [Bk], device: min(len, keep)
+ * The other places go to the largest weights, equal ones to the lower row
+ * (-0 equals 0; a NaN ranks below every number).  A set of at most keep rows
+ * keeps them all.  A block of `out` takes the largest scale of the rows that
+ * come into it; rows of that scale move unchanged, the others become
+ * q * d_old / d rounded once to the nearest integer, ties to even.  Behind
+ * len_out, up to keep, `kept` is -1 and rows, their blocks' scales and
+ * weight_out are 0.
+ */
+ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *weight, const int32_t *len,
+                              int64_t n_first, int64_t n_recent, const acefa_kv8_cache *out,
+                              const acefa_tensor *kept, const acefa_tensor *weight_out, int32_t *len_out,
+                              void *stream);
+
+/*
+ * Attention of whole sequences packed behind one another: the prompts of
+ * several requests, or the texts of several captions, in one call with no
+ * padding.  The reference prefills one sequence per call
+ * (src/pipeline-lm.cpp:317-344).
+ *   q     [D, rows_q,  Hq,  1] F16 or BF16, D 64 or 128
+ *   k, v  [D, rows_kv, Hkv, 1] of q's type; Hq % Hkv == 0
+ *   dst   [D, Hq, rows_q, 1] of q's type or F32
+ *   cu_q, cu_k  int32 [n_seq + 1], device: sequence s is rows cu_q[s] ..
+ *         cu_q[s + 1] - 1 of q and cu_k[s] .. cu_k[s + 1] - 1 of k and v
+ *         (cu_k NULL: cu_q); sequences may be empty
+ *   mask  0: every query sees every key of its sequence; ACEFA_MASK_CAUSAL:
+ *         query i of n_q sees key j <= i + n_k - n_q (a prompt, or the last
+ *         n_q tokens of one); ACEFA_MASK_WINDOW: |i - j| <= window
+ * dst = softmax(scale * q k^T) v per sequence, scale > 0, sums in F32; a query
+ * that sees nothing gives 0.  Rows of dst outside every sequence are left as
+ * they were, and rows of k and v outside a sequence never reach it, whatever
+ * they hold.  Offsets must not decrease: a sequence whose offsets do, or leave
+ * the tensors, is left unwritten and raises device error 5
+ * (acefa_device_error()).  nb[0] = the element size; data and nb[1..2] of q, k and
+ * v multiples of 16 bytes; dst aligned to its elements.  rows_q and
+ * rows_kv up to 2^24, n_seq <= 65535, Hq <= 4096.  No workspace.
+ */
+ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const acefa_tensor *k, const acefa_tensor *v,
+                                      const acefa_tensor *dst, const int32_t *cu_q, const int32_t *cu_k, int n_seq,
+                                      int mask, int window, float scale, void *stream);
+
 /* Workspace acefa_flash_attn_ext() needs for these operands on the current device
  * (dense path only: mask tile classes, the partial results of the last-wave
  * key-range split, and for BF16 K/V F16 copies of K and V, 4 bytes per K/V
@@ -357,7 +494,8 @@ ACEFA_API const char *acefa_status_string(int status);
 ACEFA_API int acefa_last_launch_count(void);
 
 /* Which kernel family served the last successful call on this thread:
- * 1 = split-KV decode (mma.sync), 2 = dense tcgen05/TMEM. */
+ * 1 = split-KV decode (mma.sync), 2 = dense tcgen05/TMEM, 3 = packed sequences
+ * (tcgen05/TMEM), 4 = decode over an 8-bit block-scaled cache. */
 ACEFA_API int acefa_last_path(void);
 
 /* ABI version: major*10000 + minor*100 + patch. */
