@@ -1,9 +1,27 @@
 // fa_packed.cu -- attention of whole sequences packed behind one another
-// (acefa_flash_attn_packed).
+// (acefa_flash_attn_packed) on the tensor cores (tcgen05 / TMEM / TMA).
 //
-// One warp per (query row, head): each lane holds D / 32 dims of the query and
-// of the running output, the keys are walked one by one with an online softmax
-// in log2 units.  Right for every shape and mask; bound by its arithmetic.
+// Mathematics: the online softmax in log2 units, S = Q K^T and O += P V on
+// 128-row x 128-key tiles with F32 accumulators in tensor memory; P is rounded to
+// the operands' type (F16 or BF16), its row sum is not.  A row's maximum only
+// moves when it grows by more than 2^8, and O is rescaled only then.
+//
+// Work.  An item is a 128-token tile of one query head; the items of a
+// (sequence, KV head), tokens slowest, go two by two to one CTA, which streams
+// their keys once for both (with an even number of heads per KV head the two
+// are heads of the same tokens, so short sequences waste no second tile).  The
+// CTAs are persistent: pairs are numbered from the longest (the last tokens of
+// a causal sequence see the most keys) and dealt out back and forth, and the
+// warps' pipelines run on across pairs -- the next pair's Q, K and V arrive and
+// its first S is computed while this pair's output is still being written.
+//   warp 0      TMA: Q (2 x 32 KB), K and V tiles (4 x 32 KB ring)
+//   warp 1      MMA issue (one thread); owns TMEM: O0 | O1 | S0 | S1
+//   warp 2      where a sequence ends inside a V tile, zeroes its rows behind the
+//               end: they belong to other sequences or to nobody, and 0 * NaN is NaN
+//   warps 4-7 / 8-11  softmax, rescaling and output of tile 0 / 1, a row per thread
+// The rows of Q behind a sequence's end are computed on whatever they hold and
+// dropped.  Every wait is bounded (error word and drain on expiry).
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -15,21 +33,36 @@ namespace acefa {
 namespace {
 
 struct PackedParams {
-    const char    *q, *k, *v;
     char          *dst;
-    int64_t        q_nb1, q_nb2, k_nb1, k_nb2, v_nb1, v_nb2, d_nb1, d_nb2;  // row, head; dst: head, row
+    int64_t        d_nb1, d_nb2;  // head, row
     const int32_t *cu_q, *cu_k;
     int            n_seq, rows_q, rows_kv, Hq, Hkv;
     int            mask, window;
     int            dst_type;
+    int            vec;  // output rows are 16-B aligned
     float          scale_log2;
     int           *dev_err;
     uint64_t       wait_limit_ns;
 };
 
-constexpr int kRowsPerCta = 4;
+constexpr int      kBM = 128, kBN = 128;
+constexpr int      kThreads   = 384;
+constexpr int      kRing      = 4;
+constexpr int      kTileBytes = 128 * 128 * 2;  // 128 rows x 128 dims
+constexpr int      kOffRing   = 2 * kTileBytes;  // Q tiles first
+constexpr int      kOffBars   = kOffRing + kRing * kTileBytes;
+constexpr int      kNumBars   = 2 * kRing + 2 * 3 + 5;
+constexpr int      kOffMisc   = kOffBars + kNumBars * 8;
+constexpr int      kSmemBytes = kOffMisc + 16 + 1024;  // + alignment of the dynamic base
+constexpr uint32_t kTmemCols  = 512;
+constexpr float    kSlack     = 8.0f;
+// Register split (setmaxnreg): the sum must stay within what the block was
+// launched with, 384 x 168 = 64512, or setmaxnreg.inc would wait forever.
+constexpr uint32_t kRegsControl = 112;
+constexpr uint32_t kRegsSoftmax = 192;
+static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= 384 * 168, "register split exceeds the launch pool");
 
-// The rows of sequence s; n_q = n_k = 0 and bad for offsets that are none.
+// The rows of sequence s; empty and bad for offsets that are none.
 struct Seq {
     int  q0, n_q, k0, n_k;
     bool bad;
@@ -43,7 +76,7 @@ __device__ __forceinline__ Seq seq_of(const PackedParams &P, int s) {
     return r;
 }
 
-// Keys [lo, hi) that query i of the sequence sees.
+// Keys [lo, hi) that query i of the sequence sees; neither end falls as i grows.
 __device__ __forceinline__ void visible(const PackedParams &P, const Seq &s, int i, int &lo, int &hi) {
     lo = 0, hi = s.n_k;
     if (P.mask == ACEFA_MASK_CAUSAL) {
@@ -54,67 +87,683 @@ __device__ __forceinline__ void visible(const PackedParams &P, const Seq &s, int
     }
 }
 
-template <int HD, class T>
-__global__ void __launch_bounds__(32 * kRowsPerCta) fa_packed_simple(const __grid_constant__ PackedParams P) {
-    constexpr int N = HD / 32;
-    if (blockIdx.x == 0 && blockIdx.y == 0) {
-        for (int s = threadIdx.x; s < P.n_seq; s += blockDim.x) {
+__device__ __forceinline__ int n_pairs(const PackedParams &P, int n_q) {
+    return ((n_q + kBM - 1) / kBM * (P.Hq / P.Hkv) + 1) / 2;
+}
+
+// One CTA's piece of work: up to two items that share a KV head's keys.
+struct Unit {
+    Seq  s;
+    int  hk;
+    int  row0[2], head[2];  // first token of the tile in its sequence, query head
+    bool has[2];
+    int  a[2], b[2];  // key tiles [a, b) that some row of the tile sees
+    int  ja, jb;      // their hull (it has no gap: the ranges meet)
+};
+
+// The u-th unit, or false behind the last; the whole warp gets the same answer.
+// Up to 32 sequences (`mine`: lane s holds sequence s) are numbered by length:
+// level L holds the pair L of every sequence that has one, the highest first.
+// More are numbered one after another, each from its last pair.
+__device__ __forceinline__ bool find_unit(const PackedParams &P, int u, const Seq &mine, Unit &t) {
+    const int G = P.Hq / P.Hkv;
+    const int x = u / P.Hkv;
+    int       pair;
+    t.hk = u % P.Hkv;
+    if (P.n_seq <= 32) {
+        const int np = n_pairs(P, mine.n_q);
+        if (x >= (int) __reduce_add_sync(0xffffffffu, np)) {
+            return false;
+        }
+        // items at level L or above: falls with L; the unit's level is the last with more than x
+        int lo = 0, hi = (int) __reduce_max_sync(0xffffffffu, np);
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (x < (int) __reduce_add_sync(0xffffffffu, max(np - mid, 0))) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        pair         = lo;
+        const int  k = x - (int) __reduce_add_sync(0xffffffffu, max(np - lo - 1, 0));
+        unsigned   m = __ballot_sync(0xffffffffu, np > lo);
+        for (int i = 0; i < k; ++i) {
+            m &= m - 1;
+        }
+        const int src = __ffs(m) - 1;
+        t.s.q0  = __shfl_sync(0xffffffffu, mine.q0, src);
+        t.s.n_q = __shfl_sync(0xffffffffu, mine.n_q, src);
+        t.s.k0  = __shfl_sync(0xffffffffu, mine.k0, src);
+        t.s.n_k = __shfl_sync(0xffffffffu, mine.n_k, src);
+    } else {
+        int s, item;
+        if (!find_item(P.n_seq, x, [&](int i) { return n_pairs(P, seq_of(P, i).n_q); }, s, item)) {
+            return false;
+        }
+        t.s  = seq_of(P, s);
+        pair = n_pairs(P, t.s.n_q) - 1 - item;
+    }
+    t.ja = 1 << 30, t.jb = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int it = 2 * pair + i;
+        t.row0[i]    = it / G * kBM;
+        t.head[i]    = t.hk * G + it % G;
+        t.has[i]     = t.row0[i] < t.s.n_q;
+        t.a[i] = t.b[i] = 0;
+        if (t.has[i]) {
+            int lo, hi, unused;
+            visible(P, t.s, t.row0[i], lo, unused);
+            visible(P, t.s, min(t.row0[i] + kBM, t.s.n_q) - 1, unused, hi);
+            if (lo < hi) {
+                t.a[i] = lo / kBN, t.b[i] = (hi + kBN - 1) / kBN;
+                t.ja = min(t.ja, t.a[i]), t.jb = max(t.jb, t.b[i]);
+            }
+        }
+    }
+    t.ja = min(t.ja, t.jb);
+    return true;
+}
+
+// Unit number k of this CTA: rounds of gridDim.x units, dealt out back and forth.
+__device__ __forceinline__ int deal(int k) {
+    return k * (int) gridDim.x + ((k & 1) ? (int) (gridDim.x - 1 - blockIdx.x) : (int) blockIdx.x);
+}
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Bits [a, b) of a 32-bit word (a, b clipped to 0..32).
+__device__ __forceinline__ uint32_t bit_range(int a, int b) {
+    a = max(a, 0);
+    b = min(b, 32);
+    if (a >= b) {
+        return 0u;
+    }
+    return (b >= 32 ? ~0u : ((1u << b) - 1u)) & ~((1u << a) - 1u);
+}
+
+// 32 scores of a row against the running maximum m (log2 units, c = the scale):
+// P pairs into pk, the raw maximum into mx, the sum into ls.  VIS: bits of v
+// mark the keys that the row sees.
+template <bool VIS, bool BF16>
+__device__ __forceinline__ void exp_chunk(const uint32_t (&x)[32], uint32_t v, float c, float m, float (&mx)[2],
+                                          float (&ls)[2], uint32_t *pk) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        float a0 = __uint_as_float(x[2 * e]), a1 = __uint_as_float(x[2 * e + 1]);
+        if constexpr (VIS) {
+            a0 = (v >> (2 * e)) & 1u ? a0 : -INFINITY;
+            a1 = (v >> (2 * e + 1)) & 1u ? a1 : -INFINITY;
+        }
+        mx[e & 1]      = fmax3(mx[e & 1], a0, a1);
+        const float p0 = fast_exp2(fmaf(a0, c, -m)), p1 = fast_exp2(fmaf(a1, c, -m));
+        ls[e & 1] += p0 + p1;
+        pk[e] = pack2<BF16>(p0, p1);
+    }
+}
+
+// A row's 128 scores in TMEM: P into pk, sums into ls, the raw maximum returned.
+// The second half's loads are issued before the first half is exponentiated.
+template <bool VIS, bool BF16>
+__device__ __forceinline__ float exp_row(uint32_t tS, const uint32_t (&vis)[4], float c, float m, float (&ls)[2],
+                                         uint32_t (&pk)[64]) {
+    float    mx[2] = {-INFINITY, -INFINITY};
+    uint32_t x0[32], x1[32], y0[32], y1[32];
+    tmem_ld32(tS, x0);
+    tmem_ld32(tS + 32, x1);
+    tmem_ld_wait32(x0);
+    tmem_ld_wait32(x1);
+    tmem_ld32(tS + 64, y0);
+    tmem_ld32(tS + 96, y1);
+    exp_chunk<VIS, BF16>(x0, vis[0], c, m, mx, ls, pk);
+    exp_chunk<VIS, BF16>(x1, vis[1], c, m, mx, ls, pk + 16);
+    tmem_ld_wait32(y0);
+    tmem_ld_wait32(y1);
+    exp_chunk<VIS, BF16>(y0, vis[2], c, m, mx, ls, pk + 32);
+    exp_chunk<VIS, BF16>(y1, vis[3], c, m, mx, ls, pk + 48);
+    return fmaxf(mx[0], mx[1]);
+}
+
+// The largest visible raw score of a row.
+__device__ __forceinline__ float max_row(uint32_t tS, const uint32_t (&vis)[4]) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int ch = 0; ch < 4; ++ch) {
+        uint32_t x[32];
+        tmem_ld32(tS + 32 * ch, x);
+        tmem_ld_wait32(x);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            mx = (vis[ch] >> e) & 1u ? fmaxf(mx, __uint_as_float(x[e])) : mx;
+        }
+    }
+    return mx;
+}
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    fa_packed_kernel(const __grid_constant__ PackedParams P, const __grid_constant__ CUtensorMap qmap,
+                     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t      *smem    = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t     *full    = reinterpret_cast<uint64_t *>(smem + kOffBars);
+    uint64_t     *empty   = full + kRing;
+    uint64_t     *s_ready = empty + kRing;   // S of tile i is in TMEM
+    uint64_t     *p_ready = s_ready + 2;     // P of tile i is in TMEM
+    uint64_t     *o_done  = p_ready + 2;     // O of tile i is complete (once per unit)
+    uint64_t     *q_full  = o_done + 2;      // the unit's Q has landed
+    uint64_t     *q_empty = q_full + 1;      // its last S is computed
+    uint64_t     *ragged  = q_empty + 1;     // [2] a V tile with rows behind the sequence's end has landed
+    uint64_t     *fin     = ragged + 2;
+    uint32_t     *s_tmem  = reinterpret_cast<uint32_t *>(smem + kOffMisc);
+    volatile int *abort_f = reinterpret_cast<volatile int *>(smem + kOffMisc + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 1) {
+        tmem_alloc(s_tmem, kTmemCols);
+        tmem_relinquish();
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRing; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_ready[i], 1);
+            mbar_init(&p_ready[i], 128);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(&ragged[0], 1);
+        mbar_init(&ragged[1], 1);
+        mbar_init(fin, 1);
+        *abort_f = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&qmap);
+        prefetch_tensormap(&kmap);
+        prefetch_tensormap(&vmap);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    pdl_wait_primary();
+
+    Seq mine = {0, 0, 0, 0, false};
+    if (P.n_seq <= 32 && lane < P.n_seq) {
+        mine = seq_of(P, lane);
+    }
+    if (blockIdx.x == 0) {
+        for (int s = threadIdx.x; s < P.n_seq; s += kThreads) {
             if (seq_of(P, s).bad) {
                 atomicCAS(P.dev_err, 0, DEVERR_APPEND_POS);
             }
         }
     }
-    int s, item;
-    if (!find_item(P.n_seq, blockIdx.x, [&](int i) { return (seq_of(P, i).n_q + kRowsPerCta - 1) / kRowsPerCta; }, s,
-                   item)) {
-        return;
-    }
-    const Seq q  = seq_of(P, s);
-    const int i  = item * kRowsPerCta + (int) (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int h  = blockIdx.y, hk = h / (P.Hq / P.Hkv);
-    if (i >= q.n_q) {
-        return;
-    }
-    int lo, hi;
-    visible(P, q, i, lo, hi);
-    float    x[N], o[N], m = -INFINITY, l = 0.0f;
-    const T *qp = reinterpret_cast<const T *>(P.q + (int64_t) (q.q0 + i) * P.q_nb1 + (int64_t) h * P.q_nb2);
+    auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
+        return mbar_wait_bounded(bar, parity & 1u, abort_f, P.dev_err, code, P.wait_limit_ns);
+    };
+
+    if (warp < 4) {
+        setmaxnreg_dec<kRegsControl>();
+        if (warp == 0) {
+            // ============================ TMA producer ============================
+            // A V tile that ends behind its sequence signals `ragged` of its ring
+            // position; warp 2 passes it on to `full` when it is clean.
+            int  use = 0, n_unit = 0, n_rag0 = 0, n_rag1 = 0;
+            bool ok = true;
+            Unit t;
+            for (int k = 0; ok && find_unit(P, deal(k), mine, t); ++k) {
+                if (t.ja == t.jb) {
+                    continue;
+                }
+                if (lane == 0) {
+                    ok = wait(q_empty, (uint32_t) (n_unit & 1) ^ 1u, DEVERR_TIMEOUT_EMPTY);
+                    if (ok) {
+                        mbar_arrive_expect_tx(q_full, (uint32_t) (kBM * HD * 2) * ((t.has[0] ? 1u : 0u) + (t.has[1] ? 1u : 0u)));
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        x[e] = (float) qp[lane * N + e];
-        o[e] = 0.0f;
-    }
-    for (int j = lo; j < hi; ++j) {
-        const T *kp = reinterpret_cast<const T *>(P.k + (int64_t) (q.k0 + j) * P.k_nb1 + (int64_t) hk * P.k_nb2);
-        const T *vp = reinterpret_cast<const T *>(P.v + (int64_t) (q.k0 + j) * P.v_nb1 + (int64_t) hk * P.v_nb2);
-        float    d  = 0.0f;
+                        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            d = fmaf(x[e], (float) kp[lane * N + e], d);
+                            for (int h = 0; h < HD / 64; ++h) {
+                                if (t.has[i]) {
+                                    tma_load_3d(smem + i * kTileBytes + h * (kBM * 128), &qmap, 64 * h,
+                                                t.s.q0 + t.row0[i], t.head[i], q_full);
+                                }
+                            }
+                        }
+                    }
+                    for (int j = t.ja; j < t.jb && ok; ++j) {
+                        for (int h = 0; h < 2 && ok; ++h) {
+                            const int seq = 2 * use + h, buf = seq % kRing, ph = (seq / kRing) & 1;
+                            ok = wait(&empty[buf], (uint32_t) ph ^ 1u, DEVERR_TIMEOUT_EMPTY);
+                            if (!ok) {
+                                break;
+                            }
+                            uint8_t           *dst = smem + kOffRing + buf * kTileBytes;
+                            const CUtensorMap *map = h ? &vmap : &kmap;
+                            const bool         rag = h && t.s.n_k < (j + 1) * kBN;
+                            uint64_t          *bar = rag ? &ragged[buf >> 1] : &full[buf];
+                            n_rag0 += rag && buf == 1;
+                            n_rag1 += rag && buf == 3;
+                            mbar_arrive_expect_tx(bar, kBN * HD * 2);
+#pragma unroll
+                            for (int e = 0; e < HD / 64; ++e) {
+                                tma_load_3d(dst + e * (kBN * 128), map, 64 * e, t.s.k0 + j * kBN, t.hk, bar);
+                            }
+                        }
+                        ++use;
+                    }
+                }
+                ++n_unit;
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+            if (!ok && lane == 0) {
+                // Let the copies in flight land before the CTA exits: the last of
+                // every barrier that this thread announced (a full barrier whose
+                // tile warp 2 was to pass on may stay open; the wait is bounded).
+                const uint64_t ts = globaltimer_ns();
+                auto drain = [&](uint64_t *bar, int n) {  // n phases announced
+                    while (n > 0 && !mbar_try_wait(bar, (uint32_t) (n - 1) & 1u)) {
+                        if (globaltimer_ns() - ts > P.wait_limit_ns) {
+                            atomicCAS(P.dev_err, 0, DEVERR_TIMEOUT_DRAIN);
+                            break;
+                        }
+                    }
+                };
+                drain(q_full, n_unit);
+                drain(&ragged[0], n_rag0);
+                drain(&ragged[1], n_rag1);
+                for (int i = 0; i < kRing; ++i) {
+                    drain(&full[i], (2 * use + kRing - 1 - i) / kRing);
+                }
+            }
+        } else if (warp == 1) {
+            // ============================ MMA issuer ==============================
+            constexpr uint32_t idS = umma_idesc_f16(128, 128, false, false, BF16);
+            constexpr uint32_t idO = umma_idesc_f16(128, HD, false, true, BF16);
+            const uint64_t     qd  = umma_desc_sw128(smem_u32(smem), 16, 1024);
+            const uint64_t     kd  = umma_desc_sw128(smem_u32(smem + kOffRing), 16, 1024);
+            const uint64_t     vd  = umma_desc_sw128(smem_u32(smem + kOffRing), kBN * 128, 1024);
+            auto issue_s = [&](int i, int slot) {
+                const uint64_t q1 = qd + (uint64_t) (i * (kTileBytes >> 4)), k1 = kd + (uint64_t) (slot * (kTileBytes >> 4));
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const uint64_t off = (uint64_t) ((ks >> 2) * (kBM * 128 >> 4) + (ks & 3) * 2);
+                    umma_ss(tmem + 256 + 128 * i, q1 + off, k1 + off, idS, ks > 0 ? 1u : 0u);
+                }
+                tc_commit(&s_ready[i]);
+            };
+            auto issue_pv = [&](int i, int slot, bool acc) {
+                const uint64_t v1 = vd + (uint64_t) (slot * (kTileBytes >> 4));
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    umma_ts(tmem + 128 * i, tmem + 256 + 128 * i + ks * 8, v1 + (uint64_t) (ks * (16 * 128 >> 4)), idO,
+                            ks > 0 || acc ? 1u : 0u);
+                }
+            };
+            // The steps (unit, key tile) in order; `n` is one step ahead of `c`.
+            struct Step {
+                bool live[2], first[2], last[2];  // of tile i in this unit
+                bool new_q, end_q;                // first / last step of its unit
+            };
+            Unit t;
+            int  k = 0, j = 0, n_unit = 0, use = 0;
+            bool have = false, ok = true;
+            uint32_t p_ph[2] = {0u, 0u};
+            auto next_unit = [&]() {
+                do {
+                    have = find_unit(P, deal(k), mine, t);
+                    ++k;
+                } while (have && t.ja == t.jb);
+                j = t.ja;
+            };
+            auto step_here = [&](Step &s) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    s.live[i]  = j >= t.a[i] && j < t.b[i];
+                    s.first[i] = j == t.a[i];
+                    s.last[i]  = j == t.b[i] - 1;
+                }
+                s.new_q  = j == t.ja;
+                s.end_q  = j == t.jb - 1;
+            };
+            auto advance = [&]() {
+                if (++j == t.jb) {
+                    next_unit();
+                }
+            };
+            // S of tile i for the step whose K is in ring position 2 * pos
+            auto start_s = [&](const Step &s, int i, int pos, bool &waited) {
+                if (!waited) {
+                    if (s.new_q) {
+                        ok = wait(q_full, (uint32_t) (n_unit & 1), DEVERR_TIMEOUT_FULL);
+                        ++n_unit;
+                    }
+                    ok = ok && wait(&full[2 * pos % kRing], (uint32_t) (2 * pos / kRing), DEVERR_TIMEOUT_FULL);
+                    waited = true;
+                    if (!ok) {
+                        return;
+                    }
+                    tc_fence_after();
+                }
+                if (s.live[i]) {
+                    issue_s(i, 2 * pos % kRing);
+                }
+            };
+            auto end_s = [&](const Step &s, int pos) {
+                tc_commit(&empty[2 * pos % kRing]);
+                if (s.end_q) {
+                    tc_commit(q_empty);
+                }
+            };
+            next_unit();
+            Step c, n;
+            if (have) {
+                step_here(c);
+                if (lane == 0) {
+                    bool waited = false;
+                    start_s(c, 0, 0, waited);
+                    if (ok) {
+                        start_s(c, 1, 0, waited);
+                        end_s(c, 0);
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+            while (ok && have) {
+                advance();
+                if (have) {
+                    step_here(n);
+                }
+                if (lane == 0) {
+                    const int vpos = 2 * use + 1, vslot = vpos % kRing;
+                    bool      waited = false;
+                    ok = wait(&full[vslot], (uint32_t) (vpos / kRing), DEVERR_TIMEOUT_FULL);
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (ok && c.live[i]) {
+                            ok = wait(&p_ready[i], p_ph[i], DEVERR_TIMEOUT_MMA);
+                            p_ph[i] ^= 1u;
+                            if (ok) {
+                                tc_fence_after();
+                                issue_pv(i, vslot, !c.first[i]);
+                                if (c.last[i]) {
+                                    tc_commit(&o_done[i]);
+                                }
+                            }
+                        }
+                        if (ok && have) {
+                            start_s(n, i, use + 1, waited);
+                        }
+                    }
+                    if (ok) {
+                        tc_commit(&empty[vslot]);
+                        if (have) {
+                            end_s(n, use + 1);
+                        }
+                    }
+                }
+                ++use;
+                c  = n;
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+            if (lane == 0) {
+                // every MMA issued by this thread completes before TMEM is released
+                tc_commit(fin);
+                const uint64_t ts = globaltimer_ns();
+                while (!mbar_try_wait(fin, 0)) {
+                    if (globaltimer_ns() - ts > P.wait_limit_ns) {
+                        atomicCAS(P.dev_err, 0, DEVERR_TIMEOUT_MMA);
+                        break;
+                    }
+                }
+            }
+        } else if (warp == 2) {
+            // ==================== V rows behind the sequence's end =================
+            int  use = 0, n_rag0 = 0, n_rag1 = 0;
+            bool ok  = true;
+            Unit t;
+            for (int k = 0; ok && find_unit(P, deal(k), mine, t); ++k) {
+                const int n_it = t.jb - t.ja;
+                if (n_it && t.s.n_k < t.jb * kBN) {
+                    const int buf = (2 * (use + n_it - 1) + 1) % kRing;
+                    int      &n   = buf == 1 ? n_rag0 : n_rag1;
+                    ok = __all_sync(0xffffffffu, wait(&ragged[buf >> 1], (uint32_t) n, DEVERR_TIMEOUT_FULL));
+                    ++n;
+                    if (ok) {
+                        // a row is 128 contiguous bytes of each 64-dim box (the swizzle stays inside them)
+                        const int valid = t.s.n_k - (t.jb - 1) * kBN;
+#pragma unroll
+                        for (int e = 0; e < HD / 64; ++e) {
+                            uint4 *p = reinterpret_cast<uint4 *>(smem + kOffRing + buf * kTileBytes + e * (kBN * 128));
+                            for (int x = valid * 8 + lane; x < kBN * 8; x += 32) {
+                                p[x] = make_uint4(0u, 0u, 0u, 0u);
+                            }
+                        }
+                        fence_proxy_async_smem();  // read next by the tensor core
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&full[buf]);
+                        }
+                    }
+                }
+                use += n_it;
+            }
         }
+    } else {
+        // ============================ softmax =================================
+        setmaxnreg_inc<kRegsSoftmax>();
+        const int      i     = (warp - 4) >> 2;  // tile
+        const int      r     = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16;
+        const uint32_t tS    = tmem + lanes + 256 + 128 * i;
+        const uint32_t tO    = tmem + lanes + 128 * i;
+        const float    c     = P.scale_log2;
+        uint32_t       n_s = 0, n_o = 0;  // S tiles and finished units so far
+        bool           ok = true;
+        Unit           t;
+        for (int k = 0; ok && find_unit(P, deal(k), mine, t); ++k) {
+            // (selects, not an index: the unit stays in registers)
+            const bool has  = i ? t.has[1] : t.has[0];
+            const int  row0 = i ? t.row0[1] : t.row0[0], head = i ? t.head[1] : t.head[0];
+            const int  ja = i ? t.a[1] : t.a[0], jb = i ? t.b[1] : t.b[0];
+            if (!has) {
+                continue;
+            }
+            const int  row      = row0 + r;
+            const bool mine_row = row < t.s.n_q;
+            int        vlo = 0, vhi = 0;
+            if (mine_row) {
+                visible(P, t.s, row, vlo, vhi);
+            }
+            // keys that every row of the tile sees: such key tiles need no masks
+            int all_lo, all_hi, unused;
+            visible(P, t.s, min(row0 + kBM, t.s.n_q) - 1, all_lo, unused);
+            visible(P, t.s, row0, unused, all_hi);
+            float m_run = -INFINITY, l_run = 0.0f;
+            for (int j = ja; j < jb && ok; ++j) {
+                const int  j0   = j * kBN;
+                const bool open = j0 >= all_lo && j0 + kBN <= all_hi;
+                uint32_t   vis[4];
 #pragma unroll
-        for (int off = 16; off; off >>= 1) {
-            d += __shfl_xor_sync(0xffffffffu, d, off);
-        }
-        d *= P.scale_log2;
-        const float mn = fmaxf(m, d), f = m == -INFINITY ? 0.0f : exp2f(m - mn), p = exp2f(d - mn);
-        l = l * f + p;
-        m = mn;
+                for (int w = 0; w < 4; ++w) {
+                    vis[w] = open ? ~0u : bit_range(vlo - (j0 + 32 * w), vhi - (j0 + 32 * w));
+                }
+                ok = __all_sync(0xffffffffu, wait(&s_ready[i], n_s, DEVERR_TIMEOUT_MMA));
+                ++n_s;
+                if (!ok) {
+                    break;
+                }
+                tc_fence_after();
+                if (__any_sync(0xffffffffu, m_run == -INFINITY)) {
+                    // some row has no maximum yet.  (No row has accumulated
+                    // anything under -inf, so nothing needs rescaling for those;
+                    // the others keep theirs.)
+                    const float top = max_row(tS, vis) * c;
+                    m_run           = m_run == -INFINITY ? top : m_run;
+                }
+                uint32_t pk[64];
+                float    ls[2] = {0.0f, 0.0f};
+                float    m_use = m_run == -INFINITY ? 0.0f : m_run;
+                float    top   = open ? exp_row<false, BF16>(tS, vis, c, m_use, ls, pk)
+                                      : exp_row<true, BF16>(tS, vis, c, m_use, ls, pk);
+                top *= c;
+                const bool grew = top > m_use + kSlack && m_run != -INFINITY;
+                if (__any_sync(0xffffffffu, grew)) {
+                    // the maximum moved by more than 2^8: rescale O and l, redo the tile
+                    const float f = grew ? fast_exp2(m_run - top) : 1.0f;
+                    m_run         = grew ? top : m_run;
+                    m_use         = grew ? top : m_use;
+                    l_run *= f;
+                    if (j > ja) {
+#pragma unroll 1
+                        for (int ch = 0; ch < HD / 16; ++ch) {
+                            uint32_t x[16];
+                            tmem_ld16(tO + 16 * ch, x);
+                            tmem_ld_wait16(x);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            o[e] = fmaf((float) vp[lane * N + e], p, o[e] * f);
+                            for (int e = 0; e < 16; ++e) {
+                                x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+                            }
+                            tmem_st16(tO + 16 * ch, x);
+                        }
+                    }
+                    ls[0] = ls[1] = 0.0f;
+                    if (open) {
+                        exp_row<false, BF16>(tS, vis, c, m_use, ls, pk);
+                    } else {
+                        exp_row<true, BF16>(tS, vis, c, m_use, ls, pk);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t part[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        part[e] = pk[16 * q + e];
+                    }
+                    tmem_st16(tS + 16 * q, part);
+                }
+                l_run += ls[0] + ls[1];
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&p_ready[i]);
+            }
+            // ---- O / l leaves, a row per thread
+            const bool any = ja < jb;
+            if (ok && any) {
+                ok = __all_sync(0xffffffffu, wait(&o_done[i], n_o, DEVERR_TIMEOUT_MMA));
+                ++n_o;
+                tc_fence_after();
+            }
+            if (!ok) {
+                break;
+            }
+            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+            char *out = P.dst + (int64_t) head * P.d_nb1 + (int64_t) (t.s.q0 + row) * P.d_nb2;
+#pragma unroll 1
+            for (int ch = 0; ch < HD / 32; ++ch) {
+                uint32_t x[32];
+                if (any) {
+                    tmem_ld32(tO + 32 * ch, x);
+                    tmem_ld_wait32(x);
+                }
+                // a row that saw nothing is 0, whatever 0 * V has left in O
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    x[e] = l_run == 0.0f ? 0u : __float_as_uint(__uint_as_float(x[e]) * inv);
+                }
+                if (!mine_row) {
+                    // nothing to write; the warp stays together for the next read
+                } else if (P.dst_type == ACEFA_TYPE_F32) {
+                    float *p = reinterpret_cast<float *>(out) + 32 * ch;
+                    if (P.vec) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            *reinterpret_cast<uint4 *>(p + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            p[e] = __uint_as_float(x[e]);
+                        }
+                    }
+                } else {
+                    uint16_t *p = reinterpret_cast<uint16_t *>(out) + 32 * ch;
+                    uint32_t  y[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        y[e] = pack2<BF16>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                    }
+                    if (P.vec) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            *reinterpret_cast<uint4 *>(p + 2 * e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            p[2 * e]     = (uint16_t) y[e];
+                            p[2 * e + 1] = (uint16_t) (y[e] >> 16);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before();  // O has been read before the next unit's P is announced
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    char       *out = P.dst + (int64_t) h * P.d_nb1 + (int64_t) (q.q0 + i) * P.d_nb2;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        if (P.dst_type == ACEFA_TYPE_F32) {
-            reinterpret_cast<float *>(out)[lane * N + e] = o[e] * inv;
-        } else {
-            reinterpret_cast<T *>(out)[lane * N + e] = (T) (o[e] * inv);
-        }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
     }
+}
+
+template <int HD, bool BF16>
+cudaError_t launch(const PackedParams &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int n_cta,
+                   cudaStream_t s) {
+    static thread_local int configured = -1;
+    int                     dev        = 0;
+    cudaGetDevice(&dev);
+    if (configured != dev) {
+        cudaError_t e =
+            cudaFuncSetAttribute(fa_packed_kernel<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        configured = dev;
+    }
+    fa_packed_kernel<HD, BF16><<<n_cta, kThreads, kSmemBytes, s>>>(p, q, k, v);
+    return cudaGetLastError();
+}
+
+// [D, rows, heads] of 16-bit elements, tiles of 64 dims x 128 rows, 128-B swizzle.
+int encode_rows(CUtensorMap *map, const acefa_tensor *t) {
+    EncodeTiledFn enc = tensor_map_encoder();
+    if (!enc) {
+        return ACEFA_ERR_CUDA;
+    }
+    // strides of extent-1 dims do not matter; keep them 16-B multiples
+    const cuuint64_t rows = (cuuint64_t) t->ne[1], heads = (cuuint64_t) t->ne[2];
+    const cuuint64_t s1   = rows > 1 ? (cuuint64_t) t->nb[1] : 2u * (cuuint64_t) t->ne[0];
+    const cuuint64_t s2   = heads > 1 ? (cuuint64_t) t->nb[2] : s1 * rows;
+    cuuint64_t       dims[3] = {(cuuint64_t) t->ne[0], rows, heads}, strides[2] = {s1, s2};
+    cuuint32_t       box[3] = {64, 128, 1}, estr[3] = {1, 1, 1};
+    CUresult rc = enc(map, t->type == ACEFA_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                      3, t->data, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? ACEFA_OK : ACEFA_ERR_LAYOUT;
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
@@ -170,32 +819,40 @@ extern "C" ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const ac
         note_launches(0, 0);
         return ACEFA_OK;
     }
+    // no keys at all: nothing is loaded, but the kernel's parameters still want a map
+    CUtensorMap qm, km, vm;
+    int         mrc = encode_rows(&qm, q);
+    if (mrc == ACEFA_OK) {
+        mrc = encode_rows(&km, rows_kv ? k : q);
+    }
+    if (mrc == ACEFA_OK) {
+        mrc = encode_rows(&vm, rows_kv ? v : q);
+    }
+    if (mrc != ACEFA_OK) {
+        return mrc;
+    }
     PackedParams p;
     std::memset(&p, 0, sizeof(p));
-    p.q = static_cast<const char *>(q->data), p.k = static_cast<const char *>(k->data);
-    p.v = static_cast<const char *>(v->data), p.dst = static_cast<char *>(dst->data);
-    p.q_nb1 = (int64_t) q->nb[1], p.q_nb2 = (int64_t) q->nb[2];
-    p.k_nb1 = (int64_t) k->nb[1], p.k_nb2 = (int64_t) k->nb[2];
-    p.v_nb1 = (int64_t) v->nb[1], p.v_nb2 = (int64_t) v->nb[2];
+    p.dst   = static_cast<char *>(dst->data);
     p.d_nb1 = (int64_t) dst->nb[1], p.d_nb2 = (int64_t) dst->nb[2];
     p.cu_q = cu_q, p.cu_k = cu_k ? cu_k : cu_q;
     p.n_seq = n_seq, p.rows_q = (int) rows_q, p.rows_kv = (int) rows_kv;
     p.Hq = (int) Hq, p.Hkv = (int) Hkv;
     p.mask = mask, p.window = window;
     p.dst_type      = dst->type;
+    p.vec           = ((reinterpret_cast<uintptr_t>(dst->data) | dst->nb[1] | dst->nb[2]) & 15u) == 0;
     p.scale_log2    = scale * kLog2e;
     p.dev_err       = ctx.dev_err;
     p.wait_limit_ns = ctx.wait_limit_ns;
-    const dim3 grid((unsigned) (rows_q / kRowsPerCta + n_seq), (unsigned) Hq);
-    auto       s = static_cast<cudaStream_t>(stream);
-    if (q->type == ACEFA_TYPE_F16) {
-        D == 128 ? fa_packed_simple<128, __half><<<grid, 32 * kRowsPerCta, 0, s>>>(p)
-                 : fa_packed_simple<64, __half><<<grid, 32 * kRowsPerCta, 0, s>>>(p);
-    } else {
-        D == 128 ? fa_packed_simple<128, __nv_bfloat16><<<grid, 32 * kRowsPerCta, 0, s>>>(p)
-                 : fa_packed_simple<64, __nv_bfloat16><<<grid, 32 * kRowsPerCta, 0, s>>>(p);
-    }
-    if (cudaGetLastError() != cudaSuccess) {
+    // units: at most (tiles of all sequences * G + 1 per sequence) / 2 per KV head
+    const int64_t tiles = rows_q / kBM + n_seq;
+    const int64_t units = (tiles * (Hq / Hkv) + n_seq) / 2 * Hkv;
+    const int     n_cta = (int) std::min<int64_t>(std::max<int64_t>(units, 1), ctx.sm_count);
+    auto          s     = static_cast<cudaStream_t>(stream);
+    const bool    bf    = q->type == ACEFA_TYPE_BF16;
+    cudaError_t   e     = D == 128 ? (bf ? launch<128, true>(p, qm, km, vm, n_cta, s) : launch<128, false>(p, qm, km, vm, n_cta, s))
+                                   : (bf ? launch<64, true>(p, qm, km, vm, n_cta, s) : launch<64, false>(p, qm, km, vm, n_cta, s));
+    if (e != cudaSuccess) {
         return ACEFA_ERR_CUDA;
     }
     note_launches(1, 3);
