@@ -189,62 +189,41 @@ __device__ __forceinline__ uint32_t bit_range(int a, int b) {
     return (b >= 32 ? ~0u : ((1u << b) - 1u)) & ~((1u << a) - 1u);
 }
 
-// 32 scores of a row against the running maximum m (log2 units, c = the scale):
-// P pairs into pk, the raw maximum into mx, the sum into ls.  VIS: bits of v
-// mark the keys that the row sees.
-template <bool VIS, bool BF16>
-__device__ __forceinline__ void exp_chunk(const uint32_t (&x)[32], uint32_t v, float c, float m, float (&mx)[2],
-                                          float (&ls)[2], uint32_t *pk) {
+__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// The largest of a row's 32 scores and mx; with VIS, keys whose bit of v is 0 become -inf.
+template <bool VIS>
+__device__ __forceinline__ float max_chunk(uint32_t (&x)[32], uint32_t v, float mx) {
+    float m2[2] = {mx, -INFINITY};
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+        if constexpr (VIS) {
+            x[e]     = (v >> e) & 1u ? x[e] : 0xFF800000u;
+            x[e + 1] = (v >> (e + 1)) & 1u ? x[e + 1] : 0xFF800000u;
+        }
+        m2[(e >> 1) & 1] = fmax3(m2[(e >> 1) & 1], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+    }
+    return fmaxf(m2[0], m2[1]);
+}
+
+// P = exp2(x * c - m) of 32 scores, packed two by two over TMEM columns tP .. + 15; sums into ls.
+template <bool BF16>
+__device__ __forceinline__ void exp_chunk(const uint32_t (&x)[32], uint32_t tP, float c, float m, uint64_t (&ls)[2]) {
+    const uint64_t c2 = f32x2(c, c), m2 = f32x2(-m, -m);
+    uint32_t       pk[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        float a0 = __uint_as_float(x[2 * e]), a1 = __uint_as_float(x[2 * e + 1]);
-        if constexpr (VIS) {
-            a0 = (v >> (2 * e)) & 1u ? a0 : -INFINITY;
-            a1 = (v >> (2 * e + 1)) & 1u ? a1 : -INFINITY;
-        }
-        mx[e & 1]      = fmax3(mx[e & 1], a0, a1);
-        const float p0 = fast_exp2(fmaf(a0, c, -m)), p1 = fast_exp2(fmaf(a1, c, -m));
-        ls[e & 1] += p0 + p1;
-        pk[e] = pack2<BF16>(p0, p1);
+        float a0, a1;
+        f32x2_split(ffma2(f32x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, m2), a0, a1);
+        const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);
+        ls[e & 1]      = fadd2(ls[e & 1], f32x2(p0, p1));
+        pk[e]          = pack2<BF16>(p0, p1);
     }
-}
-
-// A row's 128 scores in TMEM: P into pk, sums into ls, the raw maximum returned.
-// The second half's loads are issued before the first half is exponentiated.
-template <bool VIS, bool BF16>
-__device__ __forceinline__ float exp_row(uint32_t tS, const uint32_t (&vis)[4], float c, float m, float (&ls)[2],
-                                         uint32_t (&pk)[64]) {
-    float    mx[2] = {-INFINITY, -INFINITY};
-    uint32_t x0[32], x1[32], y0[32], y1[32];
-    tmem_ld32(tS, x0);
-    tmem_ld32(tS + 32, x1);
-    tmem_ld_wait32(x0);
-    tmem_ld_wait32(x1);
-    tmem_ld32(tS + 64, y0);
-    tmem_ld32(tS + 96, y1);
-    exp_chunk<VIS, BF16>(x0, vis[0], c, m, mx, ls, pk);
-    exp_chunk<VIS, BF16>(x1, vis[1], c, m, mx, ls, pk + 16);
-    tmem_ld_wait32(y0);
-    tmem_ld_wait32(y1);
-    exp_chunk<VIS, BF16>(y0, vis[2], c, m, mx, ls, pk + 32);
-    exp_chunk<VIS, BF16>(y1, vis[3], c, m, mx, ls, pk + 48);
-    return fmaxf(mx[0], mx[1]);
-}
-
-// The largest visible raw score of a row.
-__device__ __forceinline__ float max_row(uint32_t tS, const uint32_t (&vis)[4]) {
-    float mx = -INFINITY;
-#pragma unroll
-    for (int ch = 0; ch < 4; ++ch) {
-        uint32_t x[32];
-        tmem_ld32(tS + 32 * ch, x);
-        tmem_ld_wait32(x);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            mx = (vis[ch] >> e) & 1u ? fmaxf(mx, __uint_as_float(x[e])) : mx;
-        }
-    }
-    return mx;
+    tmem_st16(tP, pk);
 }
 
 template <int HD, bool BF16>
@@ -589,40 +568,44 @@ __global__ void __launch_bounds__(kThreads, 1)
             int all_lo, all_hi, unused;
             visible(P, t.s, min(row0 + kBM, t.s.n_q) - 1, all_lo, unused);
             visible(P, t.s, row0, unused, all_hi);
-            float m_run = -INFINITY, l_run = 0.0f;
+            // rows behind the sequence's end: under +inf their weights are 0 and their maximum never moves
+            float m_run = mine_row ? -INFINITY : INFINITY, l_run = 0.0f;
             for (int j = ja; j < jb && ok; ++j) {
                 const int  j0   = j * kBN;
                 const bool open = j0 >= all_lo && j0 + kBN <= all_hi;
-                uint32_t   vis[4];
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    vis[w] = open ? ~0u : bit_range(vlo - (j0 + 32 * w), vhi - (j0 + 32 * w));
-                }
                 ok = __all_sync(0xffffffffu, wait(&s_ready[i], n_s, DEVERR_TIMEOUT_MMA));
                 ++n_s;
                 if (!ok) {
                     break;
                 }
                 tc_fence_after();
-                if (__any_sync(0xffffffffu, m_run == -INFINITY)) {
-                    // some row has no maximum yet.  (No row has accumulated
-                    // anything under -inf, so nothing needs rescaling for those;
-                    // the others keep theirs.)
-                    const float top = max_row(tS, vis) * c;
-                    m_run           = m_run == -INFINITY ? top : m_run;
+                // the row's scores stay in registers between the maximum and the exponentials
+                uint32_t x0[32], x1[32], x2[32], x3[32];
+                tmem_ld32(tS, x0);
+                tmem_ld32(tS + 32, x1);
+                tmem_ld32(tS + 64, x2);
+                tmem_ld32(tS + 96, x3);
+                tmem_ld_wait32(x0);
+                tmem_ld_wait32(x1);
+                tmem_ld_wait32(x2);
+                tmem_ld_wait32(x3);
+                float top = -INFINITY;
+                if (open) {
+                    top = max_chunk<false>(x0, 0u, top);
+                    top = max_chunk<false>(x1, 0u, top);
+                    top = max_chunk<false>(x2, 0u, top);
+                    top = max_chunk<false>(x3, 0u, top);
+                } else {
+                    top = max_chunk<true>(x0, bit_range(vlo - j0, vhi - j0), top);
+                    top = max_chunk<true>(x1, bit_range(vlo - j0 - 32, vhi - j0 - 32), top);
+                    top = max_chunk<true>(x2, bit_range(vlo - j0 - 64, vhi - j0 - 64), top);
+                    top = max_chunk<true>(x3, bit_range(vlo - j0 - 96, vhi - j0 - 96), top);
                 }
-                uint32_t pk[64];
-                float    ls[2] = {0.0f, 0.0f};
-                float    m_use = m_run == -INFINITY ? 0.0f : m_run;
-                float    top   = open ? exp_row<false, BF16>(tS, vis, c, m_use, ls, pk)
-                                      : exp_row<true, BF16>(tS, vis, c, m_use, ls, pk);
                 top *= c;
-                const bool grew = top > m_use + kSlack && m_run != -INFINITY;
+                const bool grew = top > m_run + kSlack;  // the first visible key counts: any number is above -inf
                 if (__any_sync(0xffffffffu, grew)) {
-                    // the maximum moved by more than 2^8: rescale O and l, redo the tile
                     const float f = grew ? fast_exp2(m_run - top) : 1.0f;
                     m_run         = grew ? top : m_run;
-                    m_use         = grew ? top : m_use;
                     l_run *= f;
                     if (j > ja) {
 #pragma unroll 1
@@ -637,23 +620,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tmem_st16(tO + 16 * ch, x);
                         }
                     }
-                    ls[0] = ls[1] = 0.0f;
-                    if (open) {
-                        exp_row<false, BF16>(tS, vis, c, m_use, ls, pk);
-                    } else {
-                        exp_row<true, BF16>(tS, vis, c, m_use, ls, pk);
-                    }
                 }
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t part[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        part[e] = pk[16 * q + e];
-                    }
-                    tmem_st16(tS + 16 * q, part);
-                }
-                l_run += ls[0] + ls[1];
+                const float m_use = m_run == -INFINITY ? 0.0f : m_run;
+                uint64_t    ls[2] = {0ull, 0ull};
+                exp_chunk<BF16>(x0, tS, c, m_use, ls);
+                exp_chunk<BF16>(x1, tS + 16, c, m_use, ls);
+                exp_chunk<BF16>(x2, tS + 32, c, m_use, ls);
+                exp_chunk<BF16>(x3, tS + 48, c, m_use, ls);
+                float l0, l1;
+                f32x2_split(fadd2(ls[0], ls[1]), l0, l1);
+                l_run += l0 + l1;
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&p_ready[i]);
