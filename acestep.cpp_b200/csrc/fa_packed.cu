@@ -16,6 +16,7 @@
 // its first S is computed while this pair's output is still being written.
 //   warp 0      TMA: Q (2 x 32 KB), K and V tiles (4 x 32 KB ring)
 //   warp 1      MMA issue (one thread); owns TMEM: O0 | O1 | S0 | S1
+//   warp 3      finds the CTA's units and hands them to the others through a ring
 //   warp 2      where a sequence ends inside a V tile, zeroes its rows behind the
 //               end: they belong to other sequences or to nobody, and 0 * NaN is NaN
 //   warps 4-7 / 8-11  softmax, rescaling and output of tile 0 / 1, a row per thread
@@ -36,7 +37,8 @@ struct PackedParams {
     char          *dst;
     int64_t        d_nb1, d_nb2;  // head, row
     const int32_t *cu_q, *cu_k;
-    int            n_seq, rows_q, rows_kv, Hq, Hkv;
+    int            n_seq, rows_q, rows_kv, Hkv, G;  // G query heads per KV head
+    uint32_t       inv_hkv, inv_g;  // floor(2^32 / d) (d = 1: 2^32 - 1), for divide()
     int            mask, window;
     int            dst_type;
     int            vec;  // output rows are 16-B aligned
@@ -51,9 +53,15 @@ constexpr int      kRing      = 4;
 constexpr int      kTileBytes = 128 * 128 * 2;  // 128 rows x 128 dims
 constexpr int      kOffRing   = 2 * kTileBytes;  // Q tiles first
 constexpr int      kOffBars   = kOffRing + kRing * kTileBytes;
-constexpr int      kNumBars   = 2 * kRing + 2 * 3 + 5;
+constexpr int      kUnitRing  = 4;                       // units known ahead
+constexpr int      kUnitReaders = 11;                    // warps that read them: all but the one that finds them
+constexpr int      kNumBars   = 2 * kRing + 2 * 4 + 5 + 2 * kUnitRing;
 constexpr int      kOffMisc   = kOffBars + kNumBars * 8;
-constexpr int      kSmemBytes = kOffMisc + 16 + 1024;  // + alignment of the dynamic base
+constexpr int      kOffUnits  = (kOffMisc + 16 + 15) / 16 * 16;
+constexpr int      kOffOut    = kOffUnits + kUnitRing * 64;  // where each softmax warp's rows go
+constexpr int      kOffStage  = (kOffOut + 8 * 16 + 127) / 128 * 128;  // output rows, 4 KB per softmax warp
+constexpr int      kSmemBytes = kOffStage + 8 * 4096 + 1024;  // + alignment of the dynamic base
+static_assert(kSmemBytes <= 232448, "more than the 227 KB of a CTA");
 constexpr uint32_t kTmemCols  = 512;
 constexpr float    kSlack     = 8.0f;
 // Register split (setmaxnreg): the sum must stay within what the block was
@@ -88,32 +96,39 @@ __device__ __forceinline__ void visible(const PackedParams &P, const Seq &s, int
 }
 
 __device__ __forceinline__ int n_pairs(const PackedParams &P, int n_q) {
-    return ((n_q + kBM - 1) / kBM * (P.Hq / P.Hkv) + 1) / 2;
+    return ((n_q + kBM - 1) / kBM * P.G + 1) >> 1;
+}
+
+// n / d with inv = floor(2^32 / d): the product's high word is at most one short.
+__device__ __forceinline__ int divide(int n, int d, uint32_t inv) {
+    const int q = (int) __umulhi((uint32_t) n, inv);
+    return q + (n - q * d >= d);
 }
 
 // One CTA's piece of work: up to two items that share a KV head's keys.
-struct Unit {
-    Seq  s;
-    int  hk;
-    int  row0[2], head[2];  // first token of the tile in its sequence, query head
-    bool has[2];
-    int  a[2], b[2];  // key tiles [a, b) that some row of the tile sees
-    int  ja, jb;      // their hull (it has no gap: the ranges meet)
+struct alignas(16) Unit {
+    int q0, n_q, k0, n_k;   // rows of the sequence
+    int hk, more;           // KV head; 0: behind the last unit
+    int ja, jb;             // key tiles [ja, jb) that some row sees: the tiles' ranges together (they meet)
+    int row0[2], head[2];   // first token of a tile in its sequence, its query head
+    int a[2], b[2];         // key tiles [a, b) of a tile; row0 >= n_q: no such tile
 };
+static_assert(sizeof(Unit) == 64, "a slot of the ring");
 
-// The u-th unit, or false behind the last; the whole warp gets the same answer.
+// The u-th unit (t.more = 0 behind the last); the whole warp gets the same answer.
 // Up to 32 sequences (`mine`: lane s holds sequence s) are numbered by length:
 // level L holds the pair L of every sequence that has one, the highest first.
 // More are numbered one after another, each from its last pair.
-__device__ __forceinline__ bool find_unit(const PackedParams &P, int u, const Seq &mine, Unit &t) {
-    const int G = P.Hq / P.Hkv;
-    const int x = u / P.Hkv;
+__device__ __forceinline__ void find_unit(const PackedParams &P, int u, const Seq &mine, Unit &t) {
+    const int x = divide(u, P.Hkv, P.inv_hkv);
     int       pair;
-    t.hk = u % P.Hkv;
+    Seq       q;
+    t.hk   = u - x * P.Hkv;
+    t.more = 0;
     if (P.n_seq <= 32) {
         const int np = n_pairs(P, mine.n_q);
         if (x >= (int) __reduce_add_sync(0xffffffffu, np)) {
-            return false;
+            return;
         }
         // items at level L or above: falls with L; the unit's level is the last with more than x
         int lo = 0, hi = (int) __reduce_max_sync(0xffffffffu, np);
@@ -132,30 +147,32 @@ __device__ __forceinline__ bool find_unit(const PackedParams &P, int u, const Se
             m &= m - 1;
         }
         const int src = __ffs(m) - 1;
-        t.s.q0  = __shfl_sync(0xffffffffu, mine.q0, src);
-        t.s.n_q = __shfl_sync(0xffffffffu, mine.n_q, src);
-        t.s.k0  = __shfl_sync(0xffffffffu, mine.k0, src);
-        t.s.n_k = __shfl_sync(0xffffffffu, mine.n_k, src);
+        q.q0  = __shfl_sync(0xffffffffu, mine.q0, src);
+        q.n_q = __shfl_sync(0xffffffffu, mine.n_q, src);
+        q.k0  = __shfl_sync(0xffffffffu, mine.k0, src);
+        q.n_k = __shfl_sync(0xffffffffu, mine.n_k, src);
     } else {
         int s, item;
         if (!find_item(P.n_seq, x, [&](int i) { return n_pairs(P, seq_of(P, i).n_q); }, s, item)) {
-            return false;
+            return;
         }
-        t.s  = seq_of(P, s);
-        pair = n_pairs(P, t.s.n_q) - 1 - item;
+        q    = seq_of(P, s);
+        pair = n_pairs(P, q.n_q) - 1 - item;
     }
+    t.more = 1;
+    t.q0 = q.q0, t.n_q = q.n_q, t.k0 = q.k0, t.n_k = q.n_k;
     t.ja = 1 << 30, t.jb = 0;
+    const int tt = divide(2 * pair, P.G, P.inv_g), g = 2 * pair - tt * P.G;  // of the first item
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int it = 2 * pair + i;
-        t.row0[i]    = it / G * kBM;
-        t.head[i]    = t.hk * G + it % G;
-        t.has[i]     = t.row0[i] < t.s.n_q;
+        const bool wrap = i && g + 1 == P.G;
+        t.row0[i]       = (tt + (wrap ? 1 : 0)) * kBM;
+        t.head[i]       = t.hk * P.G + (wrap ? 0 : g + i);
         t.a[i] = t.b[i] = 0;
-        if (t.has[i]) {
+        if (t.row0[i] < q.n_q) {
             int lo, hi, unused;
-            visible(P, t.s, t.row0[i], lo, unused);
-            visible(P, t.s, min(t.row0[i] + kBM, t.s.n_q) - 1, unused, hi);
+            visible(P, q, t.row0[i], lo, unused);
+            visible(P, q, min(t.row0[i] + kBM, q.n_q) - 1, unused, hi);
             if (lo < hi) {
                 t.a[i] = lo / kBN, t.b[i] = (hi + kBN - 1) / kBN;
                 t.ja = min(t.ja, t.a[i]), t.jb = max(t.jb, t.b[i]);
@@ -163,7 +180,6 @@ __device__ __forceinline__ bool find_unit(const PackedParams &P, int u, const Se
         }
     }
     t.ja = min(t.ja, t.jb);
-    return true;
 }
 
 // Unit number k of this CTA: rounds of gridDim.x units, dealt out back and forth.
@@ -187,6 +203,15 @@ __device__ __forceinline__ uint32_t bit_range(int a, int b) {
         return 0u;
     }
     return (b >= 32 ? ~0u : ((1u << b) - 1u)) & ~((1u << a) - 1u);
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
@@ -236,11 +261,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t     *empty   = full + kRing;
     uint64_t     *s_ready = empty + kRing;   // S of tile i is in TMEM
     uint64_t     *p_ready = s_ready + 2;     // P of tile i is in TMEM
-    uint64_t     *o_done  = p_ready + 2;     // O of tile i is complete (once per unit)
+    uint64_t     *p_half  = p_ready + 2;     // its first 64 keys are
+    uint64_t     *o_done  = p_half + 2;      // O of tile i is complete (once per unit)
     uint64_t     *q_full  = o_done + 2;      // the unit's Q has landed
     uint64_t     *q_empty = q_full + 1;      // its last S is computed
     uint64_t     *ragged  = q_empty + 1;     // [2] a V tile with rows behind the sequence's end has landed
     uint64_t     *fin     = ragged + 2;
+    uint64_t     *u_full  = fin + 1;         // [kUnitRing] a unit is there
+    uint64_t     *u_empty = u_full + kUnitRing;
+    Unit         *units   = reinterpret_cast<Unit *>(smem + kOffUnits);
     uint32_t     *s_tmem  = reinterpret_cast<uint32_t *>(smem + kOffMisc);
     volatile int *abort_f = reinterpret_cast<volatile int *>(smem + kOffMisc + 4);
 
@@ -257,6 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_ready[i], 1);
             mbar_init(&p_ready[i], 128);
+            mbar_init(&p_half[i], 128);
             mbar_init(&o_done[i], 1);
         }
         mbar_init(q_full, 1);
@@ -264,6 +294,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&ragged[0], 1);
         mbar_init(&ragged[1], 1);
         mbar_init(fin, 1);
+        for (int i = 0; i < kUnitRing; ++i) {
+            mbar_init(&u_full[i], 1);
+            mbar_init(&u_empty[i], kUnitReaders);
+        }
         *abort_f = 0;
         fence_barrier_init();
         prefetch_tensormap(&qmap);
@@ -276,45 +310,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *s_tmem;
     pdl_wait_primary();
 
-    Seq mine = {0, 0, 0, 0, false};
-    if (P.n_seq <= 32 && lane < P.n_seq) {
-        mine = seq_of(P, lane);
-    }
-    if (blockIdx.x == 0) {
-        for (int s = threadIdx.x; s < P.n_seq; s += kThreads) {
-            if (seq_of(P, s).bad) {
-                atomicCAS(P.dev_err, 0, DEVERR_APPEND_POS);
-            }
-        }
-    }
     auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
         return mbar_wait_bounded(bar, parity & 1u, abort_f, P.dev_err, code, P.wait_limit_ns);
     };
 
+    // The k-th unit of this CTA, read by a whole warp; false behind the last (or on expiry).
+    auto next_unit = [&](int &k, Unit &t) {
+        const int  slot = k % kUnitRing;
+        const bool ok   = __all_sync(0xffffffffu, wait(&u_full[slot], (uint32_t) (k / kUnitRing), DEVERR_TIMEOUT_FULL));
+        t               = units[slot];
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(&u_empty[slot]);
+        }
+        ++k;
+        return ok && t.more != 0;
+    };
+
     if (warp < 4) {
         setmaxnreg_dec<kRegsControl>();
-        if (warp == 0) {
+        if (warp == 3) {
+            // ============================ units ====================================
+            Seq mine = {0, 0, 0, 0, false};
+            if (P.n_seq <= 32 && lane < P.n_seq) {
+                mine = seq_of(P, lane);
+            }
+            if (blockIdx.x == 0) {
+                for (int s = lane; s < P.n_seq; s += 32) {
+                    if (seq_of(P, s).bad) {
+                        atomicCAS(P.dev_err, 0, DEVERR_APPEND_POS);
+                    }
+                }
+            }
+            Unit t;
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                find_unit(P, deal(k), mine, t);
+                ok = __all_sync(0xffffffffu, wait(&u_empty[k % kUnitRing], (uint32_t) (k / kUnitRing) ^ 1u,
+                                                  DEVERR_TIMEOUT_EMPTY));
+                if (ok && lane == 0) {
+                    units[k % kUnitRing] = t;
+                    mbar_arrive(&u_full[k % kUnitRing]);
+                }
+                ok = ok && t.more != 0;
+            }
+        } else if (warp == 0) {
             // ============================ TMA producer ============================
             // A V tile that ends behind its sequence signals `ragged` of its ring
             // position; warp 2 passes it on to `full` when it is clean.
-            int  use = 0, n_unit = 0, n_rag0 = 0, n_rag1 = 0;
+            int  use = 0, n_unit = 0, n_rag0 = 0, n_rag1 = 0, k = 0;
             bool ok = true;
             Unit t;
-            for (int k = 0; ok && find_unit(P, deal(k), mine, t); ++k) {
+            while (ok && next_unit(k, t)) {
                 if (t.ja == t.jb) {
                     continue;
                 }
                 if (lane == 0) {
+                    const bool two = t.row0[1] < t.n_q;  // (the first tile is there in every unit)
                     ok = wait(q_empty, (uint32_t) (n_unit & 1) ^ 1u, DEVERR_TIMEOUT_EMPTY);
                     if (ok) {
-                        mbar_arrive_expect_tx(q_full, (uint32_t) (kBM * HD * 2) * ((t.has[0] ? 1u : 0u) + (t.has[1] ? 1u : 0u)));
+                        mbar_arrive_expect_tx(q_full, (uint32_t) (kBM * HD * 2) * (two ? 2u : 1u));
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
 #pragma unroll
                             for (int h = 0; h < HD / 64; ++h) {
-                                if (t.has[i]) {
+                                if (i == 0 || two) {
                                     tma_load_3d(smem + i * kTileBytes + h * (kBM * 128), &qmap, 64 * h,
-                                                t.s.q0 + t.row0[i], t.head[i], q_full);
+                                                t.q0 + t.row0[i], t.head[i], q_full);
                                 }
                             }
                         }
@@ -328,14 +390,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                             uint8_t           *dst = smem + kOffRing + buf * kTileBytes;
                             const CUtensorMap *map = h ? &vmap : &kmap;
-                            const bool         rag = h && t.s.n_k < (j + 1) * kBN;
+                            const bool         rag = h && t.n_k < (j + 1) * kBN;
                             uint64_t          *bar = rag ? &ragged[buf >> 1] : &full[buf];
                             n_rag0 += rag && buf == 1;
                             n_rag1 += rag && buf == 3;
                             mbar_arrive_expect_tx(bar, kBN * HD * 2);
 #pragma unroll
                             for (int e = 0; e < HD / 64; ++e) {
-                                tma_load_3d(dst + e * (kBN * 128), map, 64 * e, t.s.k0 + j * kBN, t.hk, bar);
+                                tma_load_3d(dst + e * (kBN * 128), map, 64 * e, t.k0 + j * kBN, t.hk, bar);
                             }
                         }
                         ++use;
@@ -344,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++n_unit;
                 ok = __shfl_sync(0xffffffffu, ok, 0);
             }
-            if (!ok && lane == 0) {
+            if (*abort_f && lane == 0) {
                 // Let the copies in flight land before the CTA exits: the last of
                 // every barrier that this thread announced (a full barrier whose
                 // tile warp 2 was to pass on may stay open; the wait is bounded).
@@ -380,10 +442,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_commit(&s_ready[i]);
             };
-            auto issue_pv = [&](int i, int slot, bool acc) {
+            // keys [64 h, 64 h + 64) of the tile
+            auto issue_pv = [&](int i, int h, int slot, bool acc) {
                 const uint64_t v1 = vd + (uint64_t) (slot * (kTileBytes >> 4));
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
+                for (int ks = 4 * h; ks < 4 * h + 4; ++ks) {
                     umma_ts(tmem + 128 * i, tmem + 256 + 128 * i + ks * 8, v1 + (uint64_t) (ks * (16 * 128 >> 4)), idO,
                             ks > 0 || acc ? 1u : 0u);
                 }
@@ -397,10 +460,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             int  k = 0, j = 0, n_unit = 0, use = 0;
             bool have = false, ok = true;
             uint32_t p_ph[2] = {0u, 0u};
-            auto next_unit = [&]() {
+            auto enter_unit = [&]() {
                 do {
-                    have = find_unit(P, deal(k), mine, t);
-                    ++k;
+                    have = next_unit(k, t);
                 } while (have && t.ja == t.jb);
                 j = t.ja;
             };
@@ -416,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             auto advance = [&]() {
                 if (++j == t.jb) {
-                    next_unit();
+                    enter_unit();
                 }
             };
             // S of tile i for the step whose K is in ring position 2 * pos
@@ -443,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_commit(q_empty);
                 }
             };
-            next_unit();
+            enter_unit();
             Step c, n;
             if (have) {
                 step_here(c);
@@ -470,18 +532,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (ok && c.live[i]) {
-                            ok = wait(&p_ready[i], p_ph[i], DEVERR_TIMEOUT_MMA);
+                            ok = wait(&p_half[i], p_ph[i], DEVERR_TIMEOUT_MMA);
+                            if (ok) {
+                                tc_fence_after();
+                                issue_pv(i, 0, vslot, !c.first[i]);
+                                ok = wait(&p_ready[i], p_ph[i], DEVERR_TIMEOUT_MMA);
+                            }
                             p_ph[i] ^= 1u;
                             if (ok) {
                                 tc_fence_after();
-                                issue_pv(i, vslot, !c.first[i]);
+                                issue_pv(i, 1, vslot, true);
                                 if (c.last[i]) {
                                     tc_commit(&o_done[i]);
                                 }
                             }
                         }
-                        if (ok && have) {
+                        // S of the next step between the tiles' PVs; a new unit's
+                        // waits for its Q, so there both PVs go first
+                        if (ok && have && !n.new_q) {
                             start_s(n, i, use + 1, waited);
+                        }
+                    }
+                    if (ok && have && n.new_q) {
+                        start_s(n, 0, use + 1, waited);
+                        if (ok) {
+                            start_s(n, 1, use + 1, waited);
                         }
                     }
                     if (ok) {
@@ -508,19 +583,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == 2) {
             // ==================== V rows behind the sequence's end =================
-            int  use = 0, n_rag0 = 0, n_rag1 = 0;
+            int  use = 0, n_rag0 = 0, n_rag1 = 0, k = 0;
             bool ok  = true;
             Unit t;
-            for (int k = 0; ok && find_unit(P, deal(k), mine, t); ++k) {
+            while (ok && next_unit(k, t)) {
                 const int n_it = t.jb - t.ja;
-                if (n_it && t.s.n_k < t.jb * kBN) {
+                if (n_it && t.n_k < t.jb * kBN) {
                     const int buf = (2 * (use + n_it - 1) + 1) % kRing;
-                    int      &n   = buf == 1 ? n_rag0 : n_rag1;
-                    ok = __all_sync(0xffffffffu, wait(&ragged[buf >> 1], (uint32_t) n, DEVERR_TIMEOUT_FULL));
-                    ++n;
+                    ok = __all_sync(0xffffffffu, wait(&ragged[buf >> 1], (uint32_t) (buf == 1 ? n_rag0 : n_rag1),
+                                                      DEVERR_TIMEOUT_FULL));
+                    n_rag0 += buf == 1;
+                    n_rag1 += buf == 3;
                     if (ok) {
                         // a row is 128 contiguous bytes of each 64-dim box (the swizzle stays inside them)
-                        const int valid = t.s.n_k - (t.jb - 1) * kBN;
+                        const int valid = t.n_k - (t.jb - 1) * kBN;
 #pragma unroll
                         for (int e = 0; e < HD / 64; ++e) {
                             uint4 *p = reinterpret_cast<uint4 *>(smem + kOffRing + buf * kTileBytes + e * (kBN * 128));
@@ -549,25 +625,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float    c     = P.scale_log2;
         uint32_t       n_s = 0, n_o = 0;  // S tiles and finished units so far
         bool           ok = true;
+        int            k  = 0;
+        uint8_t       *stage = smem + kOffStage + (warp - 4) * 4096;
+        volatile int  *out_at = reinterpret_cast<volatile int *>(smem + kOffOut) + (warp - 4) * 4;
         Unit           t;
-        for (int k = 0; ok && find_unit(P, deal(k), mine, t); ++k) {
+        while (ok && next_unit(k, t)) {
             // (selects, not an index: the unit stays in registers)
-            const bool has  = i ? t.has[1] : t.has[0];
-            const int  row0 = i ? t.row0[1] : t.row0[0], head = i ? t.head[1] : t.head[0];
-            const int  ja = i ? t.a[1] : t.a[0], jb = i ? t.b[1] : t.b[0];
-            if (!has) {
+            const int row0 = i ? t.row0[1] : t.row0[0], head = i ? t.head[1] : t.head[0];
+            const int ja = i ? t.a[1] : t.a[0], jb = i ? t.b[1] : t.b[0];
+            if (row0 >= t.n_q) {
                 continue;
             }
+            const Seq  q        = {t.q0, t.n_q, t.k0, t.n_k, false};
             const int  row      = row0 + r;
-            const bool mine_row = row < t.s.n_q;
+            const bool mine_row = row < q.n_q;
             int        vlo = 0, vhi = 0;
             if (mine_row) {
-                visible(P, t.s, row, vlo, vhi);
+                visible(P, q, row, vlo, vhi);
             }
             // keys that every row of the tile sees: such key tiles need no masks
             int all_lo, all_hi, unused;
-            visible(P, t.s, min(row0 + kBM, t.s.n_q) - 1, all_lo, unused);
-            visible(P, t.s, row0, unused, all_hi);
+            visible(P, q, min(row0 + kBM, q.n_q) - 1, all_lo, unused);
+            visible(P, q, row0, unused, all_hi);
+            // what the output needs waits in shared memory: the loop's registers are full of scores
+            if (lane == 0) {
+                const int w0 = row0 + (warp & 3) * 32;  // the warp's first row
+                out_at[0] = q.q0 + w0, out_at[1] = q.n_q - w0, out_at[2] = head;
+            }
+            __syncwarp();
             // rows behind the sequence's end: under +inf their weights are 0 and their maximum never moves
             float m_run = mine_row ? -INFINITY : INFINITY, l_run = 0.0f;
             for (int j = ja; j < jb && ok; ++j) {
@@ -625,6 +710,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint64_t    ls[2] = {0ull, 0ull};
                 exp_chunk<BF16>(x0, tS, c, m_use, ls);
                 exp_chunk<BF16>(x1, tS + 16, c, m_use, ls);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&p_half[i]);  // the product with V starts on these 64 keys
                 exp_chunk<BF16>(x2, tS + 32, c, m_use, ls);
                 exp_chunk<BF16>(x3, tS + 48, c, m_use, ls);
                 float l0, l1;
@@ -634,9 +722,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_before();
                 mbar_arrive(&p_ready[i]);
             }
-            // ---- O / l leaves, a row per thread
-            const bool any = ja < jb;
-            if (ok && any) {
+            // ---- O / l leaves: 128-B pieces of the warp's 32 rows through its
+            // staging slab (16-B chunk x of row y at x ^ (y & 7): no bank conflicts
+            // either way), so that a store instruction writes whole lines
+            // (a tile that saw no key reads what O happens to hold, and writes zeros)
+            if (ok && ja < jb) {
                 ok = __all_sync(0xffffffffu, wait(&o_done[i], n_o, DEVERR_TIMEOUT_MMA));
                 ++n_o;
                 tc_fence_after();
@@ -644,56 +734,102 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) {
                 break;
             }
-            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-            char *out = P.dst + (int64_t) head * P.d_nb1 + (int64_t) (t.s.q0 + row) * P.d_nb2;
-#pragma unroll 1
-            for (int ch = 0; ch < HD / 32; ++ch) {
-                uint32_t x[32];
-                if (any) {
-                    tmem_ld32(tO + 32 * ch, x);
-                    tmem_ld_wait32(x);
-                }
-                // a row that saw nothing is 0, whatever 0 * V has left in O
+            // (opaque copies: their addresses must not be hoisted into the key loop)
+            int      ln   = lane;
+            uint32_t slab = smem_u32(stage);
+            int64_t  nb2  = P.d_nb2;
+            asm volatile("" : "+r"(ln), "+r"(slab), "+l"(nb2));
+            const bool  none = l_run == 0.0f;  // the row saw nothing: 0, whatever 0 * V has left in O
+            const float inv  = none ? 0.0f : 1.0f / l_run;
+            const int   rows = out_at[1];  // of this warp, if below 32
+            char *out = P.dst + (int64_t) out_at[2] * P.d_nb1 + (int64_t) out_at[0] * nb2;
+            // 32 dims of the row, finished
+            auto finished = [&](uint32_t(&x)[32]) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    x[e] = l_run == 0.0f ? 0u : __float_as_uint(__uint_as_float(x[e]) * inv);
+                    x[e] = __float_as_uint(__uint_as_float(x[e]) * inv);
                 }
-                if (!mine_row) {
-                    // nothing to write; the warp stays together for the next read
-                } else if (P.dst_type == ACEFA_TYPE_F32) {
-                    float *p = reinterpret_cast<float *>(out) + 32 * ch;
-                    if (P.vec) {
+                if (__any_sync(0xffffffffu, none)) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            *reinterpret_cast<uint4 *>(p + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-                        }
-                    } else {
+                    for (int e = 0; e < 32; ++e) {
+                        x[e] = none ? 0u : x[e];
+                    }
+                }
+            };
+            // the slab's 32 x 128 B to dst, piece n of the rows
+            auto write_slab = [&](int n, bool f32) {
+                __syncwarp();
+                uint4 w[8];
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            p[e] = __uint_as_float(x[e]);
+                for (int st = 0; st < 8; ++st) {
+                    const int rr = 4 * st + (ln >> 3);
+                    w[st] = ld_shared_v4(slab + rr * 128 + (((ln & 7) ^ (rr & 7)) << 4));
+                }
+                char *p = out + 128 * n + 16 * (ln & 7) + (int64_t) (ln >> 3) * nb2;
+                if (P.vec) {
+#pragma unroll
+                    for (int st = 0; st < 8; ++st) {
+                        if (4 * st + (ln >> 3) < rows) {
+                            *reinterpret_cast<uint4 *>(p + (int64_t) (4 * st) * nb2) = w[st];
                         }
                     }
                 } else {
-                    uint16_t *p = reinterpret_cast<uint16_t *>(out) + 32 * ch;
-                    uint32_t  y[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        y[e] = pack2<BF16>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-                    }
-                    if (P.vec) {
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            *reinterpret_cast<uint4 *>(p + 2 * e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            p[2 * e]     = (uint16_t) y[e];
-                            p[2 * e + 1] = (uint16_t) (y[e] >> 16);
+                    for (int st = 0; st < 8; ++st) {
+                        const uint32_t y[4] = {w[st].x, w[st].y, w[st].z, w[st].w};
+                        if (4 * st + (ln >> 3) < rows) {
+                            for (int e = 0; e < 4; ++e) {
+                                char *pe = p + (int64_t) (4 * st) * nb2 + 4 * e;
+                                if (f32) {
+                                    *reinterpret_cast<uint32_t *>(pe) = y[e];
+                                } else {
+                                    reinterpret_cast<uint16_t *>(pe)[0] = (uint16_t) y[e];
+                                    reinterpret_cast<uint16_t *>(pe)[1] = (uint16_t) (y[e] >> 16);
+                                }
+                            }
                         }
                     }
                 }
-                __syncwarp();
+                __syncwarp();  // the slab has been read
+            };
+            uint32_t x[2][32];
+            tmem_ld32(tO, x[0]);
+            tmem_ld32(tO + 32, x[1]);
+#pragma unroll
+            for (int n = 0; n < HD / 64; ++n) {  // 64 dims at a time
+                tmem_ld_wait32(x[0]);
+                tmem_ld_wait32(x[1]);
+                finished(x[0]);
+                finished(x[1]);
+                if (P.dst_type == ACEFA_TYPE_F32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            st_shared_v4(slab + ln * 128 + ((e ^ (ln & 7)) << 4), x[h][4 * e], x[h][4 * e + 1],
+                                         x[h][4 * e + 2], x[h][4 * e + 3]);
+                        }
+                        write_slab(2 * n + h, true);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int d = 8 * (e & 3) + 2 * w;
+                            y[w] = pack2<BF16>(__uint_as_float(x[e >> 2][d]), __uint_as_float(x[e >> 2][d + 1]));
+                        }
+                        st_shared_v4(slab + ln * 128 + ((e ^ (ln & 7)) << 4), y[0], y[1], y[2], y[3]);
+                    }
+                }
+                if (n + 1 < HD / 64) {  // on their way while this piece is written
+                    tmem_ld32(tO + 64, x[0]);
+                    tmem_ld32(tO + 96, x[1]);
+                }
+                if (P.dst_type != ACEFA_TYPE_F32) {
+                    write_slab(n, false);
+                }
             }
             tc_fence_before();  // O has been read before the next unit's P is announced
         }
@@ -813,7 +949,9 @@ extern "C" ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const ac
     p.d_nb1 = (int64_t) dst->nb[1], p.d_nb2 = (int64_t) dst->nb[2];
     p.cu_q = cu_q, p.cu_k = cu_k ? cu_k : cu_q;
     p.n_seq = n_seq, p.rows_q = (int) rows_q, p.rows_kv = (int) rows_kv;
-    p.Hq = (int) Hq, p.Hkv = (int) Hkv;
+    p.Hkv = (int) Hkv, p.G = (int) (Hq / Hkv);
+    auto inverse = [](int d) { return d == 1 ? 0xFFFFFFFFu : (uint32_t) ((1ull << 32) / (uint64_t) d); };
+    p.inv_hkv = inverse(p.Hkv), p.inv_g = inverse(p.G);
     p.mask = mask, p.window = window;
     p.dst_type      = dst->type;
     p.vec           = ((reinterpret_cast<uintptr_t>(dst->data) | dst->nb[1] | dst->nb[2]) & 15u) == 0;
