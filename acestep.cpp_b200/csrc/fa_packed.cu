@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *s_tmem, 0);
     pdl_wait_primary();
 
     auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
@@ -451,124 +451,127 @@ __global__ void __launch_bounds__(kThreads, 1)
                             ks > 0 || acc ? 1u : 0u);
                 }
             };
-            // The steps (unit, key tile) in order; `n` is one step ahead of `c`.
-            struct Step {
-                bool live[2], first[2], last[2];  // of tile i in this unit
-                bool new_q, end_q;                // first / last step of its unit
-            };
-            Unit t;
-            int  k = 0, j = 0, n_unit = 0, use = 0;
-            bool have = false, ok = true;
-            uint32_t p_ph[2] = {0u, 0u};
-            auto enter_unit = [&]() {
-                do {
-                    have = next_unit(k, t);
-                } while (have && t.ja == t.jb);
-                j = t.ja;
-            };
-            auto step_here = [&](Step &s) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    s.live[i]  = j >= t.a[i] && j < t.b[i];
-                    s.first[i] = j == t.a[i];
-                    s.last[i]  = j == t.b[i] - 1;
-                }
-                s.new_q  = j == t.ja;
-                s.end_q  = j == t.jb - 1;
-            };
-            auto advance = [&]() {
-                if (++j == t.jb) {
-                    enter_unit();
-                }
-            };
-            // S of tile i for the step whose K is in ring position 2 * pos
-            auto start_s = [&](const Step &s, int i, int pos, bool &waited) {
-                if (!waited) {
-                    if (s.new_q) {
-                        ok = wait(q_full, (uint32_t) (n_unit & 1), DEVERR_TIMEOUT_FULL);
+            // One thread walks the steps (unit, key tile) alone: this loop's own
+            // instructions are time in which the tensor core runs dry.
+            if (lane == 0) {
+                int  k = 0, n_unit = 0;
+                bool ok = true;
+                Unit t;
+                // the next unit with keys; t.more = 0 behind the last or on expiry
+                auto enter_unit = [&]() {
+                    do {
+                        const int slot = k % kUnitRing;
+                        ok             = wait(&u_full[slot], (uint32_t) (k / kUnitRing), DEVERR_TIMEOUT_FULL);
+                        t              = units[slot];
+                        mbar_arrive(&u_empty[slot]);
+                        ++k;
+                        t.more = ok ? t.more : 0;
+                    } while (t.more && t.ja == t.jb);
+                };
+                // K of the step at ring position pos (and, in a new unit, Q) has landed
+                auto wait_k = [&](bool new_q, int pos) {
+                    if (new_q) {
+                        ok = ok && wait(q_full, (uint32_t) n_unit, DEVERR_TIMEOUT_FULL);
                         ++n_unit;
                     }
-                    ok = ok && wait(&full[2 * pos % kRing], (uint32_t) (2 * pos / kRing), DEVERR_TIMEOUT_FULL);
-                    waited = true;
-                    if (!ok) {
-                        return;
-                    }
+                    ok = ok && wait(&full[pos % kRing], (uint32_t) (pos / kRing), DEVERR_TIMEOUT_FULL);
                     tc_fence_after();
-                }
-                if (s.live[i]) {
-                    issue_s(i, 2 * pos % kRing);
-                }
-            };
-            auto end_s = [&](const Step &s, int pos) {
-                tc_commit(&empty[2 * pos % kRing]);
-                if (s.end_q) {
-                    tc_commit(q_empty);
-                }
-            };
-            enter_unit();
-            Step c, n;
-            if (have) {
-                step_here(c);
-                if (lane == 0) {
-                    bool waited = false;
-                    start_s(c, 0, 0, waited);
-                    if (ok) {
-                        start_s(c, 1, 0, waited);
-                        end_s(c, 0);
-                    }
-                }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-            }
-            while (ok && have) {
-                advance();
-                if (have) {
-                    step_here(n);
-                }
-                if (lane == 0) {
-                    const int vpos = 2 * use + 1, vslot = vpos % kRing;
-                    bool      waited = false;
-                    ok = wait(&full[vslot], (uint32_t) (vpos / kRing), DEVERR_TIMEOUT_FULL);
+                };
+                auto do_pv = [&](int i, uint32_t ph, int vslot, bool first, bool last) {
+                    ok = ok && wait(&p_half[i], ph, DEVERR_TIMEOUT_MMA);
                     tc_fence_after();
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (ok && c.live[i]) {
-                            ok = wait(&p_half[i], p_ph[i], DEVERR_TIMEOUT_MMA);
-                            if (ok) {
-                                tc_fence_after();
-                                issue_pv(i, 0, vslot, !c.first[i]);
-                                ok = wait(&p_ready[i], p_ph[i], DEVERR_TIMEOUT_MMA);
-                            }
-                            p_ph[i] ^= 1u;
-                            if (ok) {
-                                tc_fence_after();
-                                issue_pv(i, 1, vslot, true);
-                                if (c.last[i]) {
-                                    tc_commit(&o_done[i]);
-                                }
-                            }
-                        }
-                        // S of the next step between the tiles' PVs; a new unit's
-                        // waits for its Q, so there both PVs go first
-                        if (ok && have && !n.new_q) {
-                            start_s(n, i, use + 1, waited);
-                        }
-                    }
-                    if (ok && have && n.new_q) {
-                        start_s(n, 0, use + 1, waited);
-                        if (ok) {
-                            start_s(n, 1, use + 1, waited);
-                        }
-                    }
                     if (ok) {
+                        issue_pv(i, 0, vslot, !first);
+                    }
+                    ok = ok && wait(&p_ready[i], ph, DEVERR_TIMEOUT_MMA);
+                    tc_fence_after();
+                    if (ok) {
+                        issue_pv(i, 1, vslot, true);
+                        if (last) {
+                            tc_commit(&o_done[i]);
+                        }
+                    }
+                };
+                uint32_t ph0 = 0u, ph1 = 0u;
+                int      pos = 0;  // ring position of the step's K; its V is pos + 1
+                enter_unit();
+                int  j = t.ja;
+                bool l0 = false, l1 = false;  // tiles that see this key tile
+                if (t.more) {
+                    l0 = j >= t.a[0] && j < t.b[0], l1 = j >= t.a[1] && j < t.b[1];
+                    wait_k(true, 0);
+                    if (ok && l0) {
+                        issue_s(0, 0);
+                    }
+                    if (ok && l1) {
+                        issue_s(1, 0);
+                    }
+                    tc_commit(&empty[0]);
+                    if (j + 1 == t.jb) {
+                        tc_commit(q_empty);
+                    }
+                }
+                while (ok && t.more) {
+                    const bool f0 = j == t.a[0], f1 = j == t.a[1], e0 = j + 1 == t.b[0], e1 = j + 1 == t.b[1];
+                    const int  vslot = (pos + 1) % kRing, vph = (pos + 1) / kRing;
+                    ++j;
+                    const bool new_q = j == t.jb;
+                    if (new_q) {
+                        enter_unit();
+                        j = t.ja;
+                    }
+                    const bool more = t.more != 0;
+                    const bool n0   = more && j >= t.a[0] && j < t.b[0], n1 = more && j >= t.a[1] && j < t.b[1];
+                    const int  kslot = (pos + 2) % kRing;
+                    ok = ok && wait(&full[vslot], (uint32_t) vph, DEVERR_TIMEOUT_FULL);
+                    tc_fence_after();
+                    if (more && !new_q) {
+                        // S of the next step between the tiles' PVs
+                        if (l0) {
+                            do_pv(0, ph0, vslot, f0, e0);
+                            ph0 ^= 1u;
+                        }
+                        wait_k(false, pos + 2);
+                        if (ok && n0) {
+                            issue_s(0, kslot);
+                        }
+                        if (l1) {
+                            do_pv(1, ph1, vslot, f1, e1);
+                            ph1 ^= 1u;
+                        }
+                        if (ok && n1) {
+                            issue_s(1, kslot);
+                        }
                         tc_commit(&empty[vslot]);
-                        if (have) {
-                            end_s(n, use + 1);
+                        tc_commit(&empty[kslot]);
+                    } else {
+                        // the end of a unit: the next one's S waits for its Q, so both PVs go first
+                        if (l0) {
+                            do_pv(0, ph0, vslot, f0, e0);
+                            ph0 ^= 1u;
+                        }
+                        if (l1) {
+                            do_pv(1, ph1, vslot, f1, e1);
+                            ph1 ^= 1u;
+                        }
+                        tc_commit(&empty[vslot]);
+                        if (more) {
+                            wait_k(true, pos + 2);
+                            if (ok && n0) {
+                                issue_s(0, kslot);
+                            }
+                            if (ok && n1) {
+                                issue_s(1, kslot);
+                            }
+                            tc_commit(&empty[kslot]);
                         }
                     }
+                    if (more && j + 1 == t.jb) {
+                        tc_commit(q_empty);
+                    }
+                    l0 = n0, l1 = n1;
+                    pos += 2;
                 }
-                ++use;
-                c  = n;
-                ok = __shfl_sync(0xffffffffu, ok, 0);
             }
             if (lane == 0) {
                 // every MMA issued by this thread completes before TMEM is released
