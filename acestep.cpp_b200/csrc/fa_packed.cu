@@ -14,7 +14,10 @@
 // a causal sequence see the most keys) and dealt out back and forth, and the
 // warps' pipelines run on across pairs -- the next pair's Q, K and V arrive and
 // its first S is computed while this pair's output is still being written.
-//   warp 0      TMA: Q (2 x 32 KB), K and V tiles (4 x 32 KB ring)
+//   warp 0      TMA: Q (2 x 32 KB) and the key tiles (2 x 32 KB of K and of V).  Tile
+//               x's V and tile x + 1's K are awaited and given back together: they
+//               serve the same step of the tensor core, and a barrier less per
+//               step is time in which it does not run dry.
 //   warp 1      MMA issue (one thread); owns TMEM: O0 | O1 | S0 | S1
 //   warp 3      finds the CTA's units and hands them to the others through a ring
 //   warp 2      where a sequence ends inside a V tile, zeroes its rows behind the
@@ -55,7 +58,7 @@ constexpr int      kOffRing   = 2 * kTileBytes;  // Q tiles first
 constexpr int      kOffBars   = kOffRing + kRing * kTileBytes;
 constexpr int      kUnitRing  = 4;                       // units known ahead
 constexpr int      kUnitReaders = 11;                    // warps that read them: all but the one that finds them
-constexpr int      kNumBars   = 2 * kRing + 2 * 4 + 5 + 2 * kUnitRing;
+constexpr int      kNumBars   = 2 * 2 + 2 * 4 + 5 + 2 * kUnitRing;
 constexpr int      kOffMisc   = kOffBars + kNumBars * 8;
 constexpr int      kOffUnits  = (kOffMisc + 16 + 15) / 16 * 16;
 constexpr int      kOffOut    = kOffUnits + kUnitRing * 64;  // where each softmax warp's rows go
@@ -257,13 +260,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t      *smem    = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint64_t     *full    = reinterpret_cast<uint64_t *>(smem + kOffBars);
-    uint64_t     *empty   = full + kRing;
-    uint64_t     *s_ready = empty + kRing;   // S of tile i is in TMEM
+    uint64_t     *full    = reinterpret_cast<uint64_t *>(smem + kOffBars);  // [2] V of a tile and K of the next are there
+    uint64_t     *empty   = full + 2;
+    uint64_t     *s_ready = empty + 2;       // S of tile i is in TMEM
     uint64_t     *p_ready = s_ready + 2;     // P of tile i is in TMEM
     uint64_t     *p_half  = p_ready + 2;     // its first 64 keys are
     uint64_t     *o_done  = p_half + 2;      // O of tile i is complete (once per unit)
-    uint64_t     *q_full  = o_done + 2;      // the unit's Q has landed
+    uint64_t     *q_full  = o_done + 2;      // the unit's Q has landed (and the very first K)
     uint64_t     *q_empty = q_full + 1;      // its last S is computed
     uint64_t     *ragged  = q_empty + 1;     // [2] a V tile with rows behind the sequence's end has landed
     uint64_t     *fin     = ragged + 2;
@@ -279,11 +282,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_relinquish();
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kRing; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&full[i], 2);  // one arrival for V, one for K
+            mbar_init(&empty[i], 1);
             mbar_init(&s_ready[i], 1);
             mbar_init(&p_ready[i], 128);
             mbar_init(&p_half[i], 128);
@@ -356,9 +357,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == 0) {
             // ============================ TMA producer ============================
-            // A V tile that ends behind its sequence signals `ragged` of its ring
-            // position; warp 2 passes it on to `full` when it is clean.
-            int  use = 0, n_unit = 0, n_rag0 = 0, n_rag1 = 0, k = 0;
+            // A V tile that ends behind its sequence signals `ragged` of its
+            // buffer; warp 2 passes it on to `full` when it is clean.
+            int  x = 0, n_unit = 0, n_rag0 = 0, n_rag1 = 0, k = 0;  // x: key tiles so far
             bool ok = true;
             Unit t;
             while (ok && next_unit(k, t)) {
@@ -366,10 +367,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                     continue;
                 }
                 if (lane == 0) {
-                    const bool two = t.row0[1] < t.n_q;  // (the first tile is there in every unit)
-                    ok = wait(q_empty, (uint32_t) (n_unit & 1) ^ 1u, DEVERR_TIMEOUT_EMPTY);
+                    const bool     two     = t.row0[1] < t.n_q;  // (the first tile is there in every unit)
+                    const uint32_t q_bytes = (uint32_t) (kBM * HD * 2) * (two ? 2u : 1u);
+                    auto load_k = [&](int j, uint64_t *bar) {
+#pragma unroll
+                        for (int e = 0; e < HD / 64; ++e) {
+                            tma_load_3d(smem + kOffRing + (x & 1) * 2 * kTileBytes + e * (kBN * 128), &kmap, 64 * e,
+                                        t.k0 + j * kBN, t.hk, bar);
+                        }
+                    };
+                    if (x > 0) {  // its place was free when the previous V went out
+                        mbar_arrive_expect_tx(&full[(x - 1) & 1], kBN * HD * 2);
+                        load_k(t.ja, &full[(x - 1) & 1]);
+                    }
+                    ok = wait(q_empty, (uint32_t) n_unit ^ 1u, DEVERR_TIMEOUT_EMPTY);
                     if (ok) {
-                        mbar_arrive_expect_tx(q_full, (uint32_t) (kBM * HD * 2) * (two ? 2u : 1u));
+                        mbar_arrive_expect_tx(q_full, q_bytes + (x > 0 ? 0u : (uint32_t) (kBN * HD * 2)));
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -380,36 +393,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 }
                             }
                         }
+                        if (x == 0) {
+                            load_k(t.ja, q_full);
+                        }
                     }
                     for (int j = t.ja; j < t.jb && ok; ++j) {
-                        for (int h = 0; h < 2 && ok; ++h) {
-                            const int seq = 2 * use + h, buf = seq % kRing, ph = (seq / kRing) & 1;
-                            ok = wait(&empty[buf], (uint32_t) ph ^ 1u, DEVERR_TIMEOUT_EMPTY);
-                            if (!ok) {
-                                break;
-                            }
-                            uint8_t           *dst = smem + kOffRing + buf * kTileBytes;
-                            const CUtensorMap *map = h ? &vmap : &kmap;
-                            const bool         rag = h && t.n_k < (j + 1) * kBN;
-                            uint64_t          *bar = rag ? &ragged[buf >> 1] : &full[buf];
-                            n_rag0 += rag && buf == 1;
-                            n_rag1 += rag && buf == 3;
-                            mbar_arrive_expect_tx(bar, kBN * HD * 2);
-#pragma unroll
-                            for (int e = 0; e < HD / 64; ++e) {
-                                tma_load_3d(dst + e * (kBN * 128), map, 64 * e, t.k0 + j * kBN, t.hk, bar);
-                            }
+                        const int b = x & 1;
+                        // (the very first K counts as a pair of its own before empty[1]'s others)
+                        ok = wait(&empty[b], (uint32_t) (x >> 1) ^ (b ? 0u : 1u), DEVERR_TIMEOUT_EMPTY);
+                        if (!ok) {
+                            break;
                         }
-                        ++use;
+                        const bool rag = t.n_k < (j + 1) * kBN;
+                        uint64_t  *bar = rag ? &ragged[b] : &full[b];
+                        n_rag0 += rag && b == 0;
+                        n_rag1 += rag && b == 1;
+                        mbar_arrive_expect_tx(bar, kBN * HD * 2);
+#pragma unroll
+                        for (int e = 0; e < HD / 64; ++e) {
+                            tma_load_3d(smem + kOffRing + (2 * b + 1) * kTileBytes + e * (kBN * 128), &vmap, 64 * e,
+                                        t.k0 + j * kBN, t.hk, bar);
+                        }
+                        ++x;
+                        if (j + 1 < t.jb) {
+                            mbar_arrive_expect_tx(&full[b], kBN * HD * 2);
+                            load_k(j + 1, &full[b]);
+                        }
                     }
                 }
                 ++n_unit;
                 ok = __shfl_sync(0xffffffffu, ok, 0);
             }
+            if (lane == 0 && x > 0) {
+                mbar_arrive(&full[(x - 1) & 1]);  // no K goes with the last V
+            }
             if (*abort_f && lane == 0) {
                 // Let the copies in flight land before the CTA exits: the last of
-                // every barrier that this thread announced (a full barrier whose
-                // tile warp 2 was to pass on may stay open; the wait is bounded).
+                // every barrier that this thread announced (one that waits for
+                // warp 2 or for a copy never started may stay open; the wait is bounded).
                 const uint64_t ts = globaltimer_ns();
                 auto drain = [&](uint64_t *bar, int n) {  // n phases announced
                     while (n > 0 && !mbar_try_wait(bar, (uint32_t) (n - 1) & 1u)) {
@@ -422,9 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 drain(q_full, n_unit);
                 drain(&ragged[0], n_rag0);
                 drain(&ragged[1], n_rag1);
-                for (int i = 0; i < kRing; ++i) {
-                    drain(&full[i], (2 * use + kRing - 1 - i) / kRing);
-                }
+                drain(&full[0], (x + 1) >> 1);
+                drain(&full[1], x >> 1);
             }
         } else if (warp == 1) {
             // ============================ MMA issuer ==============================
@@ -468,13 +488,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         t.more = ok ? t.more : 0;
                     } while (t.more && t.ja == t.jb);
                 };
-                // K of the step at ring position pos (and, in a new unit, Q) has landed
-                auto wait_k = [&](bool new_q, int pos) {
-                    if (new_q) {
-                        ok = ok && wait(q_full, (uint32_t) n_unit, DEVERR_TIMEOUT_FULL);
-                        ++n_unit;
-                    }
-                    ok = ok && wait(&full[pos % kRing], (uint32_t) (pos / kRing), DEVERR_TIMEOUT_FULL);
+                auto wait_q = [&]() {
+                    ok = ok && wait(q_full, (uint32_t) n_unit, DEVERR_TIMEOUT_FULL);
+                    ++n_unit;
                     tc_fence_after();
                 };
                 auto do_pv = [&](int i, uint32_t ph, int vslot, bool first, bool last) {
@@ -493,27 +509,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 };
                 uint32_t ph0 = 0u, ph1 = 0u;
-                int      pos = 0;  // ring position of the step's K; its V is pos + 1
+                int      x = 0;  // key tiles so far; K of tile x is in ring slot 2 * (x & 1), V behind it
                 enter_unit();
                 int  j = t.ja;
                 bool l0 = false, l1 = false;  // tiles that see this key tile
                 if (t.more) {
                     l0 = j >= t.a[0] && j < t.b[0], l1 = j >= t.a[1] && j < t.b[1];
-                    wait_k(true, 0);
+                    wait_q();
                     if (ok && l0) {
                         issue_s(0, 0);
                     }
                     if (ok && l1) {
                         issue_s(1, 0);
                     }
-                    tc_commit(&empty[0]);
+                    tc_commit(&empty[1]);
                     if (j + 1 == t.jb) {
                         tc_commit(q_empty);
                     }
                 }
                 while (ok && t.more) {
                     const bool f0 = j == t.a[0], f1 = j == t.a[1], e0 = j + 1 == t.b[0], e1 = j + 1 == t.b[1];
-                    const int  vslot = (pos + 1) % kRing, vph = (pos + 1) / kRing;
+                    const int  b = x & 1, vslot = 2 * b + 1, kslot = 2 * (b ^ 1);
                     ++j;
                     const bool new_q = j == t.jb;
                     if (new_q) {
@@ -522,16 +538,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const bool more = t.more != 0;
                     const bool n0   = more && j >= t.a[0] && j < t.b[0], n1 = more && j >= t.a[1] && j < t.b[1];
-                    const int  kslot = (pos + 2) % kRing;
-                    ok = ok && wait(&full[vslot], (uint32_t) vph, DEVERR_TIMEOUT_FULL);
+                    ok = ok && wait(&full[b], (uint32_t) (x >> 1), DEVERR_TIMEOUT_FULL);
                     tc_fence_after();
-                    if (more && !new_q) {
+                    if (!new_q) {
                         // S of the next step between the tiles' PVs
                         if (l0) {
                             do_pv(0, ph0, vslot, f0, e0);
                             ph0 ^= 1u;
                         }
-                        wait_k(false, pos + 2);
                         if (ok && n0) {
                             issue_s(0, kslot);
                         }
@@ -542,8 +556,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (ok && n1) {
                             issue_s(1, kslot);
                         }
-                        tc_commit(&empty[vslot]);
-                        tc_commit(&empty[kslot]);
                     } else {
                         // the end of a unit: the next one's S waits for its Q, so both PVs go first
                         if (l0) {
@@ -554,23 +566,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                             do_pv(1, ph1, vslot, f1, e1);
                             ph1 ^= 1u;
                         }
-                        tc_commit(&empty[vslot]);
                         if (more) {
-                            wait_k(true, pos + 2);
+                            wait_q();
                             if (ok && n0) {
                                 issue_s(0, kslot);
                             }
                             if (ok && n1) {
                                 issue_s(1, kslot);
                             }
-                            tc_commit(&empty[kslot]);
                         }
                     }
+                    tc_commit(&empty[b]);
                     if (more && j + 1 == t.jb) {
                         tc_commit(q_empty);
                     }
                     l0 = n0, l1 = n1;
-                    pos += 2;
+                    ++x;
                 }
             }
             if (lane == 0) {
@@ -586,35 +597,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else if (warp == 2) {
             // ==================== V rows behind the sequence's end =================
-            int  use = 0, n_rag0 = 0, n_rag1 = 0, k = 0;
-            bool ok  = true;
+            int  x = 0, n_rag0 = 0, n_rag1 = 0, k = 0;
+            bool ok = true;
             Unit t;
             while (ok && next_unit(k, t)) {
-                const int n_it = t.jb - t.ja;
-                if (n_it && t.n_k < t.jb * kBN) {
-                    const int buf = (2 * (use + n_it - 1) + 1) % kRing;
-                    ok = __all_sync(0xffffffffu, wait(&ragged[buf >> 1], (uint32_t) (buf == 1 ? n_rag0 : n_rag1),
-                                                      DEVERR_TIMEOUT_FULL));
-                    n_rag0 += buf == 1;
-                    n_rag1 += buf == 3;
+                x += t.jb - t.ja;
+                if (t.ja < t.jb && t.n_k < t.jb * kBN) {
+                    const int b = (x - 1) & 1;  // the unit's last tile
+                    ok = __all_sync(0xffffffffu, wait(&ragged[b], (uint32_t) (b ? n_rag1 : n_rag0), DEVERR_TIMEOUT_FULL));
+                    n_rag0 += b == 0;
+                    n_rag1 += b == 1;
                     if (ok) {
                         // a row is 128 contiguous bytes of each 64-dim box (the swizzle stays inside them)
                         const int valid = t.n_k - (t.jb - 1) * kBN;
 #pragma unroll
                         for (int e = 0; e < HD / 64; ++e) {
-                            uint4 *p = reinterpret_cast<uint4 *>(smem + kOffRing + buf * kTileBytes + e * (kBN * 128));
-                            for (int x = valid * 8 + lane; x < kBN * 8; x += 32) {
-                                p[x] = make_uint4(0u, 0u, 0u, 0u);
+                            uint4 *p = reinterpret_cast<uint4 *>(smem + kOffRing + (2 * b + 1) * kTileBytes + e * (kBN * 128));
+                            for (int y = valid * 8 + lane; y < kBN * 8; y += 32) {
+                                p[y] = make_uint4(0u, 0u, 0u, 0u);
                             }
                         }
                         fence_proxy_async_smem();  // read next by the tensor core
                         __syncwarp();
                         if (lane == 0) {
-                            mbar_arrive(&full[buf]);
+                            mbar_arrive(&full[b]);
                         }
                     }
                 }
-                use += n_it;
             }
         }
     } else {
