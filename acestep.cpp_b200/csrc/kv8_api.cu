@@ -186,7 +186,7 @@ int plan_attn(const acefa_tensor *q, const acefa_kv8_cache *cache, const acefa_t
     p.n_rb      = (p.rows + R - 1) / R;
     const int64_t units = (int64_t) p.c.B * p.c.Hkv * p.n_rb;
     const int64_t tiles = units * ((p.c.n_max + kKv8Block - 1) / kKv8Block);
-    const int64_t weigh = weight ? (int64_t) p.c.B * p.c.Hkv * (p.c.n_max / 1024 + 1) : 0;
+    const int64_t weigh = weight ? (int64_t) p.c.B * p.c.Hkv * (p.c.n_max / 512 + 1) : 0;
     if (tiles >= (1ll << 31) || units * R + weigh >= (1ll << 31)) {
         return ACEFA_ERR_SHAPE;
     }
@@ -194,7 +194,7 @@ int plan_attn(const acefa_tensor *q, const acefa_kv8_cache *cache, const acefa_t
     if ((rc = device_ctx(&ctx)) != ACEFA_OK) {
         return rc;
     }
-    p.n_cta           = (int) std::min<int64_t>(tiles, (int64_t) ctx.sm_count * kv8_attn_ctas_per_sm(p.c.D, R));
+    p.n_cta           = (int) std::min<int64_t>(tiles, (int64_t) ctx.sm_count * kv8_attn_ctas_per_sm(R));
     p.score_stride    = std::min(R, (p.rows + 1) & ~1);
     plan->part_bytes  = ((size_t) (p.n_cta + units) * kv8_slot_floats(p.c.D, R) * sizeof(float) + 255) / 256 * 256;
     plan->ws_bytes    = plan->part_bytes +

@@ -5,11 +5,14 @@
 // Mathematics.  With K = kd * k8 and V = vd * v8 (one kd, vd per 64 keys),
 //   s_rj = scale * kd_j * (q_r . k8_j),   p_rj = exp(s_rj - m_r),
 //   o_r  = sum_j vd_j p_rj v8_j / sum_j p_rj.
-// k8 and v8 are integers below 128, exact in F16.  q_r (scaled by a power of
-// two into F16's range) and p_rj are split into two F16 numbers each, which
-// together keep 22 bits, so that the F16 tensor-core products with F32 sums
-// lose nothing beside F32 arithmetic; the scales multiply in F32: kd on the
-// finished score, vd on the 16-key partial product of V.
+// k8 and v8 are integers below 128, exact in F16.  An F32 q_r (scaled by a power
+// of two into F16's range) and the p_rj of an F32 output are split into two F16
+// numbers each, which together keep 22 bits, so that the F16 tensor-core
+// products with F32 sums lose nothing beside F32 arithmetic (a 16-bit q_r is
+// exact in one, and one rounding of p_rj to 11 bits is below a 16-bit output's
+// own); the scales multiply in F32: kd on the finished score, vd on the 16-key
+// partial product of V.  Up to four rows, the two halves of a split operand
+// ride in one product as columns r and r + 4 of its eight.
 //
 // Work.  The (set, KV head, row block) units' 64-key tiles, numbered one after
 // another over all sets' actual lengths, are cut into equal runs, one per CTA:
@@ -24,6 +27,8 @@
 // S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
 // operand layout by four movmatrix.  The running maximum moves only when a
 // score exceeds it by more than 2^8 (a warp vote), as in the other kernels.
+#include <type_traits>
+
 #include "kv8_internal.h"
 #include "ptx.cuh"
 
@@ -42,16 +47,21 @@ template <int HD>
 constexpr int stage_bytes() {
     return 2 * kChunk * HD + 256;
 }
-constexpr int kStages = 4;
+constexpr int kStages = 3;
 template <int HD, int NT>
 constexpr int merge_floats() {
     return kWarps * 8 * NT * (HD + 4) + kWarps * 8 * NT * 2;
 }
 template <int HD, int NT>
-constexpr int attn_smem_bytes() {
-    return kWarps * kStages * stage_bytes<HD>() + 4 * merge_floats<HD, NT>() + 4 * (kKv8MaxSets + 4);
+constexpr int attn_smem_bytes(int B) {  // + the sets' tile table and lengths
+    return kWarps * kStages * stage_bytes<HD>() + 4 * merge_floats<HD, NT>() + 4 * (2 * B + 2);
 }
-constexpr int ctas_per_sm(int HD, int NT) { return HD == 128 && NT == 2 ? 2 : 2; }
+constexpr int ctas_per_sm(int NT) { return NT == 2 ? 2 : 3; }
+
+// How operands of more than 11 bits enter the products.
+constexpr int kOne    = 0;  // one F16 number (16-bit Q and output)
+constexpr int kSplit  = 1;  // two, in products of their own
+constexpr int kPacked = 2;  // two, as columns r and r + 4 (up to four rows)
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -105,10 +115,34 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo              = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-__device__ __forceinline__ float load1(const char *p, int type, int e) {
-    return type == ACEFA_TYPE_F32   ? reinterpret_cast<const float *>(p)[e]
-           : type == ACEFA_TYPE_F16 ? __half2float(reinterpret_cast<const __half *>(p)[e])
-                                    : __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[e]);
+// Four values of a Q row from element e on (zeros without a row).
+__device__ __forceinline__ void load_q4(const char *p, int type, int e, float (&x)[4]) {
+    if (!p) {
+        x[0] = x[1] = x[2] = x[3] = 0.0f;
+    } else if (type == ACEFA_TYPE_F32) {
+        const float *f = reinterpret_cast<const float *>(p) + e;
+        if ((reinterpret_cast<uintptr_t>(f) & 15u) == 0) {
+            const float4 v = *reinterpret_cast<const float4 *>(f);
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else {
+            x[0] = f[0], x[1] = f[1], x[2] = f[2], x[3] = f[3];
+        }
+    } else {
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p) + e;
+        uint32_t        w[2];
+        if ((reinterpret_cast<uintptr_t>(h) & 7u) == 0) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(h);
+            w[0] = v.x, w[1] = v.y;
+        } else {
+            w[0] = h[0] | (uint32_t) h[1] << 16;
+            w[1] = h[2] | (uint32_t) h[3] << 16;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint16_t b = (uint16_t) (w[k >> 1] >> (16 * (k & 1)));
+            x[k] = type == ACEFA_TYPE_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t) b << 16);
+        }
+    }
 }
 __device__ __forceinline__ void store1(char *p, int type, int e, float x) {
     if (type == ACEFA_TYPE_F32) {
@@ -121,13 +155,14 @@ __device__ __forceinline__ void store1(char *p, int type, int e, float x) {
 }
 
 // base[b] = 64-key tiles of the sets before b, b = 0 .. B (the last is the
-// total per head and row block).  All threads; ends with a barrier.
-__device__ __forceinline__ void tile_table(int *base, const int32_t *len, int B, int n_max) {
+// total per head and row block), lens[b] = length.  All threads; ends with a barrier.
+__device__ __forceinline__ void tile_table(int *base, int *lens, const int32_t *len, int B, int n_max) {
     const int lane = threadIdx.x & 31;
     if (threadIdx.x < 32) {
         int acc = 0;
         for (int b0 = 0; b0 < B; b0 += 32) {
-            int v = b0 + lane < B ? (clamp_len(__ldg(len + b0 + lane), n_max) + kKv8Block - 1) / kKv8Block : 0;
+            const int n = b0 + lane < B ? clamp_len(__ldg(len + b0 + lane), n_max) : 0;
+            int       v = (n + kKv8Block - 1) / kKv8Block;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const int u = __shfl_up_sync(0xffffffffu, v, off);
@@ -135,6 +170,7 @@ __device__ __forceinline__ void tile_table(int *base, const int32_t *len, int B,
             }
             if (b0 + lane < B) {
                 base[b0 + lane + 1] = acc + v;
+                lens[b0 + lane]     = n;
             }
             acc += __shfl_sync(0xffffffffu, v, 31);
         }
@@ -158,8 +194,8 @@ struct Walk {
     const float *ks, *vs;       // its scales
 };
 
-template <int HD, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
+template <int HD, int NT, int MODE>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
     kv8_attn_kernel(const __grid_constant__ Kv8AttnParams P) {
     constexpr int R    = 8 * NT;
     constexpr int KS   = HD / 16;             // k-steps of S, m-tiles of O
@@ -169,13 +205,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
     float *s_o    = reinterpret_cast<float *>(smem + kWarps * kStages * kSt);  // [warp][R][kOut]
     float *s_ml   = s_o + kWarps * R * kOut;                                   // [warp][R][2]
     int   *s_base = reinterpret_cast<int *>(s_ml + kWarps * R * 2);
+    int   *s_len  = s_base + P.c.B + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     const int HU = P.c.Hkv * P.n_rb;  // units of a set
 
     pdl_wait_primary();
-    tile_table(s_base, P.len, P.c.B, P.c.n_max);
+    tile_table(s_base, s_len, P.len, P.c.B, P.c.n_max);
     const int T = s_base[P.c.B] * HU;
     const int C = min((int) gridDim.x, T);
     pdl_launch_dependents();
@@ -195,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
     };
     auto enter_set = [&](Walk &w) {
         w.nt  = s_base[w.b + 1] - s_base[w.b];
-        w.len = clamp_len(__ldg(P.len + w.b), P.c.n_max);
+        w.len = s_len[w.b];
     };
     auto advance = [&](Walk &w) {  // true: a new unit
         if (++w.t < w.nt) {
@@ -268,33 +305,49 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
         }
     };
 
+    // This thread's row of Q of a unit (kPacked: rows 4 .. 7 are the low halves of 0 .. 3), or nullptr
+    auto q_row = [&](const Walk &w, int nt, int &row) -> const char * {
+        const int hk = w.ub / P.n_rb;
+        row          = w.ub % P.n_rb * R + nt * 8 + (MODE == kPacked ? g & 3 : g);
+        return row < P.rows ? P.q.data + (int64_t) (row / P.G) * P.q.nb1 + (int64_t) (hk * P.G + row % P.G) * P.q.nb2 +
+                                  (int64_t) w.b * P.q.nb3
+                            : nullptr;
+    };
+    auto prefetch_rows = [&](const Walk &w) {  // on its way to L1 while the unit before is computed
+        if (w.b < P.c.B) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                int         row;
+                const char *p = q_row(w, nt, row);
+                if (p && warp == 0) {
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(p + (P.q.type == ACEFA_TYPE_F32 ? HD : HD / 2) * c));
+                }
+            }
+        }
+    };
+
     // ---- rows of the current unit
-    uint32_t qh[NT][KS][2], ql[NT][KS][2];  // Q^T operand, high and low halves
+    uint32_t qh[NT][KS][2], ql[MODE == kSplit ? NT : 1][KS][2];  // Q^T operand, its (other) half
     float    mul[NT][2];                    // log2-unit score per unit of accumulator, rows 2c and 2c + 1
     int      lim[NT][2];                    // keys those rows see
     float    acc_o[NT][KS][4];
     float    m[NT][2], l[NT][2];
     auto load_rows = [&]() {
-        const int hk = at.ub / P.n_rb, rb = at.ub % P.n_rb;
+        const int rb = at.ub % P.n_rb;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int   row = rb * R + nt * 8 + g;
+            int         row;
+            const char *p = q_row(at, nt, row);
             float       x[KS][4];
             float       top = 0.0f;
-            const bool  on  = row < P.rows;
-            const char *p   = P.q.data;
-            if (on) {
-                p += (int64_t) (row / P.G) * P.q.nb1 + (int64_t) (hk * P.G + row % P.G) * P.q.nb2 +
-                     (int64_t) at.b * P.q.nb3;
-            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 // word ks of this thread's K pieces: dims 64 * (ks / 4) + 16 * c + 4 * (ks % 4) ..
                 const int d = 64 * (ks >> 2) + 16 * c + 4 * (ks & 3);
+                load_q4(p, P.q.type, d, x[ks]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    x[ks][e] = on ? load1(p, P.q.type, d + e) : 0.0f;
-                    top      = fmaxf(top, fabsf(x[ks][e]));
+                    top = fmaxf(top, fabsf(x[ks][e]));
                 }
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -307,13 +360,20 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
             const float u = P.scale_log2 * __uint_as_float((uint32_t) (127 - k) << 23);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                split2(x[ks][0] * f, x[ks][1] * f, qh[nt][ks][0], ql[nt][ks][0]);
-                split2(x[ks][2] * f, x[ks][3] * f, qh[nt][ks][1], ql[nt][ks][1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t hi, lo;
+                    split2(x[ks][2 * e] * f, x[ks][2 * e + 1] * f, hi, lo);
+                    qh[nt][ks][e] = MODE == kPacked && g >= 4 ? lo : hi;
+                    if constexpr (MODE == kSplit) {
+                        ql[nt][ks][e] = lo;
+                    }
+                }
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 mul[nt][e]    = __shfl_sync(0xffffffffu, u, (2 * c + e) * 4);
-                const int rr  = rb * R + nt * 8 + 2 * c + e;
+                const int rr  = rb * R + nt * 8 + (MODE == kPacked ? (2 * c + e) & 3 : 2 * c + e);
                 lim[nt][e]    = rr < P.rows ? at.len - (P.n_q - 1 - rr / P.G) : 0;
                 m[nt][e]      = -INFINITY;
                 l[nt][e]      = 0.0f;
@@ -332,7 +392,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
     for (int i = 0; i < kStages - 1; ++i) {
         if (i < n_my) {
             issue(i);
-            advance(ahead);
+            if (advance(ahead)) {
+                prefetch_rows(ahead);
+            }
         }
         cp_commit();
     }
@@ -342,7 +404,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
     for (int i = 0; i < n_my; ++i) {
         if (i + kStages - 1 < n_my) {
             issue((i + kStages - 1) % kStages);
-            advance(ahead);
+            if (advance(ahead)) {
+                prefetch_rows(ahead);
+            }
         }
         cp_commit();
         cp_wait<kStages - 1>();
@@ -353,12 +417,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
             const float    kd = lds_f32(d + 2 * kChunk * HD + lane * 4);
             const float    vd = lds_f32(d + 2 * kChunk * HD + 128 + lane * 4);
             // ---- S^T = K Q^T
-            float s[NT][4];
+            // (two sums per product, of the even and the odd k-steps: half as long a chain)
+            float s[NT][4], s2[NT][MODE == kSplit ? 3 : 1][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[nt][e] = 0.0f;
+#pragma unroll
+                    for (int y = 0; y < (MODE == kSplit ? 3 : 1); ++y) {
+                        s2[nt][y][e] = 0.0f;
+                    }
                 }
             }
 #pragma unroll
@@ -374,8 +443,23 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
                     const int      ks   = 4 * e4 + e;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_16816<false>(s[nt], a, qh[nt][ks][0], qh[nt][ks][1]);
-                        mma_16816<false>(s[nt], a, ql[nt][ks][0], ql[nt][ks][1]);
+                        mma_16816<false>(e & 1 ? s2[nt][0] : s[nt], a, qh[nt][ks][0], qh[nt][ks][1]);
+                        if constexpr (MODE == kSplit) {
+                            mma_16816<false>(s2[nt][1 + (e & 1)], a, ql[nt][ks][0], ql[nt][ks][1]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[nt][e] += s2[nt][0][e];
+                    if constexpr (MODE == kSplit) {
+                        s[nt][e] += s2[nt][1][e] + s2[nt][2][e];
+                    }
+                    if constexpr (MODE == kPacked) {  // columns r and r + 4
+                        s[nt][e] += __shfl_xor_sync(0xffffffffu, s[nt][e], 2);
                     }
                 }
             }
@@ -426,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
                 }
             }
             // ---- P, its operand halves
-            uint32_t ph[NT][2], pl[NT][2];
+            uint32_t ph[NT][2], pl[MODE == kSplit ? NT : 1][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float p[4];
@@ -440,8 +524,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
                 for (int e = 0; e < 2; ++e) {
                     uint32_t hi, lo;
                     split2(p[2 * e], p[2 * e + 1], hi, lo);
-                    ph[nt][e] = movmatrix_trans(hi);
-                    pl[nt][e] = movmatrix_trans(lo);
+                    ph[nt][e] = movmatrix_trans(MODE == kPacked && c >= 2 ? lo : hi);
+                    if constexpr (MODE == kSplit) {
+                        pl[nt][e] = movmatrix_trans(lo);
+                    }
                 }
             }
             // ---- O^T += vd * V^T P^T.  m-tile t: dims g * HD / 8 + 2t (row g) and + 2t + 1 (row g + 8)
@@ -467,7 +553,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
                 for (int nt = 0; nt < NT; ++nt) {
                     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     mma_16816<false>(o, a, ph[nt][0], ph[nt][1]);
-                    mma_16816<false>(o, a, pl[nt][0], pl[nt][1]);
+                    if constexpr (MODE == kSplit) {
+                        mma_16816<false>(o, a, pl[nt][0], pl[nt][1]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         acc_o[nt][t][e] = fmaf(o[e], vd, acc_o[nt][t][e]);
@@ -520,7 +608,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     const float  f = exp2f(mw[w] - Mu);
-                    const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * R + row) * kOut + 4 * d4);
+                    float4       v = *reinterpret_cast<const float4 *>(s_o + (w * R + row) * kOut + 4 * d4);
+                    if constexpr (MODE == kPacked) {
+                        const float4 u = *reinterpret_cast<const float4 *>(s_o + (w * R + row + 4) * kOut + 4 * d4);
+                        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+                    }
                     L += s_ml[(w * R + row) * 2 + 1] * f;
                     o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
                 }
@@ -544,18 +636,42 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD, NT))
 // head's rows, whose M and L come from the same partials.  Every sum has a
 // fixed order, so results do not depend on scheduling.
 constexpr int kSumThreads = 128;
-constexpr int kSumKeys    = 1024;
+constexpr int kSumKeys    = 512;
+
+// Over the slots c0 .. c1 of a row (base: its first m, l at + R): the maximum
+// and the sum of l * 2^(m - maximum).  The whole warp, lanes side by side.
+__device__ __forceinline__ void merge_row(const float *base, int64_t slot_f, int R, int c0, int c1, float &M, float &L) {
+    const int lane = threadIdx.x & 31;
+    M              = -INFINITY;
+    L              = 0.0f;
+    for (int k = c0 + lane; k <= c1; k += 32) {
+        const float m = __ldcg(base + k * slot_f), l = __ldcg(base + k * slot_f + R);
+        const float mn = fmaxf(M, m), mu = mn == -INFINITY ? 0.0f : mn;
+        L = L * exp2f(M - mu) + l * exp2f(m - mu);
+        M = mn;
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+        const float m = __shfl_xor_sync(0xffffffffu, M, off), l = __shfl_xor_sync(0xffffffffu, L, off);
+        const float mn = fmaxf(M, m), mu = mn == -INFINITY ? 0.0f : mn;
+        L = L * exp2f(M - mu) + l * exp2f(m - mu);
+        M = mn;
+    }
+    L = __shfl_sync(0xffffffffu, L, 0);  // (the lanes' sums differ in the order of their terms)
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_constant__ Kv8AttnParams P, int R,
                                                                    int n_out, int key_chunks) {
-    __shared__ int    s_base[kKv8MaxSets + 4];
+    extern __shared__ __align__(16) int s_tab[];  // tile table and lengths
     __shared__ float  s_lse[ACEFA_KV8_MAX_ROWS];
     __shared__ float4 s_o[4][HD / 4];
-    const int slot_f = R * (HD + 2);
-    const int HU     = P.c.Hkv * P.n_rb;
-    pdl_wait_primary();
-    tile_table(s_base, P.len, P.c.B, P.c.n_max);
+    int          *s_base = s_tab, *s_len = s_tab + P.c.B + 1;
+    const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t slot_f = (int64_t) R * (HD + 2);
+    const int     HU     = P.c.Hkv * P.n_rb;
+    // (the lengths are older than the split kernel, which let this one start only after its own wait)
+    tile_table(s_base, s_len, P.len, P.c.B, P.c.n_max);
     const int T = s_base[P.c.B] * HU, C = min(P.n_cta, T);
     // the CTAs of the split kernel that met a unit: slots (c + unit), c0 <= c <= c1
     auto range_of = [&](int b, int ub, int &c0, int &c1) {
@@ -571,36 +687,28 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
         int       c0, c1;
         range_of(b, ub, c0, c1);
         const float *base = P.part + (int64_t) (b * HU + ub) * slot_f;
-        float        M    = -INFINITY;
-        for (int k = c0; k <= c1; ++k) {
-            M = fmaxf(M, __ldcg(base + (int64_t) k * slot_f + R * HD + r));
-        }
+        pdl_wait_primary();
+        float M, L;
+        merge_row(base + R * HD + r, slot_f, R, c0, c1, M, L);
         const float Mu = M == -INFINITY ? 0.0f : M;
         const int   w = threadIdx.x / (HD / 4), d4 = threadIdx.x % (HD / 4);
         constexpr int W = kSumThreads / (HD / 4);  // slots summed side by side
         float4      o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float       L = 0.0f;
 #pragma unroll 4
         for (int k = c0 + w; k <= c1; k += W) {
             const float *sl = base + (int64_t) k * slot_f;
             const float  f  = exp2f(__ldcg(sl + R * HD + r) - Mu);
             const float4 v  = __ldcg(reinterpret_cast<const float4 *>(sl + r * HD) + d4);
-            L = fmaf(__ldcg(sl + R * HD + R + r), f, L);
             o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
         }
-        __shared__ float s_l[8];
         for (int half = W / 2; half; half >>= 1) {
             if (w >= half && w < 2 * half) {
                 s_o[w - half][d4] = o;
-                if (d4 == 0) {
-                    s_l[w - half] = L;
-                }
             }
             __syncthreads();
             if (w < half) {
                 const float4 v = s_o[w][d4];
                 o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-                L += s_l[w];
             }
             __syncthreads();
         }
@@ -618,50 +726,52 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
     const int x = (int) blockIdx.x - n_out;
     const int bh = x / key_chunks, j0 = x % key_chunks * kSumKeys;
     const int hk = bh % P.c.Hkv, b = bh / P.c.Hkv;
-    const int len = clamp_len(__ldg(P.len + b), P.c.n_max);
+    const int len = s_len[b];
     if (j0 >= len) {
         return;
     }
-    for (int row = threadIdx.x; row < P.rows; row += kSumThreads) {
-        const int ub = hk * P.n_rb + row / R, r = row % R;
+    pdl_wait_primary();
+    for (int row = warp; row < P.rows; row += kSumThreads / 32) {
+        const int ub = hk * P.n_rb + row / R;
         int       c0, c1;
         range_of(b, ub, c0, c1);
-        const float *base = P.part + (int64_t) (b * HU + ub) * slot_f + R * HD + r;
-        float        M    = -INFINITY;
-        for (int k = c0; k <= c1; ++k) {
-            M = fmaxf(M, __ldcg(base + (int64_t) k * slot_f));
+        float M, L;
+        merge_row(P.part + (int64_t) (b * HU + ub) * slot_f + R * HD + row % R, slot_f, R, c0, c1, M, L);
+        if (lane == 0) {  // an empty row weighs nothing
+            s_lse[row] = L == 0.0f ? INFINITY : (M == -INFINITY ? 0.0f : M) + log2f(L);
         }
-        const float Mu = M == -INFINITY ? 0.0f : M;
-        float       L  = 0.0f;
-        for (int k = c0; k <= c1; ++k) {
-            L = fmaf(__ldcg(base + (int64_t) k * slot_f + R), exp2f(__ldcg(base + (int64_t) k * slot_f) - Mu), L);
-        }
-        s_lse[row] = L == 0.0f ? INFINITY : Mu + log2f(L);  // an empty row weighs nothing
     }
     __syncthreads();
     float *wp = reinterpret_cast<float *>(P.weight + (int64_t) hk * P.w_nb2 + (int64_t) b * P.w_nb3);
+    const int st = P.score_stride;  // even
     for (int j = j0 + threadIdx.x; j < min(len, j0 + kSumKeys); j += kSumThreads) {
         float sum = 0.0f;
         for (int rb = 0; rb < P.n_rb; ++rb) {
-            const float *sp =
-                P.scores + ((int64_t) (b * HU + hk * P.n_rb + rb) * P.c.n_max + j) * P.score_stride;
-            const int n_row = min(R, P.rows - rb * R);
-            for (int r = 0; r < n_row; ++r) {
-                sum += exp2f(__ldcg(sp + r) - s_lse[rb * R + r]);
+            const float2 *sp    = reinterpret_cast<const float2 *>(
+                P.scores + ((int64_t) (b * HU + hk * P.n_rb + rb) * P.c.n_max + j) * st);
+            const int     n_row = min(R, P.rows - rb * R);
+#pragma unroll 4
+            for (int r = 0; r < n_row; r += 2) {
+                const float2 s = __ldcg(sp + (r >> 1));
+                sum += exp2f(s.x - s_lse[rb * R + r]);
+                if (r + 1 < n_row) {
+                    sum += exp2f(s.y - s_lse[rb * R + r + 1]);
+                }
             }
         }
         wp[j] += sum;
     }
 }
 
-template <int HD, int NT>
+template <int HD, int NT, int MODE>
 cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
-    constexpr int          smem = attn_smem_bytes<HD, NT>();
+    const int              smem = attn_smem_bytes<HD, NT>(p.c.B);
     static thread_local int configured = -1;
     int                     dev        = 0;
     cudaGetDevice(&dev);
     if (configured != dev) {
-        cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<HD, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             attn_smem_bytes<HD, NT>(kKv8MaxSets));
         if (e != cudaSuccess) {
             return e;
         }
@@ -677,7 +787,7 @@ cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
     cfg.stream             = s;
     cfg.attrs              = attr;
     cfg.numAttrs           = 1;
-    cudaError_t e          = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT>, p);
+    cudaError_t e          = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT, MODE>, p);
     if (e != cudaSuccess) {
         return e;
     }
@@ -685,18 +795,25 @@ cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
     const int key_chunks = (p.c.n_max + kSumKeys - 1) / kSumKeys;
     cfg.gridDim          = dim3((unsigned) (n_out + (p.weight ? p.c.B * p.c.Hkv * key_chunks : 0)));
     cfg.blockDim         = dim3(kSumThreads);
-    cfg.dynamicSmemBytes = 0;
+    cfg.dynamicSmemBytes = sizeof(int) * (2 * (size_t) p.c.B + 1);
     return cudaLaunchKernelEx(&cfg, kv8_attn_sum_kernel<HD>, p, 8 * NT, n_out, key_chunks);
 }
 
 }  // namespace
 
-int kv8_attn_ctas_per_sm(int D, int unit_rows) { return ctas_per_sm(D, unit_rows / 8); }
+int kv8_attn_ctas_per_sm(int unit_rows) { return ctas_per_sm(unit_rows / 8); }
 
 cudaError_t launch_kv8_attn(const Kv8AttnParams &p, cudaStream_t s) {
-    const bool wide = kv8_unit_rows(p.rows) == 16;
-    return p.c.D == 128 ? (wide ? launch<128, 2>(p, s) : launch<128, 1>(p, s))
-                        : (wide ? launch<64, 2>(p, s) : launch<64, 1>(p, s));
+    const bool one = p.q.type != ACEFA_TYPE_F32 && p.dst.type != ACEFA_TYPE_F32;
+    auto       pick = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        if (kv8_unit_rows(p.rows) == 16) {
+            return one ? launch<HD, 2, kOne>(p, s) : launch<HD, 2, kSplit>(p, s);
+        }
+        return one ? launch<HD, 1, kOne>(p, s)
+                   : (p.rows <= 4 ? launch<HD, 1, kPacked>(p, s) : launch<HD, 1, kSplit>(p, s));
+    };
+    return p.c.D == 128 ? pick(std::integral_constant<int, 128>{}) : pick(std::integral_constant<int, 64>{});
 }
 
 }  // namespace acefa

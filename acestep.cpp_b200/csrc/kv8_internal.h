@@ -80,7 +80,7 @@ cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s);
 // Rows of a unit of the attention kernel (8 or 16) and the CTAs that it may
 // keep resident on one SM; functions of the operands alone.
 inline int kv8_unit_rows(int rows) { return rows <= 8 ? 8 : 16; }
-int        kv8_attn_ctas_per_sm(int D, int unit_rows);
+int        kv8_attn_ctas_per_sm(int unit_rows);
 inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows * (D + 2); }
 
 // ------------------------------------------------------------------ device helpers
