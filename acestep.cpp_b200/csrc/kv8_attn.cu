@@ -39,6 +39,9 @@ constexpr int   kWarps   = 4;
 constexpr int   kThreads = 32 * kWarps;
 constexpr int   kChunk   = 16;  // keys of one warp and tile
 constexpr float kSlack   = 8.0f;
+// "No maximum yet": below every score, finite so that differences stay numbers
+// (2^(anything - it) only meets weights and sums that are 0).
+constexpr float kNoMax = -1.7e38f;
 static_assert(kWarps * kChunk == kKv8Block, "a tile is one block of the cache");
 
 // ring stages of a warp: bytes of one chunk = 2 * 16 * D plus one 4-byte
@@ -189,11 +192,16 @@ __device__ __forceinline__ int cta_of(int T, int C, int x) { return (int) ((((in
 
 // A position in the sequence of tiles.
 struct Walk {
-    int     b, ub, t, nt, len;  // set, unit of the set, tile of the unit, its tiles, the set's length
-    int64_t off_k, off_v;       // byte offsets of (head, set) in k and v
-    const float *ks, *vs;       // its scales
+    int b, ub, t, nt, len;  // set, unit of the set, tile of the unit, its tiles, the set's length
 };
 
+// D = A B (a product that starts a sum)
+__device__ __forceinline__ void mma_start(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 template <int HD, int NT, int MODE>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
     kv8_attn_kernel(const __grid_constant__ Kv8AttnParams P) {
@@ -221,19 +229,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
     }
     const int x0 = run_start(T, C, blockIdx.x), n_my = run_start(T, C, blockIdx.x + 1) - x0;
 
-    auto enter_unit = [&](Walk &w) {
-        const int hk = w.ub / P.n_rb;
-        w.off_k      = (int64_t) hk * P.c.k.nb2 + (int64_t) w.b * P.c.k.nb3;
-        w.off_v      = (int64_t) hk * P.c.v.nb2 + (int64_t) w.b * P.c.v.nb3;
-        w.ks         = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.k.scale) +
-                                               hk * P.c.k.s_nb2 + w.b * P.c.k.s_nb3);
-        w.vs         = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.v.scale) +
-                                               hk * P.c.v.s_nb2 + w.b * P.c.v.s_nb3);
-    };
-    auto enter_set = [&](Walk &w) {
-        w.nt  = s_base[w.b + 1] - s_base[w.b];
-        w.len = s_len[w.b];
-    };
     auto advance = [&](Walk &w) {  // true: a new unit
         if (++w.t < w.nt) {
             return false;
@@ -247,28 +242,28 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
             if (w.b == P.c.B) {
                 return true;
             }
-            enter_set(w);
+            w.nt  = s_base[w.b + 1] - s_base[w.b];
+            w.len = s_len[w.b];
         }
-        enter_unit(w);
         return true;
     };
+    auto kv_head = [&](const Walk &w) { return P.n_rb == 1 ? w.ub : w.ub / P.n_rb; };
     Walk at;
     {
-        int lo = 0, hi = P.c.B;  // the set whose tiles hold x0: base[lo] * HU <= x0 < base[lo + 1] * HU
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (s_base[mid] * HU <= x0) {
-                lo = mid;
-            } else {
-                hi = mid;
-            }
+        // the set whose tiles hold x0: base[b] * HU <= x0 < base[b + 1] * HU, by 32nds
+        int lo = 0, n = P.c.B;
+        while (n > 1) {
+            const int step = (n + 31) >> 5, i = lo + lane * step;
+            const int below = __popc(__ballot_sync(0xffffffffu, lane * step < n && s_base[i] * HU <= x0));
+            n  = min(step, n - (below - 1) * step);
+            lo += (below - 1) * step;
         }
-        at.b = lo;
-        enter_set(at);
+        at.b          = lo;
+        at.nt         = s_base[lo + 1] - s_base[lo];
+        at.len        = s_len[lo];
         const int off = x0 - s_base[lo] * HU;
-        at.ub         = off / at.nt;
-        at.t          = off % at.nt;
-        enter_unit(at);
+        at.ub         = (int) ((unsigned) off / (unsigned) at.nt);
+        at.t          = off - at.ub * at.nt;
     }
     Walk ahead = at;
 
@@ -276,40 +271,66 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
     // Copies this thread's part of a chunk.  K: rows g and g + 8, 16-B pieces c
     // (and 4 + c) of each.  V: HD / 8 dims from g * HD / 8 of rows 2c, 2c + 1, 2c + 8,
     // 2c + 9.  Rows past the length repeat the last one (they get no weight).
+    // Pointers to rows g and 2c of the chunk and to the block's scales move along.
+    const int64_t k_nb1 = P.c.k.nb1, v_nb1 = P.c.v.nb1;
+    const int8_t *kp, *vp;
+    const float  *ksp, *vsp;
+    auto aim = [&]() {
+        const int hk = kv_head(ahead);
+        const int j  = ahead.t * kKv8Block + warp * kChunk;
+        kp = P.c.k.q + (int64_t) hk * P.c.k.nb2 + (int64_t) ahead.b * P.c.k.nb3 + (j + g) * k_nb1 + 16 * c;
+        vp = P.c.v.q + (int64_t) hk * P.c.v.nb2 + (int64_t) ahead.b * P.c.v.nb3 + (j + 2 * c) * v_nb1 + (HD / 8) * g;
+        ksp = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.k.scale) + hk * P.c.k.s_nb2 +
+                                              ahead.b * P.c.k.s_nb3) +
+              ahead.t;
+        vsp = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.v.scale) + hk * P.c.v.s_nb2 +
+                                              ahead.b * P.c.v.s_nb3) +
+              ahead.t;
+    };
+    aim();
     auto issue = [&](int st) {
-        const int j0 = ahead.t * kKv8Block + warp * kChunk;
-        if (j0 < ahead.len) {
-            const uint32_t d    = ring + (uint32_t) (st * kSt) + (uint32_t) lane * 16;
-            const int      last = ahead.len - 1;
+        const int      room = ahead.len - ahead.t * kKv8Block - warp * kChunk;  // rows of the chunk that exist
+        const uint32_t d    = ring + (uint32_t) (st * kSt) + (uint32_t) lane * 16;
+        const uint32_t dv   = HD == 128 ? d + 2048u : ring + (uint32_t) (st * kSt + 1024 + lane * 8);
+        if (room > 0) {
+            int kr[2] = {0, 8}, vr[4] = {0, 1, 8, 9};  // rows from g and from 2c
+            if (room < kChunk) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    kr[r] = min(g + kr[r], room - 1) - g;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    vr[r] = min(2 * c + vr[r], room - 1) - 2 * c;
+                }
+            }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int8_t *p = P.c.k.q + ahead.off_k + (int64_t) min(j0 + g + 8 * r, last) * P.c.k.nb1 + 16 * c;
 #pragma unroll
                 for (int e = 0; e < HD / 64; ++e) {
-                    cp16(d + (uint32_t) ((r * (HD / 64) + e) * 512), p + 64 * e);
+                    cp16(d + (uint32_t) ((r * (HD / 64) + e) * 512), kp + kr[r] * k_nb1 + 64 * e);
                 }
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int     j = j0 + 2 * c + (r & 1) + 8 * (r >> 1);
-                const int8_t *p = P.c.v.q + ahead.off_v + (int64_t) min(j, last) * P.c.v.nb1 + (HD / 8) * g;
                 if constexpr (HD == 128) {
-                    cp16(d + (uint32_t) (2048 + r * 512), p);
+                    cp16(dv + (uint32_t) (r * 512), vp + vr[r] * v_nb1);
                 } else {
-                    cp8(ring + (uint32_t) (st * kSt + 1024 + r * 256 + lane * 8), p);
+                    cp8(dv + (uint32_t) (r * 256), vp + vr[r] * v_nb1);
                 }
             }
             const uint32_t sc = ring + (uint32_t) (st * kSt + 2 * kChunk * HD + lane * 4);
-            cp4(sc, ahead.ks + ahead.t);
-            cp4(sc + 128, ahead.vs + ahead.t);
+            cp4(sc, ksp);
+            cp4(sc + 128, vsp);
         }
     };
 
     // This thread's row of Q of a unit (kPacked: rows 4 .. 7 are the low halves of 0 .. 3), or nullptr
     auto q_row = [&](const Walk &w, int nt, int &row) -> const char * {
-        const int hk = w.ub / P.n_rb;
-        row          = w.ub % P.n_rb * R + nt * 8 + (MODE == kPacked ? g & 3 : g);
-        return row < P.rows ? P.q.data + (int64_t) (row / P.G) * P.q.nb1 + (int64_t) (hk * P.G + row % P.G) * P.q.nb2 +
+        const int hk = kv_head(w);
+        row          = (w.ub - hk * P.n_rb) * R + nt * 8 + (MODE == kPacked ? g & 3 : g);
+        const int iq = P.n_q == 1 ? 0 : row / P.G;
+        return row < P.rows ? P.q.data + iq * P.q.nb1 + (int64_t) (hk * P.G + row - iq * P.G) * P.q.nb2 +
                                   (int64_t) w.b * P.q.nb3
                             : nullptr;
     };
@@ -332,22 +353,34 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
     int      lim[NT][2];                    // keys those rows see
     float    acc_o[NT][KS][4];
     float    m[NT][2], l[NT][2];
-    auto load_rows = [&]() {
-        const int rb = at.ub % P.n_rb;
+    float   *sp = nullptr;  // this thread's scores of the chunk, where weights are wanted
+    float    x[NT][KS][4];
+    auto read_rows = [&]() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             int         row;
             const char *p = q_row(at, nt, row);
-            float       x[KS][4];
-            float       top = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 // word ks of this thread's K pieces: dims 64 * (ks / 4) + 16 * c + 4 * (ks % 4) ..
-                const int d = 64 * (ks >> 2) + 16 * c + 4 * (ks & 3);
-                load_q4(p, P.q.type, d, x[ks]);
+                load_q4(p, P.q.type, 64 * (ks >> 2) + 16 * c + 4 * (ks & 3), x[nt][ks]);
+            }
+        }
+    };
+    auto start_rows = [&]() {
+        const int rb = at.ub - kv_head(at) * P.n_rb;
+        if (P.scores) {
+            sp = P.scores + ((int64_t) (at.b * HU + at.ub) * P.c.n_max + at.t * kKv8Block + warp * kChunk + g) * P.score_stride +
+                 2 * c;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float top = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    top = fmaxf(top, fabsf(x[ks][e]));
+                    top = fmaxf(top, fabsf(x[nt][ks][e]));
                 }
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -363,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint32_t hi, lo;
-                    split2(x[ks][2 * e] * f, x[ks][2 * e + 1] * f, hi, lo);
+                    split2(x[nt][ks][2 * e] * f, x[nt][ks][2 * e + 1] * f, hi, lo);
                     qh[nt][ks][e] = MODE == kPacked && g >= 4 ? lo : hi;
                     if constexpr (MODE == kSplit) {
                         ql[nt][ks][e] = lo;
@@ -374,8 +407,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
             for (int e = 0; e < 2; ++e) {
                 mul[nt][e]    = __shfl_sync(0xffffffffu, u, (2 * c + e) * 4);
                 const int rr  = rb * R + nt * 8 + (MODE == kPacked ? (2 * c + e) & 3 : 2 * c + e);
-                lim[nt][e]    = rr < P.rows ? at.len - (P.n_q - 1 - rr / P.G) : 0;
-                m[nt][e]      = -INFINITY;
+                const int iq  = P.n_q == 1 ? 0 : rr / P.G;
+                lim[nt][e]    = rr < P.rows ? at.len - (P.n_q - 1 - iq) : 0;
+                m[nt][e]      = kNoMax;
                 l[nt][e]      = 0.0f;
             }
 #pragma unroll
@@ -388,48 +422,47 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
         }
     };
 
+    auto next_ahead = [&]() {
+        if (advance(ahead)) {
+            if (ahead.b < P.c.B) {
+                aim();
+                prefetch_rows(ahead);
+            }
+        } else {
+            kp += kKv8Block * k_nb1;
+            vp += kKv8Block * v_nb1;
+            ++ksp, ++vsp;
+        }
+    };
+    read_rows();  // before the stream fills the queues
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
         if (i < n_my) {
             issue(i);
-            if (advance(ahead)) {
-                prefetch_rows(ahead);
-            }
+            next_ahead();
         }
         cp_commit();
     }
-    load_rows();
+    start_rows();
+    int stage = 0, free_stage = kStages - 1;
 
 #pragma unroll 1
     for (int i = 0; i < n_my; ++i) {
         if (i + kStages - 1 < n_my) {
-            issue((i + kStages - 1) % kStages);
-            if (advance(ahead)) {
-                prefetch_rows(ahead);
-            }
+            issue(free_stage);
+            next_ahead();
         }
         cp_commit();
         cp_wait<kStages - 1>();
         const int j0 = at.t * kKv8Block + warp * kChunk;
         if (j0 < at.len) {  // uniform over the warp
-            const uint32_t d  = ring + (uint32_t) ((i % kStages) * kSt);
+            const uint32_t d  = ring + (uint32_t) (stage * kSt);
             const uint32_t dl = d + (uint32_t) lane * 16;
             const float    kd = lds_f32(d + 2 * kChunk * HD + lane * 4);
             const float    vd = lds_f32(d + 2 * kChunk * HD + 128 + lane * 4);
             // ---- S^T = K Q^T
             // (two sums per product, of the even and the odd k-steps: half as long a chain)
             float s[NT][4], s2[NT][MODE == kSplit ? 3 : 1][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[nt][e] = 0.0f;
-#pragma unroll
-                    for (int y = 0; y < (MODE == kSplit ? 3 : 1); ++y) {
-                        s2[nt][y][e] = 0.0f;
-                    }
-                }
-            }
 #pragma unroll
             for (int e4 = 0; e4 < HD / 64; ++e4) {
                 const uint4    wa    = lds_v4(dl + (uint32_t) (e4 * 512));
@@ -443,9 +476,18 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                     const int      ks   = 4 * e4 + e;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_16816<false>(e & 1 ? s2[nt][0] : s[nt], a, qh[nt][ks][0], qh[nt][ks][1]);
+                        float(&sum)[4] = e & 1 ? s2[nt][0] : s[nt];
+                        if (ks < 2) {
+                            mma_start(sum, a, qh[nt][ks][0], qh[nt][ks][1]);
+                        } else {
+                            mma_16816<false>(sum, a, qh[nt][ks][0], qh[nt][ks][1]);
+                        }
                         if constexpr (MODE == kSplit) {
-                            mma_16816<false>(s2[nt][1 + (e & 1)], a, ql[nt][ks][0], ql[nt][ks][1]);
+                            if (ks < 2) {
+                                mma_start(s2[nt][1 + (e & 1)], a, ql[nt][ks][0], ql[nt][ks][1]);
+                            } else {
+                                mma_16816<false>(s2[nt][1 + (e & 1)], a, ql[nt][ks][0], ql[nt][ks][1]);
+                            }
                         }
                     }
                 }
@@ -468,21 +510,35 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = j0 + g + 8 * (e >> 1);
-                    const float v = s[nt][e] * (mul[nt][e & 1] * kd);
-                    s[nt][e]      = j < lim[nt][e & 1] ? v : -INFINITY;
-                    grow |= s[nt][e] > m[nt][e & 1] + kSlack;
+                for (int e = 0; e < 2; ++e) {
+                    const float u = mul[nt][e] * kd;
+                    s[nt][e] *= u;
+                    s[nt][2 + e] *= u;
+                }
+            }
+            if (j0 + kChunk > at.len - (P.n_q - 1)) {  // keys that some row does not see
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[nt][e] = j0 + g + 8 * (e >> 1) < lim[nt][e & 1] ? s[nt][e] : -INFINITY;
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    grow |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + kSlack;
                 }
             }
             if (P.scores) {
-                float *sp = P.scores + ((int64_t) (at.b * HU + at.ub) * P.c.n_max + j0) * P.score_stride;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         if (nt * 8 + 2 * c < P.score_stride && j0 + g + 8 * e < at.len) {
-                            *reinterpret_cast<float2 *>(sp + (int64_t) (g + 8 * e) * P.score_stride + nt * 8 + 2 * c) =
+                            *reinterpret_cast<float2 *>(sp + 8 * e * P.score_stride + nt * 8) =
                                 make_float2(s[nt][2 * e], s[nt][2 * e + 1]);
                         }
                     }
@@ -498,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                         top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                         const float mn = fmaxf(m[nt][e], top);
-                        const float f  = mn == -INFINITY ? 1.0f : exp2f(m[nt][e] - mn);
+                        const float f  = fast_exp2(m[nt][e] - mn);
                         m[nt][e]       = mn;
                         l[nt][e] *= f;
 #pragma unroll
@@ -516,8 +572,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                 float p[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float mu = m[nt][e & 1];
-                    p[e]           = exp2f(s[nt][e] - (mu == -INFINITY ? 0.0f : mu));
+                    p[e] = fast_exp2(s[nt][e] - m[nt][e & 1]);
                     l[nt][e & 1] += p[e];
                 }
 #pragma unroll
@@ -551,8 +606,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                                        i8x2_f16(z1, 0x4342u)};
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_16816<false>(o, a, ph[nt][0], ph[nt][1]);
+                    float o[4];
+                    mma_start(o, a, ph[nt][0], ph[nt][1]);
                     if constexpr (MODE == kSplit) {
                         mma_16816<false>(o, a, pl[nt][0], pl[nt][1]);
                     }
@@ -565,8 +620,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
         }
         // ---- end of the unit (or of this CTA's run): merge the warps' results
         const int  unit = at.b * HU + at.ub;
-        const int  rb   = at.ub % P.n_rb;
+        const int  rb   = at.ub - kv_head(at) * P.n_rb;
         const bool next = advance(at);
+        stage           = stage == kStages - 1 ? 0 : stage + 1;
+        free_stage      = free_stage == kStages - 1 ? 0 : free_stage + 1;
+        if (P.scores) {
+            sp += kKv8Block * P.score_stride;
+        }
         if (next || i + 1 == n_my) {
             __syncthreads();  // the previous merge has been read
 #pragma unroll
@@ -596,18 +656,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
             float    *slot  = P.part + (int64_t) (blockIdx.x + unit) * (R * (HD + 2));
             for (int x = threadIdx.x; x < n_row * (HD / 4); x += kThreads) {
                 const int row = x / (HD / 4), d4 = x % (HD / 4);
-                float     mw[kWarps], M = -INFINITY;
+                float     mw[kWarps], M = kNoMax;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     mw[w] = s_ml[(w * R + row) * 2];
                     M     = fmaxf(M, mw[w]);
                 }
-                const float Mu = M == -INFINITY ? 0.0f : M;
                 float       L  = 0.0f;
                 float4      o  = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    const float  f = exp2f(mw[w] - Mu);
+                    const float  f = exp2f(mw[w] - M);
                     float4       v = *reinterpret_cast<const float4 *>(s_o + (w * R + row) * kOut + 4 * d4);
                     if constexpr (MODE == kPacked) {
                         const float4 u = *reinterpret_cast<const float4 *>(s_o + (w * R + row + 4) * kOut + 4 * d4);
@@ -623,7 +682,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                 }
             }
             if (i + 1 < n_my) {
-                load_rows();
+                read_rows();
+                start_rows();
             }
         }
     }
