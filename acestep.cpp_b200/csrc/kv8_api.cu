@@ -182,7 +182,7 @@ int plan_attn(const acefa_tensor *q, const acefa_kv8_cache *cache, const acefa_t
     p.n_q  = (int) n_q;
     p.G    = (int) (Hq / p.c.Hkv);
     p.rows = p.n_q * p.G;
-    const int R = kv8_unit_rows(p.rows);
+    const int R = kv8_unit_rows(p.rows, q->type);
     p.n_rb      = (p.rows + R - 1) / R;
     const int64_t units = (int64_t) p.c.B * p.c.Hkv * p.n_rb;
     const int64_t tiles = units * ((p.c.n_max + kKv8Block - 1) / kKv8Block);
@@ -194,7 +194,9 @@ int plan_attn(const acefa_tensor *q, const acefa_kv8_cache *cache, const acefa_t
     if ((rc = device_ctx(&ctx)) != ACEFA_OK) {
         return rc;
     }
-    p.n_cta           = (int) std::min<int64_t>(tiles, (int64_t) ctx.sm_count * kv8_attn_ctas_per_sm(R));
+    p.n_cta           = (int) std::min<int64_t>(tiles, (int64_t) ctx.sm_count * kv8_attn_ctas_per_sm());
+    p.dev_err         = ctx.dev_err;
+    p.wait_limit_ns   = ctx.wait_limit_ns;
     p.score_stride    = std::min(R, (p.rows + 1) & ~1);
     plan->part_bytes  = ((size_t) (p.n_cta + units) * kv8_slot_floats(p.c.D, R) * sizeof(float) + 255) / 256 * 256;
     plan->ws_bytes    = plan->part_bytes +
@@ -344,11 +346,11 @@ ACEFA_API int acefa_kv8_attn(const acefa_tensor *q, const acefa_kv8_cache *cache
     p.scale_log2 = scale * kLog2e;
     p.part       = static_cast<float *>(workspace);
     p.scores     = weight ? reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.part_bytes) : nullptr;
-    if (launch_kv8_attn(p, static_cast<cudaStream_t>(stream)) != cudaSuccess) {
-        return ACEFA_ERR_CUDA;
+    const int launched = launch_kv8_attn(p, static_cast<cudaStream_t>(stream));
+    if (launched == ACEFA_OK) {
+        note_launches(2, 4);
     }
-    note_launches(2, 4);
-    return ACEFA_OK;
+    return launched;
 }
 
 ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *weight, const int32_t *len,

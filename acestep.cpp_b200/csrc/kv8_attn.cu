@@ -17,12 +17,13 @@
 // Work.  The (set, KV head, row block) units' 64-key tiles, numbered one after
 // another over all sets' actual lengths, are cut into equal runs, one per CTA:
 // ragged batches balance as well as even ones, and the grid depends on shapes
-// only.  A CTA's four warps take 16 keys of every tile each and never wait for
-// one another inside a unit.  Each thread copies (cp.async) exactly the bytes
-// that its MMA fragments need into its own shared-memory slots, several chunks
-// ahead, so the stream needs no barrier; the dims and keys of a fragment are
-// assigned such that these bytes are 16-B pieces of rows (dims are summed over
-// in any order, and V's dims are only named at the end).
+// only.  A producer warp streams a CTA's tiles by TMA through a ring of stages,
+// their two scales beside them by cp.async; four consumer warps take 16 keys of
+// every tile each and meet only at the end of a unit.  The dims and keys of
+// a fragment are assigned such that a thread's bytes are 16-B pieces of rows
+// (dims are summed over in any order, and V's dims are only named at the end),
+// and the boxes' layouts (K in rows of 64 B, V swizzled) such that reading the
+// pieces meets no bank conflicts.
 // Products run transposed (keys or dims are the MMA's M, the rows its N = 8):
 // S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
 // operand layout by four movmatrix.  The running maximum moves only when a
@@ -35,8 +36,8 @@
 namespace acefa {
 namespace {
 
-constexpr int   kWarps   = 4;
-constexpr int   kThreads = 32 * kWarps;
+constexpr int   kWarps   = 4;  // consumers
+constexpr int   kThreads = 32 * (kWarps + 1);
 constexpr int   kChunk   = 16;  // keys of one warp and tile
 constexpr float kSlack   = 8.0f;
 // "No maximum yet": below every score, finite so that differences stay numbers
@@ -44,41 +45,36 @@ constexpr float kSlack   = 8.0f;
 constexpr float kNoMax = -1.7e38f;
 static_assert(kWarps * kChunk == kKv8Block, "a tile is one block of the cache");
 
-// ring stages of a warp: bytes of one chunk = 2 * 16 * D plus one 4-byte
-// scale of K and V per lane
+// A stage: 64 rows of K (boxes of 64 dims) and of V.
 template <int HD>
 constexpr int stage_bytes() {
-    return 2 * kChunk * HD + 256;
+    return 2 * kKv8Block * HD;
 }
-constexpr int kStages = 3;
+template <int HD, int NT>
+constexpr int stages() {
+    return HD == 128 ? (NT == 2 ? 4 : 5) : 8;
+}
 template <int HD, int NT>
 constexpr int merge_floats() {
     return kWarps * 8 * NT * (HD + 4) + kWarps * 8 * NT * 2;
 }
+// ring (1 KB aligned), merged rows, barriers and flag, scales of the stages, the sets' tile table and lengths
 template <int HD, int NT>
-constexpr int attn_smem_bytes(int B) {  // + the sets' tile table and lengths
-    return kWarps * kStages * stage_bytes<HD>() + 4 * merge_floats<HD, NT>() + 4 * (2 * B + 2);
+constexpr int attn_smem_bytes(int B) {
+    return 1024 + stages<HD, NT>() * stage_bytes<HD>() + 4 * merge_floats<HD, NT>() + (2 * stages<HD, NT>() + 1) * 8 +
+           stages<HD, NT>() * 8 + 4 * (2 * B + 2);
 }
-constexpr int ctas_per_sm(int NT) { return NT == 2 ? 2 : 3; }
+constexpr int kCtasPerSm = 2;
 
 // How operands of more than 11 bits enter the products.
 constexpr int kOne    = 0;  // one F16 number (16-bit Q and output)
 constexpr int kSplit  = 1;  // two, in products of their own
 constexpr int kPacked = 2;  // two, as columns r and r + 4 (up to four rows)
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
+// 4 bytes global -> shared; the barrier counts this thread as arrived when they have landed.
+__device__ __forceinline__ void cp4_arrive(uint32_t dst, const void *src, uint64_t *bar) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ uint4 lds_v4(uint32_t a) {
     uint4 v;
@@ -88,11 +84,6 @@ __device__ __forceinline__ uint4 lds_v4(uint32_t a) {
 __device__ __forceinline__ uint2 lds_v2(uint32_t a) {
     uint2 v;
     asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ float lds_f32(uint32_t a) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
     return v;
 }
 // 8x8 b16 matrix spread over the warp (row = lane / 4, two columns each), transposed
@@ -203,22 +194,39 @@ __device__ __forceinline__ void mma_start(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 template <int HD, int NT, int MODE>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
-    kv8_attn_kernel(const __grid_constant__ Kv8AttnParams P) {
-    constexpr int R    = 8 * NT;
-    constexpr int KS   = HD / 16;             // k-steps of S, m-tiles of O
-    constexpr int kSt  = stage_bytes<HD>();
-    constexpr int kOut = HD + 4;              // floats between merged rows
-    extern __shared__ __align__(16) uint8_t smem[];
-    float *s_o    = reinterpret_cast<float *>(smem + kWarps * kStages * kSt);  // [warp][R][kOut]
-    float *s_ml   = s_o + kWarps * R * kOut;                                   // [warp][R][2]
-    int   *s_base = reinterpret_cast<int *>(s_ml + kWarps * R * 2);
-    int   *s_len  = s_base + P.c.B + 1;
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    kv8_attn_kernel(const __grid_constant__ Kv8AttnParams P, const __grid_constant__ CUtensorMap kmap,
+                    const __grid_constant__ CUtensorMap vmap) {
+    constexpr int R       = 8 * NT;
+    constexpr int KS      = HD / 16;  // k-steps of S, m-tiles of O
+    constexpr int kSt     = stage_bytes<HD>();
+    constexpr int kStages = stages<HD, NT>();
+    constexpr int kOut    = HD + 4;  // floats between merged rows
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t  *smem   = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    float    *s_o    = reinterpret_cast<float *>(smem + kStages * kSt);  // [warp][R][kOut]
+    float    *s_ml   = s_o + kWarps * R * kOut;                          // [warp][R][2]
+    uint64_t *full   = reinterpret_cast<uint64_t *>(s_ml + kWarps * R * 2);
+    uint64_t *empty  = full + kStages;
+    volatile int *abort_f = reinterpret_cast<volatile int *>(empty + kStages);
+    float    *s_sc   = reinterpret_cast<float *>(empty + kStages + 1);  // [stage][K, V]
+    int      *s_base = reinterpret_cast<int *>(s_sc + 2 * kStages);
+    int      *s_len  = s_base + P.c.B + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     const int HU = P.c.Hkv * P.n_rb;  // units of a set
 
+    if (threadIdx.x == kThreads - 1) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&full[i], 3);  // the boxes, and a scale each
+            mbar_init(&empty[i], kWarps);
+        }
+        *abort_f = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&kmap);
+        prefetch_tensormap(&vmap);
+    }
     pdl_wait_primary();
     tile_table(s_base, s_len, P.len, P.c.B, P.c.n_max);
     const int T = s_base[P.c.B] * HU;
@@ -265,66 +273,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
         at.ub         = (int) ((unsigned) off / (unsigned) at.nt);
         at.t          = off - at.ub * at.nt;
     }
-    Walk ahead = at;
-
-    const uint32_t ring = smem_u32(smem) + (uint32_t) (warp * kStages * kSt);
-    // Copies this thread's part of a chunk.  K: rows g and g + 8, 16-B pieces c
-    // (and 4 + c) of each.  V: HD / 8 dims from g * HD / 8 of rows 2c, 2c + 1, 2c + 8,
-    // 2c + 9.  Rows past the length repeat the last one (they get no weight).
-    // Pointers to rows g and 2c of the chunk and to the block's scales move along.
-    const int64_t k_nb1 = P.c.k.nb1, v_nb1 = P.c.v.nb1;
-    const int8_t *kp, *vp;
-    const float  *ksp, *vsp;
-    auto aim = [&]() {
-        const int hk = kv_head(ahead);
-        const int j  = ahead.t * kKv8Block + warp * kChunk;
-        kp = P.c.k.q + (int64_t) hk * P.c.k.nb2 + (int64_t) ahead.b * P.c.k.nb3 + (j + g) * k_nb1 + 16 * c;
-        vp = P.c.v.q + (int64_t) hk * P.c.v.nb2 + (int64_t) ahead.b * P.c.v.nb3 + (j + 2 * c) * v_nb1 + (HD / 8) * g;
-        ksp = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.k.scale) + hk * P.c.k.s_nb2 +
-                                              ahead.b * P.c.k.s_nb3) +
-              ahead.t;
-        vsp = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.v.scale) + hk * P.c.v.s_nb2 +
-                                              ahead.b * P.c.v.s_nb3) +
-              ahead.t;
-    };
-    aim();
-    auto issue = [&](int st) {
-        const int      room = ahead.len - ahead.t * kKv8Block - warp * kChunk;  // rows of the chunk that exist
-        const uint32_t d    = ring + (uint32_t) (st * kSt) + (uint32_t) lane * 16;
-        const uint32_t dv   = HD == 128 ? d + 2048u : ring + (uint32_t) (st * kSt + 1024 + lane * 8);
-        if (room > 0) {
-            int kr[2] = {0, 8}, vr[4] = {0, 1, 8, 9};  // rows from g and from 2c
-            if (room < kChunk) {
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    kr[r] = min(g + kr[r], room - 1) - g;
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    vr[r] = min(2 * c + vr[r], room - 1) - 2 * c;
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-#pragma unroll
-                for (int e = 0; e < HD / 64; ++e) {
-                    cp16(d + (uint32_t) ((r * (HD / 64) + e) * 512), kp + kr[r] * k_nb1 + 64 * e);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if constexpr (HD == 128) {
-                    cp16(dv + (uint32_t) (r * 512), vp + vr[r] * v_nb1);
-                } else {
-                    cp8(dv + (uint32_t) (r * 256), vp + vr[r] * v_nb1);
-                }
-            }
-            const uint32_t sc = ring + (uint32_t) (st * kSt + 2 * kChunk * HD + lane * 4);
-            cp4(sc, ksp);
-            cp4(sc + 128, vsp);
-        }
-    };
-
     // This thread's row of Q of a unit (kPacked: rows 4 .. 7 are the low halves of 0 .. 3), or nullptr
     auto q_row = [&](const Walk &w, int nt, int &row) -> const char * {
         const int hk = kv_head(w);
@@ -334,18 +282,78 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                                   (int64_t) w.b * P.q.nb3
                             : nullptr;
     };
-    auto prefetch_rows = [&](const Walk &w) {  // on its way to L1 while the unit before is computed
-        if (w.b < P.c.B) {
+
+    if (warp == kWarps) {
+        // ============================ producer =================================
+        const float *ksp = nullptr, *vsp = nullptr;  // the tile's scales
+        int          hk = 0;
+        auto         aim = [&]() {
+            hk  = kv_head(at);
+            ksp = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.k.scale) + hk * P.c.k.s_nb2 +
+                                                  at.b * P.c.k.s_nb3) +
+                  at.t;
+            vsp = reinterpret_cast<const float *>(reinterpret_cast<const char *>(P.c.v.scale) + hk * P.c.v.s_nb2 +
+                                                  at.b * P.c.v.s_nb3) +
+                  at.t;
+        };
+        aim();
+        bool     ok = true;
+        int      st = 0;
+        uint32_t ph = 0;
+        for (int i = 0; i < n_my; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], ph ^ 1u, abort_f, P.dev_err, DEVERR_TIMEOUT_EMPTY,
+                                                           P.wait_limit_ns));
+            if (!ok) {
+                break;
+            }
+            if (lane == 0) {
+                uint8_t *dst = smem + st * kSt;
+                mbar_arrive_expect_tx(&full[st], kSt);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                int         row;
-                const char *p = q_row(w, nt, row);
-                if (p && warp == 0) {
-                    asm volatile("prefetch.global.L1 [%0];" ::"l"(p + (P.q.type == ACEFA_TYPE_F32 ? HD : HD / 2) * c));
+                for (int e = 0; e < HD / 64; ++e) {
+                    tma_load_4d(dst + e * (kKv8Block * 64), &kmap, 64 * e, at.t * kKv8Block, hk, at.b, &full[st]);
+                }
+                tma_load_4d(dst + kKv8Block * HD, &vmap, 0, at.t * kKv8Block, hk, at.b, &full[st]);
+            } else if (lane == 1) {
+                cp4_arrive(smem_u32(s_sc + 2 * st), ksp, &full[st]);
+            } else if (lane == 2) {
+                cp4_arrive(smem_u32(s_sc + 2 * st + 1), vsp, &full[st]);
+            }
+            if (++st == kStages) {
+                st = 0;
+                ph ^= 1u;
+            }
+            if (!advance(at)) {
+                ++ksp, ++vsp;
+            } else if (at.b < P.c.B) {
+                aim();
+                if (i + 1 < n_my) {  // the next unit's rows of Q, on their way to L1
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        int         row;
+                        const char *p = q_row(at, nt, row);
+                        if (p) {
+                            asm volatile("prefetch.global.L1 [%0];" ::"l"(p + (P.q.type == ACEFA_TYPE_F32 ? HD : HD / 2) * c));
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+        }
+        if (!ok) {
+            // let the copies in flight land before the CTA exits
+            const uint64_t ts = globaltimer_ns();
+            for (int i = 0; i < kStages; ++i) {
+                const uint32_t last = i < st ? ph : ph ^ 1u;  // the last use of stage i, if it had one
+                while (!mbar_try_wait(&full[i], last)) {
+                    if (globaltimer_ns() - ts > P.wait_limit_ns) {
+                        break;
+                    }
                 }
             }
         }
-    };
+        return;
+    }
 
     // ---- rows of the current unit
     uint32_t qh[NT][KS][2], ql[MODE == kSplit ? NT : 1][KS][2];  // Q^T operand, its (other) half
@@ -354,19 +362,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
     float    acc_o[NT][KS][4];
     float    m[NT][2], l[NT][2];
     float   *sp = nullptr;  // this thread's scores of the chunk, where weights are wanted
-    float    x[NT][KS][4];
-    auto read_rows = [&]() {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            int         row;
-            const char *p = q_row(at, nt, row);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                // word ks of this thread's K pieces: dims 64 * (ks / 4) + 16 * c + 4 * (ks % 4) ..
-                load_q4(p, P.q.type, 64 * (ks >> 2) + 16 * c + 4 * (ks & 3), x[nt][ks]);
-            }
-        }
-    };
     auto start_rows = [&]() {
         const int rb = at.ub - kv_head(at) * P.n_rb;
         if (P.scores) {
@@ -375,12 +370,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float top = 0.0f;
+            int         row;
+            const char *p = q_row(at, nt, row);
+            float       x[KS][4], top = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                // word ks of this thread's K pieces: dims 64 * (ks / 4) + 16 * c + 4 * (ks % 4) ..
+                load_q4(p, P.q.type, 64 * (ks >> 2) + 16 * c + 4 * (ks & 3), x[ks]);
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    top = fmaxf(top, fabsf(x[nt][ks][e]));
+                    top = fmaxf(top, fabsf(x[ks][e]));
                 }
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint32_t hi, lo;
-                    split2(x[nt][ks][2 * e] * f, x[nt][ks][2 * e + 1] * f, hi, lo);
+                    split2(x[ks][2 * e] * f, x[ks][2 * e + 1] * f, hi, lo);
                     qh[nt][ks][e] = MODE == kPacked && g >= 4 ? lo : hi;
                     if constexpr (MODE == kSplit) {
                         ql[nt][ks][e] = lo;
@@ -422,51 +424,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
         }
     };
 
-    auto next_ahead = [&]() {
-        if (advance(ahead)) {
-            if (ahead.b < P.c.B) {
-                aim();
-                prefetch_rows(ahead);
-            }
-        } else {
-            kp += kKv8Block * k_nb1;
-            vp += kKv8Block * v_nb1;
-            ++ksp, ++vsp;
-        }
-    };
-    read_rows();  // before the stream fills the queues
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-        if (i < n_my) {
-            issue(i);
-            next_ahead();
-        }
-        cp_commit();
-    }
     start_rows();
-    int stage = 0, free_stage = kStages - 1;
+    // K row g of this warp's chunk, 16-B piece c; V rows 2c .. of it, HD / 8 dims of g
+    const uint32_t k_at = smem_u32(smem) + (uint32_t) ((warp * kChunk + g) * 64 + 16 * c);
+    const uint32_t v_at = smem_u32(smem) + (uint32_t) (kKv8Block * HD + (warp * kChunk + 2 * c) * HD);
+    int            stage = 0;
+    uint32_t       phase = 0;
+    bool           ok    = true;
 
 #pragma unroll 1
     for (int i = 0; i < n_my; ++i) {
-        if (i + kStages - 1 < n_my) {
-            issue(free_stage);
-            next_ahead();
-        }
-        cp_commit();
-        cp_wait<kStages - 1>();
         const int j0 = at.t * kKv8Block + warp * kChunk;
-        if (j0 < at.len) {  // uniform over the warp
-            const uint32_t d  = ring + (uint32_t) (stage * kSt);
-            const uint32_t dl = d + (uint32_t) lane * 16;
-            const float    kd = lds_f32(d + 2 * kChunk * HD + lane * 4);
-            const float    vd = lds_f32(d + 2 * kChunk * HD + 128 + lane * 4);
+        // (after an expired wait the loop runs on without data, to meet the others at the barriers)
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], phase, abort_f, P.dev_err, DEVERR_TIMEOUT_FULL,
+                                                       P.wait_limit_ns)) && ok;
+        if (ok && j0 < at.len) {  // uniform over the warp
+            const float kd = s_sc[2 * stage], vd = s_sc[2 * stage + 1];
             // ---- S^T = K Q^T
             // (two sums per product, of the even and the odd k-steps: half as long a chain)
             float s[NT][4], s2[NT][MODE == kSplit ? 3 : 1][4];
 #pragma unroll
             for (int e4 = 0; e4 < HD / 64; ++e4) {
-                const uint4    wa    = lds_v4(dl + (uint32_t) (e4 * 512));
-                const uint4    wb    = lds_v4(dl + (uint32_t) ((HD / 64 + e4) * 512));
+                const uint32_t ka    = k_at + (uint32_t) (stage * kSt + e4 * (kKv8Block * 64));
+                const uint4    wa    = lds_v4(ka);
+                const uint4    wb    = lds_v4(ka + 8 * 64);
                 const uint32_t va[4] = {wa.x, wa.y, wa.z, wa.w}, vb[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -589,13 +570,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
             uint32_t v[4][HD / 32];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if constexpr (HD == 128) {
-                    const uint4 w = lds_v4(dl + (uint32_t) (2048 + r * 512));
+                const int      row = (r & 1) + 8 * (r >> 1);  // from 2c
+                const uint32_t va  = v_at + (uint32_t) (stage * kSt + row * HD);
+                if constexpr (HD == 128) {  // 128-B swizzle: piece ^ (row & 7)
+                    const uint4 w = lds_v4(va + (uint32_t) ((g ^ (2 * c + (r & 1))) << 4));
                     v[r][0] = w.x, v[r][1] = w.y, v[r][2] = w.z, v[r][3] = w.w;
-                } else {
-                    const uint2 w = lds_v2(d + (uint32_t) (1024 + r * 256 + lane * 8));
+                } else {  // 64-B swizzle: piece ^ ((row >> 1) & 3)
+                    const uint2 w = lds_v2(va + (uint32_t) (((g >> 1) ^ c) << 4) + 8 * (g & 1));
                     v[r][0] = w.x, v[r][1] = w.y;
                 }
+            }
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&empty[stage]);  // the warp's bytes are in registers
             }
 #pragma unroll
             for (int t = 0; t < KS; ++t) {
@@ -618,17 +605,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                 }
             }
         }
+        else if (lane == 0) {
+            mbar_arrive(&empty[stage]);
+        }
         // ---- end of the unit (or of this CTA's run): merge the warps' results
         const int  unit = at.b * HU + at.ub;
         const int  rb   = at.ub - kv_head(at) * P.n_rb;
         const bool next = advance(at);
-        stage           = stage == kStages - 1 ? 0 : stage + 1;
-        free_stage      = free_stage == kStages - 1 ? 0 : free_stage + 1;
+        if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+        }
         if (P.scores) {
             sp += kKv8Block * P.score_stride;
         }
         if (next || i + 1 == n_my) {
-            __syncthreads();  // the previous merge has been read
+            named_bar_sync(1, 32 * kWarps);  // the previous merge has been read
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -651,10 +643,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                     }
                 }
             }
-            __syncthreads();
+            named_bar_sync(1, 32 * kWarps);
             const int n_row = min(R, P.rows - rb * R);
             float    *slot  = P.part + (int64_t) (blockIdx.x + unit) * (R * (HD + 2));
-            for (int x = threadIdx.x; x < n_row * (HD / 4); x += kThreads) {
+            for (int x = threadIdx.x; x < n_row * (HD / 4); x += 32 * kWarps) {
                 const int row = x / (HD / 4), d4 = x % (HD / 4);
                 float     mw[kWarps], M = kNoMax;
 #pragma unroll
@@ -682,7 +674,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT))
                 }
             }
             if (i + 1 < n_my) {
-                read_rows();
                 start_rows();
             }
         }
@@ -823,8 +814,25 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
     }
 }
 
+// K or V of the cache as [D, n_max, Hkv, B] bytes; boxes of `inner` dims x 64 rows.
+bool encode_side(CUtensorMap *map, const Kv8Dev &c, const Kv8Side &side, int inner, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn enc = tensor_map_encoder();
+    if (!enc) {
+        return false;
+    }
+    // strides of extent-1 dims do not matter; keep them 16-B multiples
+    const cuuint64_t s1 = c.n_max > 1 ? (cuuint64_t) side.nb1 : (cuuint64_t) c.D;
+    const cuuint64_t s2 = c.Hkv > 1 ? (cuuint64_t) side.nb2 : s1 * (cuuint64_t) c.n_max;
+    const cuuint64_t s3 = c.B > 1 ? (cuuint64_t) side.nb3 : s2 * (cuuint64_t) c.Hkv;
+    cuuint64_t dims[4] = {(cuuint64_t) c.D, (cuuint64_t) c.n_max, (cuuint64_t) c.Hkv, (cuuint64_t) c.B};
+    cuuint64_t strides[3] = {s1, s2, s3};
+    cuuint32_t box[4] = {(cuuint32_t) inner, kKv8Block, 1, 1}, estr[4] = {1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, side.q, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int HD, int NT, int MODE>
-cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
+cudaError_t launch(const Kv8AttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t s) {
     const int              smem = attn_smem_bytes<HD, NT>(p.c.B);
     static thread_local int configured = -1;
     int                     dev        = 0;
@@ -847,7 +855,7 @@ cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
     cfg.stream             = s;
     cfg.attrs              = attr;
     cfg.numAttrs           = 1;
-    cudaError_t e          = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT, MODE>, p);
+    cudaError_t e          = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT, MODE>, p, km, vm);
     if (e != cudaSuccess) {
         return e;
     }
@@ -861,19 +869,25 @@ cudaError_t launch(const Kv8AttnParams &p, cudaStream_t s) {
 
 }  // namespace
 
-int kv8_attn_ctas_per_sm(int unit_rows) { return ctas_per_sm(unit_rows / 8); }
+int kv8_attn_ctas_per_sm() { return kCtasPerSm; }
 
-cudaError_t launch_kv8_attn(const Kv8AttnParams &p, cudaStream_t s) {
-    const bool one = p.q.type != ACEFA_TYPE_F32 && p.dst.type != ACEFA_TYPE_F32;
+int launch_kv8_attn(const Kv8AttnParams &p, cudaStream_t s) {
+    CUtensorMap km, vm;
+    if (!encode_side(&km, p.c, p.c.k, 64, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !encode_side(&vm, p.c, p.c.v, p.c.D, p.c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B)) {
+        return ACEFA_ERR_LAYOUT;
+    }
+    const bool one  = p.q.type != ACEFA_TYPE_F32 && p.dst.type != ACEFA_TYPE_F32;
     auto       pick = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        if (kv8_unit_rows(p.rows) == 16) {
-            return one ? launch<HD, 2, kOne>(p, s) : launch<HD, 2, kSplit>(p, s);
+        if (kv8_unit_rows(p.rows, p.q.type) == 16) {
+            return one ? launch<HD, 2, kOne>(p, km, vm, s) : launch<HD, 2, kSplit>(p, km, vm, s);
         }
-        return one ? launch<HD, 1, kOne>(p, s)
-                   : (p.rows <= 4 ? launch<HD, 1, kPacked>(p, s) : launch<HD, 1, kSplit>(p, s));
+        return one ? launch<HD, 1, kOne>(p, km, vm, s)
+                   : (p.rows <= 4 ? launch<HD, 1, kPacked>(p, km, vm, s) : launch<HD, 1, kSplit>(p, km, vm, s));
     };
-    return p.c.D == 128 ? pick(std::integral_constant<int, 128>{}) : pick(std::integral_constant<int, 64>{});
+    const cudaError_t e = p.c.D == 128 ? pick(std::integral_constant<int, 128>{}) : pick(std::integral_constant<int, 64>{});
+    return e == cudaSuccess ? ACEFA_OK : ACEFA_ERR_CUDA;
 }
 
 }  // namespace acefa

@@ -58,6 +58,8 @@ struct Kv8AttnParams {
     float         *part;          // partial results, one slot per (CTA, unit) that meet
     float         *scores;        // [unit][n_max][score_stride] log2-unit scores, with weights only
     int            score_stride;
+    int           *dev_err;
+    uint64_t       wait_limit_ns;
 };
 struct Kv8EvictParams {
     Kv8Dev         c, out;
@@ -74,13 +76,15 @@ struct Kv8EvictParams {
 
 cudaError_t launch_kv8_store(const Kv8StoreParams &p, cudaStream_t s);
 cudaError_t launch_kv8_load(const Kv8LoadParams &p, cudaStream_t s);
-cudaError_t launch_kv8_attn(const Kv8AttnParams &p, cudaStream_t s);
+int         launch_kv8_attn(const Kv8AttnParams &p, cudaStream_t s);  // acefa_status
 cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s);
 
-// Rows of a unit of the attention kernel (8 or 16) and the CTAs that it may
-// keep resident on one SM; functions of the operands alone.
-inline int kv8_unit_rows(int rows) { return rows <= 8 ? 8 : 16; }
-int        kv8_attn_ctas_per_sm(int unit_rows);
+// Rows of a unit of the attention kernel and the CTAs that it may keep
+// resident on one SM; functions of the operands alone.  More than eight F32
+// rows go in units of eight that read the keys again (from L2): split Q
+// fragments of sixteen rows do not fit the registers of two CTAs per SM.
+inline int kv8_unit_rows(int rows, int q_type) { return rows <= 8 || q_type == ACEFA_TYPE_F32 ? 8 : 16; }
+int        kv8_attn_ctas_per_sm();
 inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows * (D + 2); }
 
 // ------------------------------------------------------------------ device helpers
