@@ -109,32 +109,63 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo              = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// Four values of a Q row from element e on (zeros without a row).
-__device__ __forceinline__ void load_q4(const char *p, int type, int e, float (&x)[4]) {
+// This thread's HD / 4 values of a Q row (zeros without one): four from dim
+// 64 * (ks / 4) + 16 * c + 4 * (ks % 4) for each k-step.  The type and the
+// alignment are looked at once, so that all loads leave together.
+template <int HD>
+__device__ __forceinline__ void load_q(const char *p, int type, int c, float (&x)[HD / 16][4]) {
+    constexpr int KS = HD / 16;
+    auto          at = [&](int ks) { return 64 * (ks >> 2) + 16 * c + 4 * (ks & 3); };
     if (!p) {
-        x[0] = x[1] = x[2] = x[3] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            x[ks][0] = x[ks][1] = x[ks][2] = x[ks][3] = 0.0f;
+        }
     } else if (type == ACEFA_TYPE_F32) {
-        const float *f = reinterpret_cast<const float *>(p) + e;
+        const float *f = reinterpret_cast<const float *>(p);
         if ((reinterpret_cast<uintptr_t>(f) & 15u) == 0) {
-            const float4 v = *reinterpret_cast<const float4 *>(f);
-            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+            float4 v[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                v[ks] = *reinterpret_cast<const float4 *>(f + at(ks));
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                x[ks][0] = v[ks].x, x[ks][1] = v[ks].y, x[ks][2] = v[ks].z, x[ks][3] = v[ks].w;
+            }
         } else {
-            x[0] = f[0], x[1] = f[1], x[2] = f[2], x[3] = f[3];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[ks][e] = f[at(ks) + e];
+                }
+            }
         }
     } else {
-        const uint16_t *h = reinterpret_cast<const uint16_t *>(p) + e;
-        uint32_t        w[2];
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+        uint2           w[KS];
         if ((reinterpret_cast<uintptr_t>(h) & 7u) == 0) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(h);
-            w[0] = v.x, w[1] = v.y;
-        } else {
-            w[0] = h[0] | (uint32_t) h[1] << 16;
-            w[1] = h[2] | (uint32_t) h[3] << 16;
-        }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint16_t b = (uint16_t) (w[k >> 1] >> (16 * (k & 1)));
-            x[k] = type == ACEFA_TYPE_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t) b << 16);
+            for (int ks = 0; ks < KS; ++ks) {
+                w[ks] = *reinterpret_cast<const uint2 *>(h + at(ks));
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint16_t *q = h + at(ks);
+                w[ks] = make_uint2(q[0] | (uint32_t) q[1] << 16, q[2] | (uint32_t) q[3] << 16);
+            }
+        }
+        const bool f16 = type == ACEFA_TYPE_F16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t v = e < 2 ? w[ks].x : w[ks].y;
+                const uint32_t b = e & 1 ? v >> 16 : v & 0xFFFFu;
+                x[ks][e] = f16 ? __half2float(__ushort_as_half((uint16_t) b)) : __uint_as_float(b << 16);
+            }
         }
     }
 }
@@ -373,11 +404,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             int         row;
             const char *p = q_row(at, nt, row);
             float       x[KS][4], top = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                // word ks of this thread's K pieces: dims 64 * (ks / 4) + 16 * c + 4 * (ks % 4) ..
-                load_q4(p, P.q.type, 64 * (ks >> 2) + 16 * c + 4 * (ks & 3), x[ks]);
-            }
+            load_q<HD>(p, P.q.type, c, x);  // (the dims of the words of this thread's K pieces)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -683,11 +710,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 // ---------------------------------------------------------------------------
 // The second launch.  CTAs below n_out finish one row each: O = sum of the
 // partials, each times 2^(m - M), over their summed l.  The others add the
-// weights of 1024 keys of a (set, KV head): p = 2^(s - M) / L summed over the
+// weights of 256 keys of a (set, KV head): p = 2^(s - M) / L summed over the
 // head's rows, whose M and L come from the same partials.  Every sum has a
 // fixed order, so results do not depend on scheduling.
 constexpr int kSumThreads = 128;
-constexpr int kSumKeys    = 512;
+constexpr int kSumKeys    = 2 * kSumThreads;  // of a CTA
 
 // Over the slots c0 .. c1 of a row (base: its first m, l at + R): the maximum
 // and the sum of l * 2^(m - maximum).  The whole warp, lanes side by side.
@@ -782,6 +809,24 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
         return;
     }
     pdl_wait_primary();
+    // two keys per thread; the scores of the first row block are on their way
+    // while the rows' sums are put together
+    const int     st    = P.score_stride;  // even
+    const int     j[2]  = {j0 + (int) threadIdx.x, j0 + (int) threadIdx.x + kSumThreads};
+    const float2 *sp    = reinterpret_cast<const float2 *>(P.scores + (int64_t) (b * HU + hk * P.n_rb) * P.c.n_max * st);
+    float2        s[2][8];
+    auto          fetch = [&](int rb) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                s[k][r] = j[k] < len && 2 * r < st
+                                       ? __ldcg(sp + ((int64_t) rb * P.c.n_max + j[k]) * (st >> 1) + r)
+                                       : make_float2(-INFINITY, -INFINITY);
+            }
+        }
+    };
+    fetch(0);
     for (int row = warp; row < P.rows; row += kSumThreads / 32) {
         const int ub = hk * P.n_rb + row / R;
         int       c0, c1;
@@ -793,24 +838,27 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
         }
     }
     __syncthreads();
-    float *wp = reinterpret_cast<float *>(P.weight + (int64_t) hk * P.w_nb2 + (int64_t) b * P.w_nb3);
-    const int st = P.score_stride;  // even
-    for (int j = j0 + threadIdx.x; j < min(len, j0 + kSumKeys); j += kSumThreads) {
-        float sum = 0.0f;
-        for (int rb = 0; rb < P.n_rb; ++rb) {
-            const float2 *sp    = reinterpret_cast<const float2 *>(
-                P.scores + ((int64_t) (b * HU + hk * P.n_rb + rb) * P.c.n_max + j) * st);
-            const int     n_row = min(R, P.rows - rb * R);
-#pragma unroll 4
-            for (int r = 0; r < n_row; r += 2) {
-                const float2 s = __ldcg(sp + (r >> 1));
-                sum += exp2f(s.x - s_lse[rb * R + r]);
-                if (r + 1 < n_row) {
-                    sum += exp2f(s.y - s_lse[rb * R + r + 1]);
-                }
+    float sum[2] = {0.0f, 0.0f};
+    for (int rb = 0; rb < P.n_rb; ++rb) {
+        if (rb) {
+            fetch(rb);
+        }
+        const int n_row = min(R, P.rows - rb * R);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if (r < n_row) {
+                const float lse = s_lse[rb * R + r];
+                sum[0] += exp2f((r & 1 ? s[0][r >> 1].y : s[0][r >> 1].x) - lse);
+                sum[1] += exp2f((r & 1 ? s[1][r >> 1].y : s[1][r >> 1].x) - lse);
             }
         }
-        wp[j] += sum;
+    }
+    float *wp = reinterpret_cast<float *>(P.weight + (int64_t) hk * P.w_nb2 + (int64_t) b * P.w_nb3);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if (j[k] < len) {
+            wp[j[k]] += sum[k];
+        }
     }
 }
 
