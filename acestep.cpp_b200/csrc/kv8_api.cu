@@ -185,9 +185,9 @@ int plan_attn(const acefa_tensor *q, const acefa_kv8_cache *cache, const acefa_t
     const int R = kv8_unit_rows(p.rows, q->type);
     p.n_rb      = (p.rows + R - 1) / R;
     const int64_t units = (int64_t) p.c.B * p.c.Hkv * p.n_rb;
-    const int64_t tiles = units * ((p.c.n_max + kKv8Block - 1) / kKv8Block);
+    const int64_t tiles = units * ((p.c.n_max + kKv8Block - 1) / kKv8Block);  // places of the kernel: + 2 per unit
     const int64_t weigh = weight ? (int64_t) p.c.B * p.c.Hkv * (p.c.n_max / 256 + 1) : 0;
-    if (tiles >= (1ll << 31) || units * R + weigh >= (1ll << 31)) {
+    if (tiles + 2 * units >= (1ll << 31) || units * R + weigh >= (1ll << 31)) {
         return ACEFA_ERR_SHAPE;
     }
     DeviceCtx ctx;

@@ -17,7 +17,9 @@
 // Work.  The (set, KV head, row block) units' 64-key tiles, numbered one after
 // another over all sets' actual lengths, are cut into equal runs, one per CTA:
 // ragged batches balance as well as even ones, and the grid depends on shapes
-// only.  A producer warp streams a CTA's tiles by TMA through a ring of stages,
+// only.  A unit counts as kUnitCost places more than it has tiles, about what
+// beginning and merging it takes (without them a CTA could get many
+// units of one tile: 8 sets of 1 .. 2560 rows took 18 us instead of 10).  A producer warp streams a CTA's tiles by TMA through a ring of stages,
 // their two scales beside them by cp.async; four consumer warps take 16 keys of
 // every tile each and meet only at the end of a unit.  The dims and keys of
 // a fragment are assigned such that a thread's bytes are 16-B pieces of rows
@@ -28,6 +30,7 @@
 // S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
 // operand layout by four movmatrix.  The running maximum moves only when a
 // score exceeds it by more than 2^8 (a warp vote), as in the other kernels.
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8_internal.h"
@@ -40,6 +43,7 @@ constexpr int   kWarps   = 4;  // consumers
 constexpr int   kThreads = 32 * (kWarps + 1);
 constexpr int   kChunk   = 16;  // keys of one warp and tile
 constexpr float kSlack   = 8.0f;
+constexpr int   kUnitCost = 2;
 // "No maximum yet": below every score, finite so that differences stay numbers
 // (2^(anything - it) only meets weights and sums that are 0).
 constexpr float kNoMax = -1.7e38f;
@@ -179,15 +183,16 @@ __device__ __forceinline__ void store1(char *p, int type, int e, float x) {
     }
 }
 
-// base[b] = 64-key tiles of the sets before b, b = 0 .. B (the last is the
-// total per head and row block), lens[b] = length.  All threads; ends with a barrier.
+// base[b] = places of one unit of each set before b, b = 0 .. B: its 64-key tiles
+// and, ahead of them, kUnitCost (none without tiles); lens[b] = length.  All
+// threads; ends with a barrier.
 __device__ __forceinline__ void tile_table(int *base, int *lens, const int32_t *len, int B, int n_max) {
     const int lane = threadIdx.x & 31;
     if (threadIdx.x < 32) {
         int acc = 0;
         for (int b0 = 0; b0 < B; b0 += 32) {
             const int n = b0 + lane < B ? clamp_len(__ldg(len + b0 + lane), n_max) : 0;
-            int       v = (n + kKv8Block - 1) / kKv8Block;
+            int       v = n ? (n + kKv8Block - 1) / kKv8Block + kUnitCost : 0;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
                 const int u = __shfl_up_sync(0xffffffffu, v, off);
@@ -206,15 +211,16 @@ __device__ __forceinline__ void tile_table(int *base, int *lens, const int32_t *
     __syncthreads();
 }
 
-// Run of tiles of CTA c of C: [T * c / C, T * (c + 1) / C).  C <= T, so no run
-// is empty and the CTAs that meet a unit are consecutive.
+// Run of places of CTA c of C: [T * c / C, T * (c + 1) / C).  C <= T, so no run
+// is empty and the CTAs that meet a unit's tiles are consecutive.
 __device__ __forceinline__ int run_start(int T, int C, int c) { return (int) ((int64_t) T * c / C); }
-// the CTA whose run holds tile x
+// the CTA whose run holds place x
 __device__ __forceinline__ int cta_of(int T, int C, int x) { return (int) ((((int64_t) x + 1) * C - 1) / T); }
 
 // A position in the sequence of tiles.
 struct Walk {
     int b, ub, t, nt, len;  // set, unit of the set, tile of the unit, its tiles, the set's length
+    int at;                 // place
 };
 
 // D = A B (a product that starts a sum)
@@ -266,13 +272,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     if ((int) blockIdx.x >= C) {
         return;
     }
-    const int x0 = run_start(T, C, blockIdx.x), n_my = run_start(T, C, blockIdx.x + 1) - x0;
+    const int x0 = run_start(T, C, blockIdx.x), x1 = run_start(T, C, blockIdx.x + 1);
 
     auto advance = [&](Walk &w) {  // true: a new unit
+        ++w.at;
         if (++w.t < w.nt) {
             return false;
         }
         w.t = 0;
+        w.at += kUnitCost;
         if (++w.ub == HU) {
             w.ub = 0;
             do {
@@ -281,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             if (w.b == P.c.B) {
                 return true;
             }
-            w.nt  = s_base[w.b + 1] - s_base[w.b];
+            w.nt  = s_base[w.b + 1] - s_base[w.b] - kUnitCost;
             w.len = s_len[w.b];
         }
         return true;
@@ -289,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     auto kv_head = [&](const Walk &w) { return P.n_rb == 1 ? w.ub : w.ub / P.n_rb; };
     Walk at;
     {
-        // the set whose tiles hold x0: base[b] * HU <= x0 < base[b + 1] * HU, by 32nds
+        // the set whose places hold x0: base[b] * HU <= x0 < base[b + 1] * HU, by 32nds
         int lo = 0, n = P.c.B;
         while (n > 1) {
             const int step = (n + 31) >> 5, i = lo + lane * step;
@@ -298,11 +306,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             lo += (below - 1) * step;
         }
         at.b          = lo;
-        at.nt         = s_base[lo + 1] - s_base[lo];
+        const int per = s_base[lo + 1] - s_base[lo];
+        at.nt         = per - kUnitCost;
         at.len        = s_len[lo];
         const int off = x0 - s_base[lo] * HU;
-        at.ub         = (int) ((unsigned) off / (unsigned) at.nt);
-        at.t          = off - at.ub * at.nt;
+        at.ub         = (int) ((unsigned) off / (unsigned) per);
+        const int r   = off - at.ub * per;
+        at.t          = max(r - kUnitCost, 0);
+        at.at         = x0 + max(kUnitCost - r, 0);
+    }
+    if (at.at >= x1) {
+        return;  // no tile in this run
     }
     // This thread's row of Q of a unit (kPacked: rows 4 .. 7 are the low halves of 0 .. 3), or nullptr
     auto q_row = [&](const Walk &w, int nt, int &row) -> const char * {
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         bool     ok = true;
         int      st = 0;
         uint32_t ph = 0;
-        for (int i = 0; i < n_my; ++i) {
+        while (at.at < x1) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], ph ^ 1u, abort_f, P.dev_err, DEVERR_TIMEOUT_EMPTY,
                                                            P.wait_limit_ns));
             if (!ok) {
@@ -358,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 ++ksp, ++vsp;
             } else if (at.b < P.c.B) {
                 aim();
-                if (i + 1 < n_my) {  // the next unit's rows of Q, on their way to L1
+                if (at.at < x1) {  // the next unit's rows of Q, on their way to L1
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         int         row;
@@ -460,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     bool           ok    = true;
 
 #pragma unroll 1
-    for (int i = 0; i < n_my; ++i) {
+    while (at.at < x1) {
         const int j0 = at.t * kKv8Block + warp * kChunk;
         // (after an expired wait the loop runs on without data, to meet the others at the barriers)
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], phase, abort_f, P.dev_err, DEVERR_TIMEOUT_FULL,
@@ -646,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (P.scores) {
             sp += kKv8Block * P.score_stride;
         }
-        if (next || i + 1 == n_my) {
+        if (next || at.at >= x1) {
             named_bar_sync(1, 32 * kWarps);  // the previous merge has been read
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -700,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     slot[R * HD + R + row] = L;
                 }
             }
-            if (i + 1 < n_my) {
+            if (at.at < x1) {
                 start_rows();
             }
         }
@@ -710,42 +724,49 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 // ---------------------------------------------------------------------------
 // The second launch.  CTAs below n_out finish one row each: O = sum of the
 // partials, each times 2^(m - M), over their summed l.  The others add the
-// weights of 256 keys of a (set, KV head): p = 2^(s - M) / L summed over the
+// weights of a few hundred keys of a (set, KV head): p = 2^(s - M) / L summed over the
 // head's rows, whose M and L come from the same partials.  Every sum has a
 // fixed order, so results do not depend on scheduling.
 constexpr int kSumThreads = 128;
-constexpr int kSumKeys    = 2 * kSumThreads;  // of a CTA
+constexpr int kSumKeys    = 2 * kSumThreads;  // at a time
+constexpr int kSumCtas    = 1024;             // about what the device holds
 
-// Over the slots c0 .. c1 of a row (base: its first m, l at + R): the maximum
-// and the sum of l * 2^(m - maximum).  The whole warp, lanes side by side.
-__device__ __forceinline__ void merge_row(const float *base, int64_t slot_f, int R, int c0, int c1, float &M, float &L) {
-    const int lane = threadIdx.x & 31;
-    M              = -INFINITY;
-    L              = 0.0f;
-    for (int k = c0 + lane; k <= c1; k += 32) {
-        const float m = __ldcg(base + k * slot_f), l = __ldcg(base + k * slot_f + R);
-        const float mn = fmaxf(M, m), mu = mn == -INFINITY ? 0.0f : mn;
-        L = L * exp2f(M - mu) + l * exp2f(m - mu);
-        M = mn;
-    }
+// A maximum and the sum of l * 2^(m - maximum), joined with another pair.
+__device__ __forceinline__ void join(float &M, float &L, float m, float l) {
+    const float mn = fmaxf(M, m), mu = mn == -INFINITY ? 0.0f : mn;
+    L = L * fast_exp2(M - mu) + l * fast_exp2(m - mu);
+    M = mn;
+}
+// The pairs of a row in slots c0 + first, c0 + first + step .. c1 (base: its
+// first m; l is R further), four loads of each on their way at a time.
+__device__ __forceinline__ void join_slots(const float *base, int64_t slot_f, int R, int first, int step, int c0, int c1,
+                                           float &M, float &L) {
+    M = -INFINITY;
+    L = 0.0f;
+    for (int k = c0 + first; k <= c1; k += 4 * step) {
+        float m[4], l[4];
 #pragma unroll
-    for (int off = 16; off; off >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, M, off), l = __shfl_xor_sync(0xffffffffu, L, off);
-        const float mn = fmaxf(M, m), mu = mn == -INFINITY ? 0.0f : mn;
-        L = L * exp2f(M - mu) + l * exp2f(m - mu);
-        M = mn;
+        for (int e = 0; e < 4; ++e) {
+            const bool on = k + e * step <= c1;
+            m[e] = on ? __ldcg(base + (k + e * step) * slot_f) : -INFINITY;
+            l[e] = on ? __ldcg(base + (k + e * step) * slot_f + R) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            join(M, L, m[e], l[e]);
+        }
     }
-    L = __shfl_sync(0xffffffffu, L, 0);  // (the lanes' sums differ in the order of their terms)
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_constant__ Kv8AttnParams P, int R,
-                                                                   int n_out, int key_chunks) {
+                                                                   int n_out, int key_chunks, int keys) {
     extern __shared__ __align__(16) int s_tab[];  // tile table and lengths
     __shared__ float  s_lse[ACEFA_KV8_MAX_ROWS];
     __shared__ float4 s_o[4][HD / 4];
+    __shared__ float2 s_join[kSumThreads];
     int          *s_base = s_tab, *s_len = s_tab + P.c.B + 1;
-    const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int     lane = threadIdx.x & 31;
     const int64_t slot_f = (int64_t) R * (HD + 2);
     const int     HU     = P.c.Hkv * P.n_rb;
     // (the lengths are older than the split kernel, which let this one start only after its own wait)
@@ -753,10 +774,10 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
     const int T = s_base[P.c.B] * HU, C = min(P.n_cta, T);
     // the CTAs of the split kernel that met a unit: slots (c + unit), c0 <= c <= c1
     auto range_of = [&](int b, int ub, int &c0, int &c1) {
-        const int nt = s_base[b + 1] - s_base[b];
-        const int a  = s_base[b] * HU + ub * nt;
-        c0 = nt ? cta_of(T, C, a) : 0;
-        c1 = nt ? cta_of(T, C, a + nt - 1) : -1;
+        const int per = s_base[b + 1] - s_base[b];
+        const int a   = s_base[b] * HU + ub * per;
+        c0 = per ? cta_of(T, C, a + kUnitCost) : 0;
+        c1 = per ? cta_of(T, C, a + per - 1) : -1;
     };
     if ((int) blockIdx.x < n_out) {
         const int row = blockIdx.x % P.rows, bh = blockIdx.x / P.rows;
@@ -767,7 +788,12 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
         const float *base = P.part + (int64_t) (b * HU + ub) * slot_f;
         pdl_wait_primary();
         float M, L;
-        merge_row(base + R * HD + r, slot_f, R, c0, c1, M, L);
+        join_slots(base + R * HD + r, slot_f, R, lane, 32, c0, c1, M, L);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) {
+            join(M, L, __shfl_xor_sync(0xffffffffu, M, off), __shfl_xor_sync(0xffffffffu, L, off));
+        }
+        L = __shfl_sync(0xffffffffu, L, 0);  // (the lanes' sums differ in the order of their terms)
         const float Mu = M == -INFINITY ? 0.0f : M;
         const int   w = threadIdx.x / (HD / 4), d4 = threadIdx.x % (HD / 4);
         constexpr int W = kSumThreads / (HD / 4);  // slots summed side by side
@@ -802,7 +828,7 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
         return;
     }
     const int x = (int) blockIdx.x - n_out;
-    const int bh = x / key_chunks, j0 = x % key_chunks * kSumKeys;
+    const int bh = x / key_chunks, j0 = x % key_chunks * keys;
     const int hk = bh % P.c.Hkv, b = bh / P.c.Hkv;
     const int len = s_len[b];
     if (j0 >= len) {
@@ -812,7 +838,8 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
     // two keys per thread; the scores of the first row block are on their way
     // while the rows' sums are put together
     const int     st    = P.score_stride;  // even
-    const int     j[2]  = {j0 + (int) threadIdx.x, j0 + (int) threadIdx.x + kSumThreads};
+    const int     j_end = min(len, j0 + keys);
+    int           j[2]  = {j0 + (int) threadIdx.x, j0 + (int) threadIdx.x + kSumThreads};
     const float2 *sp    = reinterpret_cast<const float2 *>(P.scores + (int64_t) (b * HU + hk * P.n_rb) * P.c.n_max * st);
     float2        s[2][8];
     auto          fetch = [&](int rb) {
@@ -820,44 +847,60 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                s[k][r] = j[k] < len && 2 * r < st
+                s[k][r] = j[k] < j_end && 2 * r < st
                                        ? __ldcg(sp + ((int64_t) rb * P.c.n_max + j[k]) * (st >> 1) + r)
                                        : make_float2(-INFINITY, -INFINITY);
             }
         }
     };
     fetch(0);
-    for (int row = warp; row < P.rows; row += kSumThreads / 32) {
-        const int ub = hk * P.n_rb + row / R;
+    // every row's maximum and sum: thread = (row of the block, share of its slots)
+    const int n_sh = kSumThreads / R, row = (int) threadIdx.x % R, sh = (int) threadIdx.x / R;
+    for (int rb = 0; rb < P.n_rb; ++rb) {
+        const int ub = hk * P.n_rb + rb;
         int       c0, c1;
         range_of(b, ub, c0, c1);
-        float M, L;
-        merge_row(P.part + (int64_t) (b * HU + ub) * slot_f + R * HD + row % R, slot_f, R, c0, c1, M, L);
-        if (lane == 0) {  // an empty row weighs nothing
-            s_lse[row] = L == 0.0f ? INFINITY : (M == -INFINITY ? 0.0f : M) + log2f(L);
+        float M = -INFINITY, L = 0.0f;
+        if (rb * R + row < P.rows) {
+            join_slots(P.part + (int64_t) (b * HU + ub) * slot_f + R * HD + row, slot_f, R, sh, n_sh, c0, c1, M, L);
         }
-    }
-    __syncthreads();
-    float sum[2] = {0.0f, 0.0f};
-    for (int rb = 0; rb < P.n_rb; ++rb) {
-        if (rb) {
-            fetch(rb);
-        }
-        const int n_row = min(R, P.rows - rb * R);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            if (r < n_row) {
-                const float lse = s_lse[rb * R + r];
-                sum[0] += exp2f((r & 1 ? s[0][r >> 1].y : s[0][r >> 1].x) - lse);
-                sum[1] += exp2f((r & 1 ? s[1][r >> 1].y : s[1][r >> 1].x) - lse);
+        s_join[threadIdx.x] = make_float2(M, L);
+        __syncthreads();
+        if (sh == 0 && rb * R + row < P.rows) {
+            for (int k = 1; k < n_sh; ++k) {
+                const float2 v = s_join[k * R + row];
+                join(M, L, v.x, v.y);
             }
+            // an empty row weighs nothing
+            s_lse[rb * R + row] = L == 0.0f ? INFINITY : (M == -INFINITY ? 0.0f : M) + log2f(L);
         }
+        __syncthreads();
     }
     float *wp = reinterpret_cast<float *>(P.weight + (int64_t) hk * P.w_nb2 + (int64_t) b * P.w_nb3);
+    for (int jb = j0; jb < j_end; jb += kSumKeys) {
+        float sum[2] = {0.0f, 0.0f};
+        for (int rb = 0; rb < P.n_rb; ++rb) {
+            if (rb) {
+                fetch(rb);
+            }
+            const int n_row = min(R, P.rows - rb * R);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        if (j[k] < len) {
-            wp[j[k]] += sum[k];
+            for (int r = 0; r < 16; ++r) {
+                if (r < n_row) {
+                    const float lse = s_lse[rb * R + r];
+                    sum[0] += fast_exp2((r & 1 ? s[0][r >> 1].y : s[0][r >> 1].x) - lse);
+                    sum[1] += fast_exp2((r & 1 ? s[1][r >> 1].y : s[1][r >> 1].x) - lse);
+                }
+            }
+        }
+        const int w[2] = {j[0], j[1]};
+        j[0] += kSumKeys, j[1] += kSumKeys;
+        fetch(0);  // (nothing behind the last)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (w[k] < j_end) {
+                wp[w[k]] += sum[k];
+            }
         }
     }
 }
@@ -908,11 +951,14 @@ cudaError_t launch(const Kv8AttnParams &p, const CUtensorMap &km, const CUtensor
         return e;
     }
     const int n_out      = p.c.B * p.c.Hkv * p.rows;
-    const int key_chunks = (p.c.n_max + kSumKeys - 1) / kSumKeys;
+    // keys of a CTA: enough for about kSumCtas of them in all
+    const int64_t all  = (int64_t) p.c.B * p.c.Hkv * p.c.n_max;
+    const int     keys = (int) std::max<int64_t>(1, std::min<int64_t>(all / kSumCtas, p.c.n_max) / kSumKeys) * kSumKeys;
+    const int     key_chunks = (p.c.n_max + keys - 1) / keys;
     cfg.gridDim          = dim3((unsigned) (n_out + (p.weight ? p.c.B * p.c.Hkv * key_chunks : 0)));
     cfg.blockDim         = dim3(kSumThreads);
     cfg.dynamicSmemBytes = sizeof(int) * (2 * (size_t) p.c.B + 1);
-    return cudaLaunchKernelEx(&cfg, kv8_attn_sum_kernel<HD>, p, 8 * NT, n_out, key_chunks);
+    return cudaLaunchKernelEx(&cfg, kv8_attn_sum_kernel<HD>, p, 8 * NT, n_out, key_chunks, keys);
 }
 
 }  // namespace
