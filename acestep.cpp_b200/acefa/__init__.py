@@ -512,29 +512,39 @@ class _Call:
     """An entry with its operands: keeps the tensors alive, runs on their device,
     on the stream given or that device's current one."""
 
-    def _bind(self, what, tensors, *args):
+    def _bind(self, what, tensors, head, tail):
         dev = tensors[0].device
         for t in tensors:
             if t.device != dev:
                 raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-        self._what, self._keep, self._args, self._device = what, tensors, args, dev
+        # a CUDA tensor's device always has an index; CPU tensors reach the ABI only in its argument checks
+        self._what, self._keep, self._head, self._tail = what, tensors, head, tail
+        self._index = dev.index if dev.type == "cuda" else None
         self._fn = getattr(load_library(), what)
 
     def _launch(self, stream):
-        # a CUDA tensor's device always has an index; CPU tensors reach the ABI only in its argument checks
-        index = self._device.index if self._device.type == "cuda" else None
+        index = self._index
         if stream is None:
-            stream = torch.cuda.current_stream(index) if index is not None else None
+            handle = _current_stream(index) if index is not None else 0
         elif index is not None and stream.device.index != index:
-            raise ValueError(f"{self._what}: a stream of {stream.device} for tensors on {self._device}")
-        handle = ctypes.c_void_p(stream.cuda_stream if stream is not None else 0)
+            raise ValueError(f"{self._what}: a stream of {stream.device} for tensors on cuda:{index}")
+        else:
+            handle = stream.cuda_stream
         if index is None or index == torch.cuda.current_device():
-            st = self._fn(*self._args[0], handle, *self._args[1])
+            st = self._fn(*self._head, handle, *self._tail)
         else:
             with torch.cuda.device(index):
-                st = self._fn(*self._args[0], handle, *self._args[1])
+                st = self._fn(*self._head, handle, *self._tail)
         if st != OK:
             raise AcefaError(st, self._what)
+
+
+def _current_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same number without building a Stream object (1.2 us of a call)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
 def _int32(t, n, what):

@@ -111,15 +111,13 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(const __grid_consta
         top = fmaxf(top, s_max[w]);
     }
     const float d  = odd ? NAN : max_nan(__fdiv_rn(top, 127.0f), d_old);
+    const float inv = quant_inv(d);
     int8_t     *qb = side.q + (int64_t) lo * side.nb1 + h * side.nb2 + s * side.nb3;
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
         const int r = r0 + p * kRows;
         if (lo + r >= a && lo + r < hi) {
-            const uint32_t w = (uint32_t) (quant_rne(x[p].x, d) & 0xFF) | (uint32_t) (quant_rne(x[p].y, d) & 0xFF) << 8 |
-                               (uint32_t) (quant_rne(x[p].z, d) & 0xFF) << 16 |
-                               (uint32_t) (quant_rne(x[p].w, d) & 0xFF) << 24;
-            *reinterpret_cast<uint32_t *>(qb + (int64_t) r * side.nb1 + e0) = w;
+            *reinterpret_cast<uint32_t *>(qb + (int64_t) r * side.nb1 + e0) = quant4(x[p], d, inv);
         }
     }
     if (a > lo && d > d_old) {  // the rows that stay move to the new scale

@@ -3,9 +3,10 @@
 //
 // Selection.  A weight becomes a 32-bit key that orders like it; the keep-th
 // largest key is found by a radix descent (11 + 11 + 10 bits, one histogram
-// each, counts only, so atomics change nothing), and a scan in row order
-// writes the rows above it and the first of those equal to it.  One CTA per
-// (head, set); the weights are a few hundred KB that stay in L2.
+// each, counts only, so the atomics' order changes nothing; it ends early where
+// a whole bin stays), and a scan in row order writes the rows above it and
+// the first of those equal to it.  One CTA per (head, set), the keys in shared
+// memory: bound by the latency of its passes.
 // Move.  One CTA per 64 destination rows of (head, set) of K or V: it reads the
 // rows' source blocks' scales, takes the largest, and copies the rows, rounding
 // those of another scale once more.  Every source row and destination byte is
@@ -16,8 +17,10 @@
 namespace acefa {
 namespace {
 
-constexpr int kSelThreads = 1024;
-constexpr int kBins       = 2048;
+constexpr int kSelThreads  = 1024;
+constexpr int kSelWarps    = kSelThreads / 32;
+constexpr int kBins        = 2048;
+constexpr int kSelMaxKeys  = 49152;  // keys held in shared memory; more are read again from L2
 constexpr int kMoveThreads = 256;
 
 // Orders like the weight: larger weight, larger key; -0 as 0, NaN below all.
@@ -29,11 +32,14 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// One CTA per (head, set).  KEPT: the keys of [0, len) stay in shared memory.
+template <bool KEPT>
 __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_constant__ Kv8EvictParams P) {
+    extern __shared__ uint32_t s_key[];
     __shared__ int      hist[kBins];
-    __shared__ int      s_warp[2][kSelThreads / 32];
+    __shared__ int      s_eq[kSelWarps], s_sure[kSelWarps];
     __shared__ uint32_t s_prefix;
-    __shared__ int      s_need;
+    __shared__ int      s_need, s_done;
     const int    h = blockIdx.x, b = blockIdx.y;
     const int    tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int    len  = clamp_len(__ldg(P.len + b), P.c.n_max);
@@ -59,17 +65,35 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         }
         return;
     }
+    auto key_of = [&](int x) { return KEPT ? s_key[x] : order_key(__ldg(w + x)); };
     // candidates: rows [lo, hi); the others stay.  len > keep >= n_first + n_recent.
-    const int lo = P.n_first, hi = len - P.n_recent;
+    const int  lo = P.n_first, hi = len - P.n_recent;
+    const bool none = P.keep == P.n_first + P.n_recent;  // no candidate stays
+    if (KEPT) {
+        for (int x = tid; x < len; x += 4 * kSelThreads) {  // four loads on their way
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = x + e * kSelThreads < len ? __ldg(w + x + e * kSelThreads) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (x + e * kSelThreads < len) {
+                    s_key[x + e * kSelThreads] = order_key(v[e]);
+                }
+            }
+        }
+    }
     if (tid == 0) {
         s_prefix = 0u;
         s_need   = P.keep - P.n_first - P.n_recent;  // of the candidates
+        s_done   = 0;
     }
     // ---- the need-th largest key, and how many of those equal to it are kept
     const int shifts[3] = {21, 10, 0};
     uint32_t  mask      = 0u;  // bits of the key settled so far
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
+    for (int pass = 0; pass < 3 && !none; ++pass) {
         const int shift = shifts[pass], bins = pass == 2 ? 1024 : 2048;
         for (int x = tid; x < kBins; x += kSelThreads) {
             hist[x] = 0;
@@ -77,17 +101,10 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         __syncthreads();
         const uint32_t prefix = s_prefix;
         const int      need   = s_need;
-        if (need == 0) {
-            break;  // uniform
-        }
-        for (int x0 = lo + warp * 32; x0 < hi; x0 += kSelThreads) {
-            const int      x   = x0 + lane;
-            const uint32_t key = x < hi ? order_key(__ldg(w + x)) : 0u;
-            const bool     on  = x < hi && (key & mask) == prefix;
-            const int      bin = on ? (int) ((key >> shift) & (uint32_t) (bins - 1)) : -1;
-            const unsigned eq  = __match_any_sync(0xffffffffu, bin);  // many weights share a bin (zeros)
-            if (on && lane == __ffs(eq) - 1) {
-                atomicAdd(&hist[bin], __popc(eq));
+        for (int x = lo + tid; x < hi; x += kSelThreads) {
+            const uint32_t key = key_of(x);
+            if ((key & mask) == prefix) {
+                atomicAdd(&hist[(key >> shift) & (uint32_t) (bins - 1)], 1);
             }
         }
         __syncthreads();
@@ -101,73 +118,87 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
             incl += lane >= off ? v : 0;
         }
         if (lane == 31) {
-            s_warp[0][warp] = incl;
+            s_eq[warp] = incl;
         }
         __syncthreads();
-        int before = 0;
-        for (int k = 0; k < warp; ++k) {
-            before += s_warp[0][k];
-        }
+        const int before = (int) __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0);
         const int above1 = before + incl - c1 - c0;  // keys in bins above b0 + 1
         const int above0 = above1 + c1;
-        if (above1 < need && need <= above1 + c1) {
-            s_prefix = prefix | (uint32_t) (b0 + 1) << shift;
-            s_need   = need - above1;
-        } else if (above0 < need && need <= above0 + c0) {
-            s_prefix = prefix | (uint32_t) b0 << shift;
-            s_need   = need - above0;
+        const bool in1 = above1 < need && need <= above1 + c1, in0 = above0 < need && need <= above0 + c0;
+        if (in1 || in0) {
+            const uint32_t bin  = (uint32_t) (in1 ? b0 + 1 : b0);
+            const int      left = need - (in1 ? above1 : above0);
+            if (left == (in1 ? c1 : c0)) {
+                // the whole bin stays: everything above the key before its first
+                s_done   = 1;
+                s_prefix = prefix | bin << shift;
+                s_need   = 0;
+            } else {
+                s_prefix = prefix | bin << shift;
+                s_need   = left;
+            }
         }
         mask |= (uint32_t) (bins - 1) << shift;
         __syncthreads();
-    }
-    const uint32_t top  = s_prefix;
-    const int      need = s_need;                              // rows equal to `top` that stay, 0: none at all
-    const bool     none = P.keep == P.n_first + P.n_recent;    // no candidate stays
-    // ---- rows in order: each thread owns a contiguous run
-    const int per = (len + kSelThreads - 1) / kSelThreads;
-    const int r0 = min(len, tid * per), r1 = min(len, r0 + per);
-    int       n_eq = 0, n_sure = 0;
-    for (int x = r0; x < r1; ++x) {
-        if (x < lo || x >= hi) {
-            ++n_sure;
-        } else if (!none) {
-            const uint32_t key = order_key(__ldg(w + x));
-            n_eq += key == top;
-            n_sure += key > top;
+        if (s_done) {
+            break;  // uniform
         }
     }
-    int i_eq = n_eq, i_sure = n_sure;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, i_eq, off), v = __shfl_up_sync(0xffffffffu, i_sure, off);
-        i_eq += lane >= off ? u : 0;
-        i_sure += lane >= off ? v : 0;
+    if (none) {
+        __syncthreads();
     }
-    if (lane == 31) {
-        s_warp[0][warp] = i_eq;
-        s_warp[1][warp] = i_sure;
+    // a candidate stays with a key above `top`, or as one of the first `need` equal
+    // to it.  (A bin that starts at key 0 and stays whole keeps every candidate:
+    // len > keep rules that out, so top - 1 does not wrap.)
+    const uint32_t top  = s_done ? s_prefix - 1u : s_prefix;
+    const int      need = s_need;
+    // ---- rows in order: each warp owns a contiguous run, 32 rows at a time
+    const int per = (len + kSelThreads - 1) / kSelThreads * 32;
+    const int r0 = min(len, warp * per), r1 = min(len, r0 + per);
+    auto look = [&](int x, bool &sure, bool &eq) {
+        sure = eq = false;
+        if (x < r1) {
+            if (x < lo || x >= hi) {
+                sure = true;
+            } else if (!none) {
+                const uint32_t key = key_of(x);
+                sure               = key > top;
+                eq                 = !s_done && key == top;
+            }
+        }
+    };
+    int n_eq = 0, n_sure = 0;
+    for (int x = r0; x < r1; x += 32) {
+        bool sure, eq;
+        look(x + lane, sure, eq);
+        n_sure += __popc(__ballot_sync(0xffffffffu, sure));
+        n_eq += __popc(__ballot_sync(0xffffffffu, eq));
+    }
+    __syncthreads();  // s_eq is free
+    if (lane == 0) {
+        s_eq[warp]   = n_eq;
+        s_sure[warp] = n_sure;
     }
     __syncthreads();
-    for (int k = 0; k < warp; ++k) {
-        i_eq += s_warp[0][k];
-        i_sure += s_warp[1][k];
-    }
-    int eq = i_eq - n_eq;                            // equal rows before this run
-    int at = i_sure - n_sure + min(eq, none ? 0 : need);  // kept rows before it
-    for (int x = r0; x < r1; ++x) {
-        bool stay = x < lo || x >= hi;
-        if (!stay && !none) {
-            const uint32_t key = order_key(__ldg(w + x));
-            stay               = key > top || (key == top && eq < need);
-            eq += key == top;
-        }
+    int eq_before = (int) __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0);  // before this run
+    int at = (int) __reduce_add_sync(0xffffffffu, lane < warp ? s_sure[lane] : 0) + min(eq_before, need);
+    const unsigned below = (1u << lane) - 1u;
+    for (int x0 = r0; x0 < r1; x0 += 32) {
+        const int x = x0 + lane;
+        bool      sure, eq;
+        look(x, sure, eq);
+        const unsigned m_eq = __ballot_sync(0xffffffffu, eq);
+        const bool     stay = sure || (eq && eq_before + __popc(m_eq & below) < need);
+        const unsigned m    = __ballot_sync(0xffffffffu, stay);
         if (stay) {
-            out[at] = x;
+            const int to = at + __popc(m & below);
+            out[to]      = x;
             if (wo) {
-                wo[at] = w[x];
+                wo[to] = w[x];
             }
-            ++at;
         }
+        eq_before += __popc(m_eq);
+        at += __popc(m);
     }
 }
 
@@ -237,7 +268,23 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const __grid_con
 }  // namespace
 
 cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s) {
-    kv8_select_kernel<<<dim3((unsigned) p.c.Hkv, (unsigned) p.c.B), kSelThreads, 0, s>>>(p);
+    const dim3 sel((unsigned) p.c.Hkv, (unsigned) p.c.B);
+    if (p.c.n_max <= kSelMaxKeys) {
+        static thread_local int configured = -1;
+        int                     dev        = 0;
+        cudaGetDevice(&dev);
+        if (configured != dev) {
+            const cudaError_t e = cudaFuncSetAttribute(kv8_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       kSelMaxKeys * (int) sizeof(uint32_t));
+            if (e != cudaSuccess) {
+                return e;
+            }
+            configured = dev;
+        }
+        kv8_select_kernel<true><<<sel, kSelThreads, (size_t) p.c.n_max * sizeof(uint32_t), s>>>(p);
+    } else {
+        kv8_select_kernel<false><<<sel, kSelThreads, 0, s>>>(p);
+    }
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
         return e;

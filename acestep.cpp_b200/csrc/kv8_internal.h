@@ -126,7 +126,7 @@ __device__ __forceinline__ float max_nan(float a, float b) { return a != a || b 
 // exact, clamped to 127.  Rounding is monotonic, so rounding the F32 quotient
 // t can only differ where t landed on a half-integer h; there the sign of
 // x - h * d (one FMA: h * d is exact inside it) says on which side of h the
-// true quotient lies.  d > 0 and finite; the result is 0 for d == 0.
+// true quotient lies.  d > 0 and finite; the result is 0 for d == 0 and NaN.
 __device__ __forceinline__ int quant_rne(float x, float d) {
     const float t = __fdiv_rn(x, d);
     float       q = rintf(t);
@@ -141,26 +141,64 @@ __device__ __forceinline__ int quant_rne(float x, float d) {
 }
 
 // q * d_old / d_new rounded once to the nearest integer, ties to even, for
-// |q| <= 127 and d_old <= d_new, with ratio = d_old / d_new in F32.  The F32
-// product is off by at most 127 * 2^-23 < 2^-15; within that of a half-integer
-// the quotient is formed in F64, where q * d_old is exact and the division
+// |q| <= 127 and d_old <= d_new: q * d_old is exact in F64 and the division
 // rounds correctly (a tie is then a tie, and nothing else is within 2^-40 of one).
-__device__ __forceinline__ int requant_rne(int q, float d_old, float d_new, float ratio) {
-    const float t = (float) q * ratio;
-    const float r = rintf(t);
-    if (fabsf(fabsf(t - r) - 0.5f) <= 3.0517578125e-5f) {
-        return (int) rint(__ddiv_rn((double) q * (double) d_old, (double) d_new));
-    }
-    return __float2int_rn(r);
+__device__ __forceinline__ int requant_rne(int q, float d_old, float d_new) {
+    return d_new > 0.0f ? (int) rint(__ddiv_rn((double) q * (double) d_old, (double) d_new)) : 0;
 }
 
-// Four int8 values of a 32-bit word moved from scale d_old to d_new.
-__device__ __forceinline__ uint32_t requant4(uint32_t w, float d_old, float d_new, float ratio) {
-    uint32_t o = 0;
+// Adding 1.5 * 2^23 rounds an F32 number below 2^22 to an integer (ties to even)
+// that stands in the low bits of the sum.
+constexpr float kRoundMagic = 12582912.0f;
+// How near a half-integer v * f, taken for the true quotient, may not be: with
+// f in error by 2^-23 (a rounded reciprocal or ratio) and |v * f| <= 127 the
+// quotient is within 2^-15 of it, and beyond that distance both round alike.
+constexpr float kNearTie = 0.5f - 3.0517578125e-5f;
+
+// The low bytes of four rounded sums.
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040u),
+                       __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040u), 0x5410u);
+}
+
+// Four values of a block of scale d; inv = 1 / d rounded, or 0 where the quick
+// way does not hold (d = 0, subnormal or not a number).
+__device__ __forceinline__ uint32_t quant4(float4 x, float d, float inv) {
+    const float  v[4] = {x.x, x.y, x.z, x.w};
+    float        y[4], off = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int q = (int) (int8_t) (w >> (8 * e));
-        o |= (uint32_t) (requant_rne(q, d_old, d_new, ratio) & 0xFF) << (8 * e);
+        y[e] = fmaf(v[e], inv, kRoundMagic);
+        off  = fmaxf(off, fabsf(fmaf(v[e], inv, kRoundMagic - y[e])));
+    }
+    if (off < kNearTie && inv != 0.0f) {
+        return low_bytes(y[0], y[1], y[2], y[3]);
+    }
+    return (uint32_t) (quant_rne(x.x, d) & 0xFF) | (uint32_t) (quant_rne(x.y, d) & 0xFF) << 8 |
+           (uint32_t) (quant_rne(x.z, d) & 0xFF) << 16 | (uint32_t) (quant_rne(x.w, d) & 0xFF) << 24;
+}
+// 1 / d for quant4
+__device__ __forceinline__ float quant_inv(float d) { return d >= 1.1754944e-36f && d <= 1.0e36f ? __frcp_rn(d) : 0.0f; }
+
+// Four int8 values of a 32-bit word moved from scale d_old to d_new, ratio =
+// d_old / d_new rounded.
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float d_old, float d_new, float ratio) {
+    const uint32_t b = w ^ 0x80808080u;  // int8 + 128
+    float          y[4], off = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        // 2^23 + byte, exactly
+        const float q = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7650u + (uint32_t) e)) - 8388736.0f;
+        y[e]          = fmaf(q, ratio, kRoundMagic);
+        off           = fmaxf(off, fabsf(fmaf(q, ratio, kRoundMagic - y[e])));
+    }
+    if (off < kNearTie) {
+        return low_bytes(y[0], y[1], y[2], y[3]);
+    }
+    uint32_t o = 0;
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+        o |= (uint32_t) (requant_rne((int) (int8_t) (w >> (8 * e)), d_old, d_new) & 0xFF) << (8 * e);
     }
     return o;
 }
