@@ -195,6 +195,7 @@ int plan_attn(const acefa_tensor *q, const acefa_kv8_cache *cache, const acefa_t
         return rc;
     }
     p.n_cta           = (int) std::min<int64_t>(tiles, (int64_t) ctx.sm_count * kv8_attn_ctas_per_sm());
+    p.cluster         = kv8_attn_cluster(p, units, ctx.sm_count);
     p.dev_err         = ctx.dev_err;
     p.wait_limit_ns   = ctx.wait_limit_ns;
     p.score_stride    = std::min(R, (p.rows + 1) & ~1);
@@ -348,7 +349,7 @@ ACEFA_API int acefa_kv8_attn(const acefa_tensor *q, const acefa_kv8_cache *cache
     p.scores     = weight ? reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.part_bytes) : nullptr;
     const int launched = launch_kv8_attn(p, static_cast<cudaStream_t>(stream));
     if (launched == ACEFA_OK) {
-        note_launches(2, 4);
+        note_launches(p.cluster ? 1 : 2, 4);
     }
     return launched;
 }

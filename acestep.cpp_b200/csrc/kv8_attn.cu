@@ -26,6 +26,9 @@
 // (dims are summed over in any order, and V's dims are only named at the end),
 // and the boxes' layouts (K in rows of 64 B, V swizzled) such that reading the
 // pieces meets no bank conflicts.
+// Few short units (CL): a thread-block cluster takes each unit instead, its CTAs
+// an equal share of its tiles, and the partial results meet in distributed shared
+// memory -- one launch, no table of the sets, no partials in HBM.
 // Products run transposed (keys or dims are the MMA's M, the rows its N = 8):
 // S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
 // operand layout by four movmatrix.  The running maximum moves only when a
@@ -183,6 +186,17 @@ __device__ __forceinline__ void store1(char *p, int type, int e, float x) {
     }
 }
 
+// Four finished dims of a row (L = its sum; 0: it saw nothing).
+__device__ __forceinline__ void store_row4(const Kv8AttnParams &P, int row, int hk, int b, int d4, float4 o, float L) {
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    char *p = P.dst.data + (int64_t) (hk * P.G + row % P.G) * P.dst.nb1 + (int64_t) (row / P.G) * P.dst.nb2 +
+              (int64_t) b * P.dst.nb3;
+    store1(p, P.dst.type, 4 * d4, o.x * inv);
+    store1(p, P.dst.type, 4 * d4 + 1, o.y * inv);
+    store1(p, P.dst.type, 4 * d4 + 2, o.z * inv);
+    store1(p, P.dst.type, 4 * d4 + 3, o.w * inv);
+}
+
 // base[b] = places of one unit of each set before b, b = 0 .. B: its 64-key tiles
 // and, ahead of them, kUnitCost (none without tiles); lens[b] = length.  All
 // threads; ends with a barrier.
@@ -230,7 +244,7 @@ __device__ __forceinline__ void mma_start(float (&d)[4], const uint32_t (&a)[4],
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-template <int HD, int NT, int MODE>
+template <int HD, int NT, int MODE, bool CL>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     kv8_attn_kernel(const __grid_constant__ Kv8AttnParams P, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap) {
@@ -265,18 +279,52 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         prefetch_tensormap(&vmap);
     }
     pdl_wait_primary();
-    tile_table(s_base, s_len, P.len, P.c.B, P.c.n_max);
-    const int T = s_base[P.c.B] * HU;
-    const int C = min((int) gridDim.x, T);
-    pdl_launch_dependents();
-    if ((int) blockIdx.x >= C) {
-        return;
+    Walk at;
+    int  x1;  // behind the last place of this CTA's run
+    if constexpr (CL) {
+        const int unit = (int) blockIdx.x / P.cluster, rank = (int) blockIdx.x - unit * P.cluster;
+        at.b   = unit / HU;
+        at.ub  = unit - at.b * HU;
+        at.len = clamp_len(__ldg(P.len + at.b), P.c.n_max);
+        at.nt  = (at.len + kKv8Block - 1) / kKv8Block;
+        at.t = at.at = run_start(at.nt, P.cluster, rank);
+        x1           = run_start(at.nt, P.cluster, rank + 1);
+        __syncthreads();
+    } else {
+        tile_table(s_base, s_len, P.len, P.c.B, P.c.n_max);
+        const int T = s_base[P.c.B] * HU;
+        const int C = min((int) gridDim.x, T);
+        pdl_launch_dependents();
+        if ((int) blockIdx.x >= C) {
+            return;
+        }
+        const int x0 = run_start(T, C, blockIdx.x);
+        x1           = run_start(T, C, blockIdx.x + 1);
+        // the set whose places hold x0: base[b] * HU <= x0 < base[b + 1] * HU, by 32nds
+        int lo = 0, n = P.c.B;
+        while (n > 1) {
+            const int step = (n + 31) >> 5, i = lo + lane * step;
+            const int below = __popc(__ballot_sync(0xffffffffu, lane * step < n && s_base[i] * HU <= x0));
+            n  = min(step, n - (below - 1) * step);
+            lo += (below - 1) * step;
+        }
+        at.b          = lo;
+        const int per = s_base[lo + 1] - s_base[lo];
+        at.nt         = per - kUnitCost;
+        at.len        = s_len[lo];
+        const int off = x0 - s_base[lo] * HU;
+        at.ub         = (int) ((unsigned) off / (unsigned) per);
+        const int r   = off - at.ub * per;
+        at.t          = max(r - kUnitCost, 0);
+        at.at         = x0 + max(kUnitCost - r, 0);
+        if (at.at >= x1) {
+            return;  // no tile in this run
+        }
     }
-    const int x0 = run_start(T, C, blockIdx.x), x1 = run_start(T, C, blockIdx.x + 1);
 
     auto advance = [&](Walk &w) {  // true: a new unit
         ++w.at;
-        if (++w.t < w.nt) {
+        if (++w.t < w.nt || CL) {
             return false;
         }
         w.t = 0;
@@ -295,29 +343,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         return true;
     };
     auto kv_head = [&](const Walk &w) { return P.n_rb == 1 ? w.ub : w.ub / P.n_rb; };
-    Walk at;
-    {
-        // the set whose places hold x0: base[b] * HU <= x0 < base[b + 1] * HU, by 32nds
-        int lo = 0, n = P.c.B;
-        while (n > 1) {
-            const int step = (n + 31) >> 5, i = lo + lane * step;
-            const int below = __popc(__ballot_sync(0xffffffffu, lane * step < n && s_base[i] * HU <= x0));
-            n  = min(step, n - (below - 1) * step);
-            lo += (below - 1) * step;
-        }
-        at.b          = lo;
-        const int per = s_base[lo + 1] - s_base[lo];
-        at.nt         = per - kUnitCost;
-        at.len        = s_len[lo];
-        const int off = x0 - s_base[lo] * HU;
-        at.ub         = (int) ((unsigned) off / (unsigned) per);
-        const int r   = off - at.ub * per;
-        at.t          = max(r - kUnitCost, 0);
-        at.at         = x0 + max(kUnitCost - r, 0);
-    }
-    if (at.at >= x1) {
-        return;  // no tile in this run
-    }
     // This thread's row of Q of a unit (kPacked: rows 4 .. 7 are the low halves of 0 .. 3), or nullptr
     auto q_row = [&](const Walk &w, int nt, int &row) -> const char * {
         const int hk = kv_head(w);
@@ -370,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             }
             if (!advance(at)) {
                 ++ksp, ++vsp;
-            } else if (at.b < P.c.B) {
+            } else if (!CL && at.b < P.c.B) {
                 aim();
                 if (at.at < x1) {  // the next unit's rows of Q, on their way to L1
 #pragma unroll
@@ -465,6 +490,64 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
     };
 
+    // The four warps' results of a unit as one: n_row rows of HD at dst, R maxima
+    // and R sums behind R rows.
+    auto merge = [&](float *dst, int n_row) {
+        named_bar_sync(1, 32 * kWarps);  // the previous merge has been read
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[nt][e];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int row = nt * 8 + 2 * c + e;
+                if (g == 0) {
+                    s_ml[(warp * R + row) * 2]     = m[nt][e];
+                    s_ml[(warp * R + row) * 2 + 1] = sum;
+                }
+                // element e of the accumulators is dim 2t of row 2c + e, element 2 + e dim 2t + 1
+                float *o = s_o + (warp * R + row) * kOut + g * (HD / 8);
+#pragma unroll
+                for (int t = 0; t < KS; t += 2) {
+                    *reinterpret_cast<float4 *>(o + 2 * t) = make_float4(acc_o[nt][t][e], acc_o[nt][t][2 + e],
+                                                                         acc_o[nt][t + 1][e], acc_o[nt][t + 1][2 + e]);
+                }
+            }
+        }
+        named_bar_sync(1, 32 * kWarps);
+        if (MODE == kPacked) {
+            n_row = min(n_row, 4);
+        }
+        for (int x = threadIdx.x; x < n_row * (HD / 4); x += 32 * kWarps) {
+            const int row = x / (HD / 4), d4 = x % (HD / 4);
+            float     mw[kWarps], M = kNoMax;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                mw[w] = s_ml[(w * R + row) * 2];
+                M     = fmaxf(M, mw[w]);
+            }
+            float  L = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = exp2f(mw[w] - M);
+                float4      v = *reinterpret_cast<const float4 *>(s_o + (w * R + row) * kOut + 4 * d4);
+                if constexpr (MODE == kPacked) {
+                    const float4 u = *reinterpret_cast<const float4 *>(s_o + (w * R + row + 4) * kOut + 4 * d4);
+                    v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+                }
+                L += s_ml[(w * R + row) * 2 + 1] * f;
+                o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+            }
+            *reinterpret_cast<float4 *>(dst + row * HD + 4 * d4) = o;
+            if (d4 == 0) {
+                dst[R * HD + row]     = M;
+                dst[R * HD + R + row] = L;
+            }
+        }
+    };
     start_rows();
     // K row g of this warp's chunk, 16-B piece c; V rows 2c .. of it, HD / 8 dims of g
     const uint32_t k_at = smem_u32(smem) + (uint32_t) ((warp * kChunk + g) * 64 + 16 * c);
@@ -660,64 +743,89 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (P.scores) {
             sp += kKv8Block * P.score_stride;
         }
-        if (next || at.at >= x1) {
-            named_bar_sync(1, 32 * kWarps);  // the previous merge has been read
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float sum = l[nt][e];
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                    const int row = nt * 8 + 2 * c + e;
-                    if (g == 0) {
-                        s_ml[(warp * R + row) * 2]     = m[nt][e];
-                        s_ml[(warp * R + row) * 2 + 1] = sum;
-                    }
-                    // element e of the accumulators is dim 2t of row 2c + e, element 2 + e dim 2t + 1
-                    float *o = s_o + (warp * R + row) * kOut + g * (HD / 8);
-#pragma unroll
-                    for (int t = 0; t < KS; t += 2) {
-                        *reinterpret_cast<float4 *>(o + 2 * t) = make_float4(
-                            acc_o[nt][t][e], acc_o[nt][t][2 + e], acc_o[nt][t + 1][e], acc_o[nt][t + 1][2 + e]);
-                    }
-                }
-            }
-            named_bar_sync(1, 32 * kWarps);
-            const int n_row = min(R, P.rows - rb * R);
-            float    *slot  = P.part + (int64_t) (blockIdx.x + unit) * (R * (HD + 2));
-            for (int x = threadIdx.x; x < n_row * (HD / 4); x += 32 * kWarps) {
-                const int row = x / (HD / 4), d4 = x % (HD / 4);
-                float     mw[kWarps], M = kNoMax;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    mw[w] = s_ml[(w * R + row) * 2];
-                    M     = fmaxf(M, mw[w]);
-                }
-                float       L  = 0.0f;
-                float4      o  = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float  f = exp2f(mw[w] - M);
-                    float4       v = *reinterpret_cast<const float4 *>(s_o + (w * R + row) * kOut + 4 * d4);
-                    if constexpr (MODE == kPacked) {
-                        const float4 u = *reinterpret_cast<const float4 *>(s_o + (w * R + row + 4) * kOut + 4 * d4);
-                        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-                    }
-                    L += s_ml[(w * R + row) * 2 + 1] * f;
-                    o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
-                }
-                *reinterpret_cast<float4 *>(slot + row * HD + 4 * d4) = o;
-                if (d4 == 0) {
-                    slot[R * HD + row]     = M;
-                    slot[R * HD + R + row] = L;
-                }
-            }
+        if (!CL && (next || at.at >= x1)) {
+            merge(P.part + (int64_t) (blockIdx.x + unit) * (R * (HD + 2)), min(R, P.rows - rb * R));
             if (at.at < x1) {
                 start_rows();
             }
         }
+    }
+    if constexpr (CL) {
+        // Every CTA's result to its own shared memory (the ring is empty: each of
+        // its tiles has been awaited), then the cluster's CTAs finish a share of
+        // the unit's values each from all of them.
+        float *fin = reinterpret_cast<float *>(smem);
+        merge(fin, R);
+        cluster_arrive();
+        cluster_wait();
+        const int      rank = (int) cluster_ctarank(), hk = kv_head(at), rb = at.ub - hk * P.n_rb;
+        const int      n_row = min(R, P.rows - rb * R);
+        const uint32_t f_at  = smem_u32(fin);
+        for (int x = (int) threadIdx.x * P.cluster + rank; x < n_row * (HD / 4); x += 32 * kWarps * P.cluster) {
+            const int r = x / (HD / 4), d4 = x % (HD / 4);
+            float     m8[8], l8[8], M = kNoMax, L = 0.0f;
+            float4    o8[8], o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {  // every value asked for at once
+                if (k < P.cluster) {
+                    const uint32_t p = mapa_shared(f_at, (uint32_t) k);
+                    m8[k] = ld_cluster_f32(p + 4u * (R * HD + r));
+                    l8[k] = ld_cluster_f32(p + 4u * (R * HD + R + r));
+                    o8[k] = ld_cluster_f32x4(p + 4u * (r * HD + 4 * d4));
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                M = k < P.cluster ? fmaxf(M, m8[k]) : M;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (k < P.cluster) {
+                    const float f = exp2f(m8[k] - M);
+                    L = fmaf(l8[k], f, L);
+                    o.x = fmaf(o8[k].x, f, o.x), o.y = fmaf(o8[k].y, f, o.y);
+                    o.z = fmaf(o8[k].z, f, o.z), o.w = fmaf(o8[k].w, f, o.w);
+                }
+            }
+            store_row4(P, rb * R + r, hk, at.b, d4, o, L);
+        }
+        if (P.weight) {  // (n_rb == 1) this CTA's own keys
+            float *s_lse = s_ml;  // free: the merge is behind the cluster's barrier
+            for (int r = threadIdx.x; r < n_row; r += 32 * kWarps) {
+                float M = kNoMax, L = 0.0f;
+                for (int k = 0; k < P.cluster; ++k) {
+                    M = fmaxf(M, ld_cluster_f32(mapa_shared(f_at, (uint32_t) k) + 4u * (R * HD + r)));
+                }
+                for (int k = 0; k < P.cluster; ++k) {
+                    const uint32_t q = mapa_shared(f_at, (uint32_t) k) + 4u * (R * HD + r);
+                    L = fmaf(ld_cluster_f32(q + 4u * R), exp2f(ld_cluster_f32(q) - M), L);
+                }
+                s_lse[r] = L == 0.0f ? INFINITY : M + log2f(L);  // an empty row weighs nothing
+            }
+            cluster_arrive_relaxed();  // the peers' memory is read
+            named_bar_sync(1, 32 * kWarps);  // (and orders the scores that the warps of this CTA wrote)
+            const int j0 = run_start(at.nt, P.cluster, rank) * kKv8Block, j1 = min(at.len, x1 * kKv8Block);
+            float    *wp = reinterpret_cast<float *>(P.weight + (int64_t) hk * P.w_nb2 + (int64_t) at.b * P.w_nb3);
+            for (int j = j0 + (int) threadIdx.x; j < j1; j += 32 * kWarps) {
+                const float2 *q = reinterpret_cast<const float2 *>(
+                    P.scores + ((int64_t) (at.b * HU + at.ub) * P.c.n_max + j) * P.score_stride);
+                float sum = 0.0f;
+#pragma unroll
+                for (int r = 0; r < R; r += 2) {
+                    if (r < n_row) {
+                        const float2 v = __ldcg(q + (r >> 1));
+                        sum += fast_exp2(v.x - s_lse[r]);
+                        if (r + 1 < n_row) {
+                            sum += fast_exp2(v.y - s_lse[r + 1]);
+                        }
+                    }
+                }
+                wp[j] += sum;
+            }
+        } else {
+            cluster_arrive_relaxed();
+        }
+        cluster_wait();  // no CTA leaves while a peer reads its memory
     }
 }
 
@@ -817,13 +925,7 @@ __global__ void __launch_bounds__(kSumThreads) kv8_attn_sum_kernel(const __grid_
             __syncthreads();
         }
         if (w == 0) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            char *p = P.dst.data + (int64_t) (hk * P.G + row % P.G) * P.dst.nb1 + (int64_t) (row / P.G) * P.dst.nb2 +
-                      (int64_t) b * P.dst.nb3;
-            store1(p, P.dst.type, 4 * d4, o.x * inv);
-            store1(p, P.dst.type, 4 * d4 + 1, o.y * inv);
-            store1(p, P.dst.type, 4 * d4 + 2, o.z * inv);
-            store1(p, P.dst.type, 4 * d4 + 3, o.w * inv);
+            store_row4(P, row, hk, b, d4, o, L);
         }
         return;
     }
@@ -922,35 +1024,59 @@ bool encode_side(CUtensorMap *map, const Kv8Dev &c, const Kv8Side &side, int inn
                swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, int NT, int MODE>
-cudaError_t launch(const Kv8AttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t s) {
-    const int              smem = attn_smem_bytes<HD, NT>(p.c.B);
+template <int HD, int NT, int MODE, bool CL>
+cudaError_t configure(int *smem, int B) {
+    *smem = attn_smem_bytes<HD, NT>(CL ? 0 : B);
     static thread_local int configured = -1;
     int                     dev        = 0;
     cudaGetDevice(&dev);
     if (configured != dev) {
-        cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<HD, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<HD, NT, MODE, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              attn_smem_bytes<HD, NT>(kKv8MaxSets));
         if (e != cudaSuccess) {
             return e;
         }
         configured = dev;
     }
-    cudaLaunchAttribute attr[1];
+    return cudaSuccess;
+}
+
+template <int HD, int NT, int MODE>
+cudaError_t launch(const Kv8AttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t s) {
+    cudaLaunchAttribute attr[2];
     attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim            = dim3((unsigned) p.n_cta);
-    cfg.blockDim           = dim3(kThreads);
-    cfg.dynamicSmemBytes   = smem;
-    cfg.stream             = s;
-    cfg.attrs              = attr;
-    cfg.numAttrs           = 1;
-    cudaError_t e          = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT, MODE>, p, km, vm);
+    attr[1].id                                         = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x                           = (unsigned) p.cluster;
+    attr[1].val.clusterDim.y                           = 1;
+    attr[1].val.clusterDim.z                           = 1;
+    int                smem = 0;
+    cudaLaunchConfig_t cfg  = {};
+    cfg.blockDim            = dim3(kThreads);
+    cfg.stream              = s;
+    cfg.attrs               = attr;
+    if (p.cluster) {
+        cudaError_t e = configure<HD, NT, MODE, true>(&smem, p.c.B);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        cfg.gridDim          = dim3((unsigned) (p.c.B * p.c.Hkv * p.n_rb * p.cluster));
+        cfg.dynamicSmemBytes = (size_t) smem;
+        cfg.numAttrs         = 2;
+        return cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT, MODE, true>, p, km, vm);
+    }
+    cudaError_t e = configure<HD, NT, MODE, false>(&smem, p.c.B);
     if (e != cudaSuccess) {
         return e;
     }
-    const int n_out      = p.c.B * p.c.Hkv * p.rows;
+    cfg.gridDim          = dim3((unsigned) p.n_cta);
+    cfg.dynamicSmemBytes = (size_t) smem;
+    cfg.numAttrs         = 1;
+    e                    = cudaLaunchKernelEx(&cfg, kv8_attn_kernel<HD, NT, MODE, false>, p, km, vm);
+    if (e != cudaSuccess) {
+        return e;
+    }
+    const int n_out = p.c.B * p.c.Hkv * p.rows;
     // keys of a CTA: enough for about kSumCtas of them in all
     const int64_t all  = (int64_t) p.c.B * p.c.Hkv * p.c.n_max;
     const int     keys = (int) std::max<int64_t>(1, std::min<int64_t>(all / kSumCtas, p.c.n_max) / kSumKeys) * kSumKeys;
@@ -962,6 +1088,20 @@ cudaError_t launch(const Kv8AttnParams &p, const CUtensorMap &km, const CUtensor
 }
 
 }  // namespace
+
+// A cluster per unit (in one wave) or runs of tiles over the whole device and
+// a second launch?  A CTA's tiles either way, and the second launch with its
+// way through HBM as kSecond tiles (0.7 us each; it measured ~3 us).
+int kv8_attn_cluster(const Kv8AttnParams &p, int64_t units, int sm_count) {
+    constexpr int64_t kSecond = 4;
+    const int64_t     nt = (p.c.n_max + kKv8Block - 1) / kKv8Block;
+    const int64_t     c  = std::min<int64_t>({8, nt, (int64_t) kCtasPerSm * sm_count / units});
+    if (c < 1 || (p.weight && p.n_rb > 1)) {
+        return 0;
+    }
+    const int64_t split = (units * (nt + kUnitCost) + p.n_cta - 1) / p.n_cta;
+    return (nt + c - 1) / c <= split + kSecond ? (int) c : 0;
+}
 
 int kv8_attn_ctas_per_sm() { return kCtasPerSm; }
 

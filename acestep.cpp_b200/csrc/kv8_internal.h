@@ -54,6 +54,7 @@ struct Kv8AttnParams {
     int            n_q, G, rows;  // rows = G * n_q per kv head
     int            n_rb;          // row blocks per (set, kv head)
     int            n_cta;         // CTAs of the split kernel
+    int            cluster;       // CTAs of a unit's cluster, or 0: the split kernel and the sum kernel
     float          scale_log2;    // scale * log2(e)
     float         *part;          // partial results, one slot per (CTA, unit) that meet
     float         *scores;        // [unit][n_max][score_stride] log2-unit scores, with weights only
@@ -85,6 +86,7 @@ cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s);
 // fragments of sixteen rows do not fit the registers of two CTAs per SM.
 inline int kv8_unit_rows(int rows, int q_type) { return rows <= 8 || q_type == ACEFA_TYPE_F32 ? 8 : 16; }
 int        kv8_attn_ctas_per_sm();
+int        kv8_attn_cluster(const Kv8AttnParams &p, int64_t units, int sm_count);
 inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows * (D + 2); }
 
 // ------------------------------------------------------------------ device helpers

@@ -201,7 +201,7 @@ def test_attend(D, Hq, H, n_q, lens, n_max, kind, weigh):
     w0 = r.random((len(lens), H, n_max)).astype(np.float32) if weigh else None
     weight = torch.from_numpy(w0).cuda() if weigh else None
     out = acefa.kv8_attn(qd, cache, _i32(lens), weight=weight)
-    assert acefa.last_path() == 4 and acefa.last_launch_count() == 2
+    assert acefa.last_path() == 4 and acefa.last_launch_count() in (1, 2)
     qn = q.float().numpy().astype(np.float64).transpose(0, 2, 1, 3)
     k, v = ref.values(cq[0], cs[0]), ref.values(cq[1], cs[1])
     want, ww = ref.attend(qn, k, v, lens, D ** -0.5)
