@@ -217,12 +217,6 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
     return v;
 }
 
-__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // The largest of a row's 32 scores and mx; with VIS, keys whose bit of v is 0 become -inf.
 template <bool VIS>
 __device__ __forceinline__ float max_chunk(uint32_t (&x)[32], uint32_t v, float mx) {

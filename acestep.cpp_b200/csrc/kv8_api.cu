@@ -255,6 +255,7 @@ ACEFA_API int acefa_kv8_store(const acefa_kv8_cache *cache, const acefa_tensor *
     p.k_new = rows_of(*k_new), p.v_new = rows_of(*v_new);
     p.rows    = rows;
     p.cu      = cu_rows;
+    p.per_set = (int) (rows / p.c.B);
     p.pos     = pos;
     p.dev_err = ctx.dev_err;
     if (launch_kv8_store(p, static_cast<cudaStream_t>(stream)) != cudaSuccess) {

@@ -806,21 +806,38 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             named_bar_sync(1, 32 * kWarps);  // (and orders the scores that the warps of this CTA wrote)
             const int j0 = run_start(at.nt, P.cluster, rank) * kKv8Block, j1 = min(at.len, x1 * kKv8Block);
             float    *wp = reinterpret_cast<float *>(P.weight + (int64_t) hk * P.w_nb2 + (int64_t) at.b * P.w_nb3);
-            for (int j = j0 + (int) threadIdx.x; j < j1; j += 32 * kWarps) {
-                const float2 *q = reinterpret_cast<const float2 *>(
-                    P.scores + ((int64_t) (at.b * HU + at.ub) * P.c.n_max + j) * P.score_stride);
-                float sum = 0.0f;
+            const float2 *sc = reinterpret_cast<const float2 *>(P.scores + (int64_t) (at.b * HU + at.ub) * P.c.n_max * P.score_stride);
+            constexpr int kAtOnce = R == 8 ? 4 : 2;  // keys of a thread on their way together
+            for (int jb = j0 + (int) threadIdx.x; jb < j1; jb += kAtOnce * 32 * kWarps) {
+                float2 v[kAtOnce][R / 2];
+                float  w[kAtOnce], sum[kAtOnce];
 #pragma unroll
-                for (int r = 0; r < R; r += 2) {
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const int j = jb + k * 32 * kWarps;
+                    w[k]        = j < j1 ? wp[j] : 0.0f;
+                    sum[k]      = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < R / 2; ++r) {
+                        v[k][r] = j < j1 && 2 * r < P.score_stride ? __ldcg(sc + (int64_t) j * (P.score_stride >> 1) + r)
+                                                                   : make_float2(-INFINITY, -INFINITY);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
                     if (r < n_row) {
-                        const float2 v = __ldcg(q + (r >> 1));
-                        sum += fast_exp2(v.x - s_lse[r]);
-                        if (r + 1 < n_row) {
-                            sum += fast_exp2(v.y - s_lse[r + 1]);
+#pragma unroll
+                        for (int k = 0; k < kAtOnce; ++k) {
+                            sum[k] += fast_exp2((r & 1 ? v[k][r >> 1].y : v[k][r >> 1].x) - s_lse[r]);
                         }
                     }
                 }
-                wp[j] += sum;
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const int j = jb + k * 32 * kWarps;
+                    if (j < j1) {
+                        wp[j] = w[k] + sum[k];
+                    }
+                }
             }
         } else {
             cluster_arrive_relaxed();

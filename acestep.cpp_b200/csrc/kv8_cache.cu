@@ -18,21 +18,33 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Rows of set s among k_new (first row, count); count 0 for offsets that are none.
-__device__ __forceinline__ void set_rows(const Kv8StoreParams &P, int s, int64_t &first, int64_t &count, int &pos,
-                                         bool &bad) {
-    pos = P.pos[s];
+// Rows of set s among k_new (first row, count), the cache row of the first, and
+// whether they are none (count 0).  All fit in 32 bits.
+struct SetRows {
+    int  first, count, pos;
+    bool bad;
+};
+__device__ __forceinline__ SetRows set_rows(const Kv8StoreParams &P, int s) {
+    SetRows r;
+    r.pos = __ldg(P.pos + s);
     if (P.cu) {
-        first = P.cu[s];
-        count = (int64_t) P.cu[s + 1] - first;
+        r.first         = __ldg(P.cu + s);
+        const int end   = __ldg(P.cu + s + 1);
+        r.bad           = r.first < 0 || end < r.first || end > (int) P.rows;
+        r.count         = r.bad ? 0 : end - r.first;
     } else {
-        count = P.rows / P.c.B;
-        first = count * s;
+        r.count = P.per_set;
+        r.first = r.count * s;
+        r.bad   = false;
     }
-    bad = count < 0 || first < 0 || first + count > P.rows || (count > 0 && (pos < 0 || pos + count > P.c.n_max));
-    if (bad) {
-        count = 0;
+    if (r.count > 0 && (r.pos < 0 || r.pos > P.c.n_max - r.count)) {
+        r.bad   = true;
+        r.count = 0;
     }
+    return r;
+}
+__device__ __forceinline__ int blocks_of(const SetRows &r) {
+    return r.count > 0 ? (r.pos + r.count - 1) / kKv8Block - r.pos / kKv8Block + 1 : 0;
 }
 
 // grid (blocks touched, an upper bound; Hkv; K and V).  A thread holds four
@@ -42,46 +54,32 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(const __grid_consta
     constexpr int kLanes = D / 4;               // threads per row
     constexpr int kRows  = kThreads / kLanes;   // rows per pass
     constexpr int kPass  = kKv8Block / kRows;   // passes over the block
-    __shared__ float s_max[kThreads / 32];
-    auto blocks_of = [&](int s) {
-        int64_t first, count;
-        int     pos;
-        bool    bad;
-        set_rows(P, s, first, count, pos, bad);
-        return count > 0 ? (int) ((pos + count - 1) / kKv8Block - pos / kKv8Block + 1) : 0;
-    };
+    __shared__ uint32_t s_max[kThreads / 32];
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
         for (int s = threadIdx.x; s < P.c.B; s += kThreads) {
-            int64_t first, count;
-            int     pos;
-            bool    bad;
-            set_rows(P, s, first, count, pos, bad);
-            if (bad) {
+            if (set_rows(P, s).bad) {
                 atomicCAS(P.dev_err, 0, DEVERR_APPEND_POS);
             }
         }
     }
     int s, item;
-    if (!find_item(P.c.B, blockIdx.x, blocks_of, s, item)) {
+    if (!find_item(P.c.B, blockIdx.x, [&](int i) { return blocks_of(set_rows(P, i)); }, s, item)) {
         return;
     }
-    int64_t first, count;
-    int     pos;
-    bool    bad;
-    set_rows(P, s, first, count, pos, bad);
+    const SetRows  rows = set_rows(P, s);
+    const int      pos  = rows.pos;
     const int      h    = blockIdx.y;
     const Kv8Rows &src  = blockIdx.z ? P.v_new : P.k_new;
     const Kv8Side &side = blockIdx.z ? P.c.v : P.c.k;
     const int      blk  = pos / kKv8Block + item;
     const int      lo   = blk * kKv8Block;                                        // first row of the block
     const int      a    = max(lo, pos);                                           // first new row
-    const int      hi   = (int) min((int64_t) lo + kKv8Block, pos + count);       // behind the last one
+    const int      hi   = min(lo + kKv8Block, pos + rows.count);                  // behind the last one
     const int      r0   = threadIdx.x / kLanes, e0 = 4 * (threadIdx.x % kLanes);
-    const char    *base = src.data + (first + (a - pos)) * src.nb1 + (int64_t) h * src.nb2;
+    const char    *base = src.data + (rows.first + (a - pos)) * src.nb1 + h * src.nb2;
     const bool     vec  = ((reinterpret_cast<uintptr_t>(base) | (uintptr_t) src.nb1) & (4 * sizeof(T) - 1)) == 0;
     float4         x[kPass];
-    float          top = 0.0f;
-    bool           odd = false;  // a NaN or an infinity among this thread's values
+    uint32_t       top = 0u;  // |x| as bits order like |x|, infinities and NaNs above all
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
         const int r = lo + r0 + p * kRows;
@@ -93,31 +91,27 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(const __grid_consta
     const float d_old = a > lo ? *scale : 0.0f;
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
-        const float m = fmaxf(fmaxf(fabsf(x[p].x), fabsf(x[p].y)), fmaxf(fabsf(x[p].z), fabsf(x[p].w)));
-        odd |= !(fabsf(x[p].x) <= 3.4028235e38f && fabsf(x[p].y) <= 3.4028235e38f && fabsf(x[p].z) <= 3.4028235e38f &&
-                 fabsf(x[p].w) <= 3.4028235e38f);
-        top = fmaxf(top, m);
+        const uint32_t u[4] = {__float_as_uint(x[p].x) & 0x7FFFFFFFu, __float_as_uint(x[p].y) & 0x7FFFFFFFu,
+                               __float_as_uint(x[p].z) & 0x7FFFFFFFu, __float_as_uint(x[p].w) & 0x7FFFFFFFu};
+        top = max(max(top, u[0]), max(u[1], max(u[2], u[3])));
     }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    }
+    top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) {
         s_max[threadIdx.x >> 5] = top;
     }
-    odd = __syncthreads_or(odd);
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-        top = fmaxf(top, s_max[w]);
+        top = max(top, s_max[w]);
     }
-    const float d  = odd ? NAN : max_nan(__fdiv_rn(top, 127.0f), d_old);
+    const float d = top >= 0x7F800000u ? NAN : max_nan(__fdiv_rn(__uint_as_float(top), 127.0f), d_old);
     const float inv = quant_inv(d);
     int8_t     *qb = side.q + (int64_t) lo * side.nb1 + h * side.nb2 + s * side.nb3;
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
         const int r = r0 + p * kRows;
         if (lo + r >= a && lo + r < hi) {
-            *reinterpret_cast<uint32_t *>(qb + (int64_t) r * side.nb1 + e0) = quant4(x[p], d, inv);
+            *reinterpret_cast<uint32_t *>(qb + r * side.nb1 + e0) = quant4(x[p], d, inv);
         }
     }
     if (a > lo && d > d_old) {  // the rows that stay move to the new scale

@@ -7,7 +7,7 @@
 // a whole bin stays), and a scan in row order writes the rows above it and
 // the first of those equal to it.  One CTA per (head, set), the keys in shared
 // memory: bound by the latency of its passes.
-// Move.  One CTA per 64 destination rows of (head, set) of K or V: it reads the
+// Move.  One CTA per 64 destination rows of K and V of a (head, set): it reads the
 // rows' source blocks' scales, takes the largest, and copies the rows, rounding
 // those of another scale once more.  Every source row and destination byte is
 // touched once: HBM-bound, 2 bytes per value kept.
@@ -202,66 +202,83 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     }
 }
 
-// grid (64-row blocks of `keep`, Hkv, 2 * B)
+// grid (64-row blocks of `keep`, Hkv, B); K and V of the block
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const __grid_constant__ Kv8EvictParams P) {
-    constexpr int kLanes = D / 4;
+    constexpr int kLanes = D / 16;  // 16 values each
     constexpr int kRows  = kMoveThreads / kLanes;
     constexpr int kPass  = kKv8Block / kRows;
-    __shared__ int   s_row[kKv8Block];
-    __shared__ float s_d[kKv8Block];
-    __shared__ float s_top[2];
-    const int      blk = blockIdx.x, h = blockIdx.y, b = blockIdx.z >> 1;
-    const Kv8Side &src = (blockIdx.z & 1) ? P.c.v : P.c.k;
-    const Kv8Side &dst = (blockIdx.z & 1) ? P.out.v : P.out.k;
+    __shared__ int    s_row[kKv8Block];
+    __shared__ float2 s_d[kKv8Block];  // scales of the row in K and V
+    __shared__ float2 s_ratio[kKv8Block];  // of those scales to the block's new ones
+    __shared__ float2 s_top[2];
+    const int      blk = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int      lo  = blk * kKv8Block;
     const int      n   = min(kKv8Block, P.keep - lo);  // rows of the block that are written
     const int32_t *kept = reinterpret_cast<const int32_t *>(P.kept + h * P.k_nb2 + b * P.k_nb3);
+    auto           scales = [&](const Kv8Side &s) {
+        return reinterpret_cast<float *>(reinterpret_cast<char *>(s.scale) + h * s.s_nb2 + b * s.s_nb3);
+    };
     pdl_wait_primary();
     if (threadIdx.x < kKv8Block) {
         const int x = threadIdx.x;
         // written by the selection; a value that is no row moves nothing
-        const int   row = x < n ? __ldcg(kept + lo + x) : -1;
-        const bool  on  = row >= 0 && row < P.c.n_max;
-        const float d   = on ? *(reinterpret_cast<const float *>(reinterpret_cast<const char *>(src.scale) +
-                                                               h * src.s_nb2 + b * src.s_nb3) +
-                               row / kKv8Block)
-                             : 0.0f;
+        const int  row = x < n ? __ldcg(kept + lo + x) : -1;
+        const bool on  = row >= 0 && row < P.c.n_max;
+        float2     d   = on ? make_float2(scales(P.c.k)[row / kKv8Block], scales(P.c.v)[row / kKv8Block])
+                            : make_float2(0.0f, 0.0f);
         s_row[x] = on ? row : -1;
         s_d[x]   = d;
-        float top = d;
 #pragma unroll
         for (int off = 16; off; off >>= 1) {
-            top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
+            d.x = max_nan(d.x, __shfl_xor_sync(0xffffffffu, d.x, off));
+            d.y = max_nan(d.y, __shfl_xor_sync(0xffffffffu, d.y, off));
         }
         if ((x & 31) == 0) {
-            s_top[x >> 5] = top;
+            s_top[x >> 5] = d;
         }
     }
     __syncthreads();
-    const float    d_new = max_nan(s_top[0], s_top[1]);
-    const int      r0 = threadIdx.x / kLanes, e0 = 4 * (threadIdx.x % kLanes);
-    const int8_t  *sp = src.q + h * src.nb2 + b * src.nb3;
-    int8_t        *dp = dst.q + (int64_t) lo * dst.nb1 + h * dst.nb2 + b * dst.nb3;
-    uint32_t       w[kPass];
+    const float   d_new[2] = {max_nan(s_top[0].x, s_top[1].x), max_nan(s_top[0].y, s_top[1].y)};
+    const int     r0 = threadIdx.x / kLanes, e0 = 16 * (threadIdx.x % kLanes);
+    const int8_t *sp[2] = {P.c.k.q + h * P.c.k.nb2 + b * P.c.k.nb3 + e0, P.c.v.q + h * P.c.v.nb2 + b * P.c.v.nb3 + e0};
+    uint4         w[2][kPass];
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
         const int row = s_row[r0 + p * kRows];
-        w[p]          = row >= 0 ? __ldcs(reinterpret_cast<const uint32_t *>(sp + (int64_t) row * src.nb1 + e0)) : 0u;
+        w[0][p] = w[1][p] = make_uint4(0u, 0u, 0u, 0u);
+        if (row >= 0) {
+            w[0][p] = __ldcs(reinterpret_cast<const uint4 *>(sp[0] + row * P.c.k.nb1));
+            w[1][p] = __ldcs(reinterpret_cast<const uint4 *>(sp[1] + row * P.c.v.nb1));
+        }
     }
+    if (threadIdx.x < kKv8Block) {
+        const float2 d       = s_d[threadIdx.x];
+        s_ratio[threadIdx.x] = make_float2(__fdiv_rn(d.x, d_new[0]), __fdiv_rn(d.y, d_new[1]));
+    }
+    __syncthreads();
 #pragma unroll
-    for (int p = 0; p < kPass; ++p) {
-        const int   r = r0 + p * kRows;
-        const float d = s_d[r];
-        if (d != d_new && w[p]) {
-            w[p] = requant4(w[p], d, d_new, __fdiv_rn(d, d_new));
-        }
-        if (r < n) {
-            *reinterpret_cast<uint32_t *>(dp + (int64_t) r * dst.nb1 + e0) = w[p];
+    for (int i = 0; i < 2; ++i) {
+        const Kv8Side &dst = i ? P.out.v : P.out.k;
+        int8_t        *dp  = dst.q + (int64_t) lo * dst.nb1 + h * dst.nb2 + b * dst.nb3 + e0;
+#pragma unroll
+        for (int p = 0; p < kPass; ++p) {
+            const int   r = r0 + p * kRows;
+            const float d = i ? s_d[r].y : s_d[r].x;
+            if (d != d_new[i]) {
+                const float ratio = i ? s_ratio[r].y : s_ratio[r].x;
+                w[i][p].x = requant4(w[i][p].x, d, d_new[i], ratio);
+                w[i][p].y = requant4(w[i][p].y, d, d_new[i], ratio);
+                w[i][p].z = requant4(w[i][p].z, d, d_new[i], ratio);
+                w[i][p].w = requant4(w[i][p].w, d, d_new[i], ratio);
+            }
+            if (r < n) {
+                *reinterpret_cast<uint4 *>(dp + r * dst.nb1) = w[i][p];
+            }
         }
     }
-    if (threadIdx.x == 0) {
-        *(reinterpret_cast<float *>(reinterpret_cast<char *>(dst.scale) + h * dst.s_nb2 + b * dst.s_nb3) + blk) = d_new;
+    if (threadIdx.x < 2) {
+        scales(threadIdx.x ? P.out.v : P.out.k)[blk] = d_new[threadIdx.x];
     }
 }
 
@@ -294,7 +311,7 @@ cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim            = dim3((unsigned) ((p.keep + kKv8Block - 1) / kKv8Block), (unsigned) p.c.Hkv,
-                                  (unsigned) (2 * p.c.B));
+                                  (unsigned) p.c.B);
     cfg.blockDim           = dim3(kMoveThreads);
     cfg.stream             = s;
     cfg.attrs              = attr;

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include "fa_internal.h"
+#include "ptx.cuh"
 
 namespace acefa {
 
@@ -34,8 +35,9 @@ struct Kv8Rows {
 struct Kv8StoreParams {
     Kv8Dev         c;
     Kv8Rows        k_new, v_new;  // nb3 unused
-    int64_t        rows;          // rows of k_new
-    const int32_t *cu;            // or nullptr: rows / B each
+    int64_t        rows;          // rows of k_new (at most 2^30)
+    const int32_t *cu;            // or nullptr: per_set rows each
+    int            per_set;
     const int32_t *pos;
     int           *dev_err;
 };
@@ -93,28 +95,28 @@ inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows 
 #ifdef __CUDACC__
 
 // Finds item x among the items of n segments, count(i) of segment i in their
-// order.  The whole warp calls it with the same arguments and gets the same
-// answer: the segment and the item's number in it, or false behind the last.
+// order (fewer than 2^31 in all).  The whole warp calls it with the same arguments
+// and gets the same answer: the segment and the item's number in it, or false
+// behind the last.
 template <class F>
-__device__ __forceinline__ bool find_item(int n, int64_t x, F count, int &seg, int &item) {
+__device__ __forceinline__ bool find_item(int n, int x, F count, int &seg, int &item) {
     const int lane = threadIdx.x & 31;
-    int64_t   acc  = 0;
     for (int base = 0; base < n; base += 32) {
         const int mine = base + lane < n ? count(base + lane) : 0;
-        int64_t   incl = mine;
+        int       incl = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, incl, off);
+            const int v = __shfl_up_sync(0xffffffffu, incl, off);
             incl += lane >= off ? v : 0;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, x < acc + incl);
+        const unsigned hit = __ballot_sync(0xffffffffu, x < incl);
         if (hit) {
             const int l = __ffs(hit) - 1;
             seg         = base + l;
-            item        = (int) (x - acc - __shfl_sync(0xffffffffu, incl - mine, l));
+            item        = x - __shfl_sync(0xffffffffu, incl - mine, l);
             return true;
         }
-        acc += __shfl_sync(0xffffffffu, incl, 31);
+        x -= __shfl_sync(0xffffffffu, incl, 31);
     }
     return false;
 }
@@ -166,12 +168,16 @@ __device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d
 // Four values of a block of scale d; inv = 1 / d rounded, or 0 where the quick
 // way does not hold (d = 0, subnormal or not a number).
 __device__ __forceinline__ uint32_t quant4(float4 x, float d, float inv) {
-    const float  v[4] = {x.x, x.y, x.z, x.w};
-    float        y[4], off = 0.0f;
+    const uint64_t v[2] = {f32x2(x.x, x.y), f32x2(x.z, x.w)}, i2 = f32x2(inv, inv);
+    const uint64_t magic = f32x2(kRoundMagic, kRoundMagic), minus = f32x2(-1.0f, -1.0f);
+    float          y[4], off = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        y[e] = fmaf(v[e], inv, kRoundMagic);
-        off  = fmaxf(off, fabsf(fmaf(v[e], inv, kRoundMagic - y[e])));
+    for (int e = 0; e < 2; ++e) {  // two values per instruction
+        const uint64_t s = ffma2(v[e], i2, magic);
+        float          d0, d1;
+        f32x2_split(ffma2(v[e], i2, ffma2(s, minus, magic)), d0, d1);
+        f32x2_split(s, y[2 * e], y[2 * e + 1]);
+        off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
     }
     if (off < kNearTie && inv != 0.0f) {
         return low_bytes(y[0], y[1], y[2], y[3]);
@@ -186,13 +192,20 @@ __device__ __forceinline__ float quant_inv(float d) { return d >= 1.1754944e-36f
 // d_old / d_new rounded.
 __device__ __forceinline__ uint32_t requant4(uint32_t w, float d_old, float d_new, float ratio) {
     const uint32_t b = w ^ 0x80808080u;  // int8 + 128
+    const uint64_t bias = f32x2(-8388736.0f, -8388736.0f), r2 = f32x2(ratio, ratio);
+    const uint64_t magic = f32x2(kRoundMagic, kRoundMagic), minus = f32x2(-1.0f, -1.0f);
     float          y[4], off = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 4; e += 2) {  // two values per instruction
         // 2^23 + byte, exactly
-        const float q = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7650u + (uint32_t) e)) - 8388736.0f;
-        y[e]          = fmaf(q, ratio, kRoundMagic);
-        off           = fmaxf(off, fabsf(fmaf(q, ratio, kRoundMagic - y[e])));
+        const uint64_t q = fadd2(f32x2(__uint_as_float(__byte_perm(b, 0x4B000000u, 0x7650u + (uint32_t) e)),
+                                       __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7651u + (uint32_t) e))),
+                                 bias);
+        const uint64_t s = ffma2(q, r2, magic);
+        float          d0, d1;
+        f32x2_split(ffma2(q, r2, ffma2(s, minus, magic)), d0, d1);
+        f32x2_split(s, y[e], y[e + 1]);
+        off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
     }
     if (off < kNearTie) {
         return low_bytes(y[0], y[1], y[2], y[3]);
