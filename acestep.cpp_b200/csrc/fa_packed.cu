@@ -145,11 +145,10 @@ __device__ __forceinline__ void find_unit(const PackedParams &P, int u, const Se
         }
         pair         = lo;
         const int  k = x - (int) __reduce_add_sync(0xffffffffu, max(np - lo - 1, 0));
-        unsigned   m = __ballot_sync(0xffffffffu, np > lo);
-        for (int i = 0; i < k; ++i) {
-            m &= m - 1;
-        }
-        const int src = __ffs(m) - 1;
+        // the k-th sequence (from 0) that reaches the level
+        const unsigned m    = __ballot_sync(0xffffffffu, np > lo);
+        const int      lane = threadIdx.x & 31;
+        const int      src  = __ffs(__ballot_sync(0xffffffffu, np > lo && __popc(m & ((1u << lane) - 1u)) == k)) - 1;
         q.q0  = __shfl_sync(0xffffffffu, mine.q0, src);
         q.n_q = __shfl_sync(0xffffffffu, mine.n_q, src);
         q.k0  = __shfl_sync(0xffffffffu, mine.k0, src);
@@ -280,8 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&full[i], 2);  // one arrival for V, one for K
             mbar_init(&empty[i], 1);
             mbar_init(&s_ready[i], 1);
-            mbar_init(&p_ready[i], 128);
-            mbar_init(&p_half[i], 128);
+            mbar_init(&p_ready[i], 4);  // the tile's warps
+            mbar_init(&p_half[i], 4);
             mbar_init(&o_done[i], 1);
         }
         mbar_init(q_full, 1);
@@ -718,7 +717,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 exp_chunk<BF16>(x1, tS + 16, c, m_use, ls);
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&p_half[i]);  // the product with V starts on these 64 keys
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&p_half[i]);  // the product with V starts on these 64 keys
+                }
                 exp_chunk<BF16>(x2, tS + 32, c, m_use, ls);
                 exp_chunk<BF16>(x3, tS + 48, c, m_use, ls);
                 float l0, l1;
@@ -726,7 +728,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l_run += l0 + l1;
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&p_ready[i]);
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&p_ready[i]);
+                }
             }
             // ---- O / l leaves: 128-B pieces of the warp's 32 rows through its
             // staging slab (16-B chunk x of row y at x ^ (y & 7): no bank conflicts
