@@ -510,7 +510,10 @@ def cfg_logit_combine(cond: torch.Tensor, uncond: torch.Tensor | None, eos_idx: 
 
 class _Call:
     """An entry with its operands: keeps the tensors alive, runs on their device,
-    on the stream given or that device's current one."""
+    on the stream given or that device's current one.  What a handle allocates
+    (an output, a workspace) belongs to the stream that was current when it was
+    made; another stream waits for that one first, as for any tensor, and calls that
+    may overlap need a handle each."""
 
     def _bind(self, what, tensors, head, tail):
         dev = tensors[0].device

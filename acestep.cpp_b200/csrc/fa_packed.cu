@@ -30,7 +30,6 @@
 #include <cstring>
 
 #include "fa_internal.h"
-#include "kv8_internal.h"  // find_item
 #include "ptx.cuh"
 
 namespace acefa {
@@ -121,8 +120,10 @@ static_assert(sizeof(Unit) == 64, "a slot of the ring");
 // The u-th unit (t.more = 0 behind the last); the whole warp gets the same answer.
 // Up to 32 sequences (`mine`: lane s holds sequence s) are numbered by length:
 // level L holds the pair L of every sequence that has one, the highest first.
-// More are numbered one after another, each from its last pair.
-__device__ __forceinline__ void find_unit(const PackedParams &P, int u, const Seq &mine, Unit &t) {
+// More are numbered one after another, each from its last pair; the search goes
+// on from the sequence `from`, before which `before` pairs lie (0, 0 at first:
+// a CTA asks for ever higher units, so it passes over the sequences once).
+__device__ __forceinline__ void find_unit(const PackedParams &P, int u, const Seq &mine, int &from, int &before, Unit &t) {
     const int x = divide(u, P.Hkv, P.inv_hkv);
     int       pair;
     Seq       q;
@@ -154,12 +155,29 @@ __device__ __forceinline__ void find_unit(const PackedParams &P, int u, const Se
         q.k0  = __shfl_sync(0xffffffffu, mine.k0, src);
         q.n_k = __shfl_sync(0xffffffffu, mine.n_k, src);
     } else {
-        int s, item;
-        if (!find_item(P.n_seq, x, [&](int i) { return n_pairs(P, seq_of(P, i).n_q); }, s, item)) {
-            return;
+        const int lane = threadIdx.x & 31;
+        int       np, incl;
+        unsigned  hit;
+        for (;; from += 32) {
+            if (from >= P.n_seq) {
+                return;
+            }
+            np   = from + lane < P.n_seq ? n_pairs(P, seq_of(P, from + lane).n_q) : 0;
+            incl = np;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, off);
+                incl += lane >= off ? v : 0;
+            }
+            hit = __ballot_sync(0xffffffffu, x < before + incl);
+            if (hit) {
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
         }
-        q    = seq_of(P, s);
-        pair = n_pairs(P, q.n_q) - 1 - item;
+        const int l = __ffs(hit) - 1;
+        q    = seq_of(P, from + l);
+        pair = __shfl_sync(0xffffffffu, before + incl, l) - 1 - x;
     }
     t.more = 1;
     t.q0 = q.q0, t.n_q = q.n_q, t.k0 = q.k0, t.n_k = q.n_k;
@@ -329,17 +347,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (P.n_seq <= 32 && lane < P.n_seq) {
                 mine = seq_of(P, lane);
             }
-            if (blockIdx.x == 0) {
-                for (int s = lane; s < P.n_seq; s += 32) {
-                    if (seq_of(P, s).bad) {
-                        atomicCAS(P.dev_err, 0, DEVERR_APPEND_POS);
-                    }
-                }
-            }
             Unit t;
-            bool ok = true;
+            bool ok   = true;
+            int  from = 0, before = 0;
             for (int k = 0; ok; ++k) {
-                find_unit(P, deal(k), mine, t);
+                find_unit(P, deal(k), mine, from, before, t);
                 ok = __all_sync(0xffffffffu, wait(&u_empty[k % kUnitRing], (uint32_t) (k / kUnitRing) ^ 1u,
                                                   DEVERR_TIMEOUT_EMPTY));
                 if (ok && lane == 0) {
@@ -347,6 +359,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&u_full[k % kUnitRing]);
                 }
                 ok = ok && t.more != 0;
+            }
+            for (int s = (int) blockIdx.x * 32 + lane; s < P.n_seq; s += (int) gridDim.x * 32) {
+                if (seq_of(P, s).bad) {
+                    atomicCAS(P.dev_err, 0, DEVERR_APPEND_POS);
+                }
             }
         } else if (warp == 0) {
             // ============================ TMA producer ============================

@@ -358,7 +358,8 @@ typedef struct acefa_kv8_cache {
  * new length are left as they are.  A set whose rows are no rows of the
  * cache or of k_new (a negative pos, an end past n_max, offsets that
  * decrease or leave [0, rows]) is left unwritten and raises device error 5
- * (acefa_device_error()).  k_new and v_new must not overlap the cache.
+ * (acefa_device_error()); where offsets decrease, other sets may be left
+ * unfinished.  k_new and v_new must not overlap the cache.
  */
 ACEFA_API int acefa_kv8_store(const acefa_kv8_cache *cache, const acefa_tensor *k_new, const acefa_tensor *v_new,
                               const int32_t *cu_rows, const int32_t *pos, void *stream);

@@ -191,6 +191,13 @@ def _attend_tol(q, k, v, scale, D, kind):
     (128, 1, 1, 17, [40], 64, "f32"),
     (64, 32, 8, 1, [2500, 30, 1200, 64, 1, 640, 0, 128], 2560, "bf16"),
     (128, 2, 2, 1, list(range(0, 140, 2)), 140, "f32"),
+    # long caches of few units, and more units than CTAs: two launches
+    (128, 4, 1, 1, [4000], 4096, "f32"),
+    (64, 16, 2, 1, [3000, 4100], 4200, "bf16"),
+    (128, 3, 1, 3, [5000], 5000, "f32"),
+    (128, 16, 1, 1, [4500], 5000, "f16"),
+    (64, 6, 1, 2, [6001], 6001, "f32"),
+    (64, 2, 1, 1, [(37 * i) % 131 for i in range(400)], 130, "f32"),
 ])
 @pytest.mark.parametrize("weigh", [False, True])
 def test_attend(D, Hq, H, n_q, lens, n_max, kind, weigh):
@@ -297,6 +304,49 @@ def test_attend_captured_with_new_lengths():
         assert np.all(np.abs(weight.cpu().numpy() - total) <= total * (2 * wtol + 2.0 ** -20))
 
 
+def test_calls_side_by_side():
+    """Two calls with handles of their own on two streams, on one cache."""
+    r = _rng(3, 3, 3)
+    cache, *_ = _cache(r, 3, 2, 3000, 64)
+    lens = _i32([3000, 1, 1700])
+    calls = [acefa.Kv8Attn(torch.from_numpy(r.standard_normal((3, 4, n, 64)).astype(np.float32)).cuda(), cache, lens)
+             for n in (1, 3)]
+    want = [c().clone() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for c, s in zip(calls, streams):
+            c(s)
+    torch.cuda.synchronize()
+    for c, w in zip(calls, want):
+        assert torch.equal(c.out, w)
+
+
+def test_offsets_past_32_bits():
+    """The second of two sets lies more than 4 GB behind the first: stored, read, attended, evicted."""
+    r = _rng(32, 33)
+    D, n, gap = 128, 200, (1 << 32) + 4096
+    big = [torch.empty(gap + n * D, dtype=torch.int8, device="cuda") for _ in range(2)]
+    k, v = (t.as_strided((2, 1, n, D), (gap, n * D, D, 1)) for t in big)
+    scales = [torch.empty((2, 1, 4), device="cuda") for _ in range(2)]
+    cache = acefa.Kv8Cache(k, v, *scales)
+    x = [_rows(r, 1, 2 * n, D) for _ in range(2)]
+    acefa.kv8_store(cache, torch.from_numpy(x[0]).cuda(), torch.from_numpy(x[1]).cuda(), _i32([0, 0]))
+    cq, cs = zip(*[ref.store(np.zeros((2, 1, n, D), np.int8), np.zeros((2, 1, 4), np.float32), y, [0, 0], [0, n, 2 * n])
+                   for y in x])
+    kk, vv = acefa.kv8_load(cache, _i32([n, n]))
+    assert np.array_equal(kk.cpu().numpy(), ref.values(cq[0], cs[0], np.float32))
+    assert np.array_equal(vv.cpu().numpy(), ref.values(cq[1], cs[1], np.float32))
+    q = r.standard_normal((2, 2, 1, D)).astype(np.float32)
+    out = acefa.kv8_attn(torch.from_numpy(q).cuda(), cache, _i32([n, n - 7])).cpu().numpy()
+    kn, vn = ref.values(cq[0], cs[0]), ref.values(cq[1], cs[1])
+    want, _ = ref.attend(q.astype(np.float64), kn, vn, [n, n - 7], D ** -0.5)
+    tol, _, half = _attend_tol(q, kn, vn, D ** -0.5, D, "f32")
+    assert np.abs(out - want).max() <= tol + half * np.abs(want).max()
+    _check_evict(cache, list(cq), list(cs), r.random((2, 1, n)).astype(np.float32), [n, n - 7], 90, 2, 5)
+
+
 # ------------------------------------------------------------------ eviction
 def _check_evict(cache, cq, cs, weight, lens, keep, n_first, n_recent):
     out, kept, lo, wo = acefa.kv8_evict(cache, torch.from_numpy(weight).cuda(), _i32(lens), keep, n_first, n_recent)
@@ -321,6 +371,17 @@ def test_evict(D, H, n, lens, keep, first, recent):
     w = np.exp(2 * r.standard_normal((len(lens), H, n))).astype(np.float32)
     w[r.random(w.shape) < 0.3] = 0.0
     _check_evict(cache, cq, cs, w, lens, keep, first, recent)
+
+
+def test_evict_more_rows_than_shared_memory_holds():
+    r = _rng(50, 50)
+    n, keep = 60000, 333
+    q = [r.integers(-127, 128, (1, 1, n, 64), dtype=np.int8) for _ in range(2)]
+    s = [r.random((1, 1, -(-n // 64))).astype(np.float32) + 0.1 for _ in range(2)]
+    cache = acefa.Kv8Cache(*(torch.from_numpy(t).cuda() for t in (*q, *s)))
+    w = np.exp(2 * r.standard_normal((1, 1, n))).astype(np.float32)
+    w[0, 0, ::3] = w[0, 0].max()  # more equal ones than places
+    _check_evict(cache, q, s, w, [n - 11], keep, 3, 4)
 
 
 def test_evict_ties_and_odd_weights():

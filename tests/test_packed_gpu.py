@@ -119,6 +119,16 @@ def test_a_sequence_never_reads_its_neighbour():
     assert torch.equal(a[:100], b[:100]) and torch.equal(a[150:], b[150:]) and torch.isnan(b[100:150]).all()
 
 
+@pytest.mark.parametrize("mask", [0, 1])
+def test_thousands_of_short_sequences(mask):
+    lens = [(7 * i) % 5 for i in range(3000)] + [200, 0, 131]
+    D, total = 64, sum(lens)
+    q, k, v = _inputs([30, mask], 2, 1, total, total, D, "f16")
+    cu = _cu(lens)
+    out = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu.tolist()), mask=mask)
+    _check(out, q, k, v, cu, cu, mask, 0, D ** -0.5, "f16", "f16")
+
+
 def test_large_and_small_scales():
     D, lens = 128, [200, 129]
     q, k, v = _inputs([7, 7], 2, 1, 329, 329, D, "f16")
