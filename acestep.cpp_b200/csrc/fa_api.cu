@@ -923,6 +923,6 @@ ACEFA_API const char *acefa_status_string(int status) {
 
 ACEFA_API int acefa_last_launch_count(void) { return t_last_launches; }
 ACEFA_API int acefa_last_path(void) { return t_last_path; }
-ACEFA_API int acefa_version(void) { return 100; }
+ACEFA_API int acefa_version(void) { return 200; }
 
 }  // extern "C"

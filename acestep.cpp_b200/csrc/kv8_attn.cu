@@ -29,6 +29,10 @@
 // Few short units (CL): a thread-block cluster takes each unit instead, its CTAs
 // an equal share of its tiles, and the partial results meet in distributed shared
 // memory -- one launch, no table of the sets, no partials in HBM.
+// Measured (B200): 16 sets of up to 8192 rows, 8 KV heads, D = 128, BF16 rows:
+// 46 us, 5.4 TB/s in all and 6.9 TB/s between the first and the last tile (bound by
+// HBM and, closely, by the four warps' instructions: 0.70 us per tile and
+// CTA); 2 sets of 700 rows: 6 us, bound by the latencies of launch, Q and merge.
 // Products run transposed (keys or dims are the MMA's M, the rows its N = 8):
 // S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
 // operand layout by four movmatrix.  The running maximum moves only when a

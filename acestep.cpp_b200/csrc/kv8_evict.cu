@@ -10,7 +10,8 @@
 // Move.  One CTA per 64 destination rows of K and V of a (head, set): it reads the
 // rows' source blocks' scales, takes the largest, and copies the rows, rounding
 // those of another scale once more.  Every source row and destination byte is
-// touched once: HBM-bound, 2 bytes per value kept.
+// touched once, 2 bytes per value kept.  Measured (B200), 8 sets x 8 heads, 8192
+// rows to 4000: selection 13 us, move 25 us (5.2 TB/s); 2 sets, 2048 to 1024: 7 and 6 us.
 #include "kv8_internal.h"
 #include "ptx.cuh"
 
