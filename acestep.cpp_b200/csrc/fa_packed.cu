@@ -36,6 +36,7 @@
 #include <cstring>
 
 #include "fa_internal.h"
+#include "kv8_internal.h"  // find_item
 #include "ptx.cuh"
 
 namespace acefa {
@@ -876,6 +877,253 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows: the same attention on mma.sync, 16 tokens of one query head per CTA.
+// No tensor memory, no staging and no pipeline to fill: each of the four warps takes
+// 16 keys of every 64 and loads exactly its fragments' 16-B pieces of rows to
+// registers, products run transposed (S^T = K Q^T, O^T = V^T P^T; P changes layout by
+// movmatrix), and the warps' results meet once in shared memory.  Bound by latency:
+// 3-5 us up to 128 rows of 16 heads against 8.5 us of the kernel above.
+constexpr int   kSmallRows = 16;
+constexpr int   kSmallWarps = 4;
+constexpr float kNoMax = -1.7e38f;  // below every score, finite
+
+struct SmallParams {
+    PackedParams p;
+    const char  *q, *k, *v;
+    int64_t      q_nb1, q_nb2, k_nb1, k_nb2, v_nb1, v_nb2;  // row, head
+};
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid_constant__ SmallParams S) {
+    constexpr int NT = kSmallRows / 8, KS = HD / 16, kOut = HD + 4;
+    __shared__ float s_o[kSmallWarps][kSmallRows][kOut];
+    __shared__ float s_m[kSmallWarps][kSmallRows], s_l[kSmallWarps][kSmallRows];
+    const PackedParams &P = S.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int h = blockIdx.y, hk = divide(h, P.G, P.inv_g);
+    if (h == 0 && warp == 0) {
+        for (int s = (int) blockIdx.x * 32 + lane; s < P.n_seq; s += (int) gridDim.x * 32) {
+            if (seq_of(P, s).bad) {
+                atomicCAS(P.dev_err, 0, DEVERR_APPEND_POS);
+            }
+        }
+    }
+    int si, item;
+    if (!find_item(P.n_seq, blockIdx.x, [&](int i) { return (seq_of(P, i).n_q + kSmallRows - 1) / kSmallRows; }, si, item)) {
+        return;
+    }
+    const Seq q    = seq_of(P, si);
+    const int row0 = item * kSmallRows, n_row = min(kSmallRows, q.n_q - row0);
+    // ---- Q^T: row nt * 8 + g; the dims of word pairs as K's pieces have them
+    uint32_t qf[NT][KS][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int   r = nt * 8 + g;
+        const char *p = S.q + (int64_t) (q.q0 + row0 + r) * S.q_nb1 + h * S.q_nb2 + 16 * c;
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) {
+            const uint4 w = r < n_row ? __ldg(reinterpret_cast<const uint4 *>(p + 64 * e)) : make_uint4(0u, 0u, 0u, 0u);
+            qf[nt][2 * e][0] = w.x, qf[nt][2 * e][1] = w.y, qf[nt][2 * e + 1][0] = w.z, qf[nt][2 * e + 1][1] = w.w;
+        }
+    }
+    int   lo[NT][2], hi[NT][2];  // what rows nt * 8 + 2c, + 1 see
+    float m[NT][2], l[NT][2], acc[NT][KS][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = nt * 8 + 2 * c + e;
+            lo[nt][e] = hi[nt][e] = 0;
+            if (r < n_row) {
+                visible(P, q, row0 + r, lo[nt][e], hi[nt][e]);
+            }
+            m[nt][e] = kNoMax;
+            l[nt][e] = 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+            acc[nt][t][0] = acc[nt][t][1] = acc[nt][t][2] = acc[nt][t][3] = 0.0f;
+        }
+    }
+    int j_lo, j_hi, unused;
+    visible(P, q, row0, j_lo, unused);
+    visible(P, q, row0 + n_row - 1, unused, j_hi);
+    const char *kb = S.k + (int64_t) q.k0 * S.k_nb1 + hk * S.k_nb2 + 16 * c;
+    const char *vb = S.v + (int64_t) q.k0 * S.v_nb1 + hk * S.v_nb2 + (HD / 4) * g;
+#pragma unroll 1
+    for (int j0 = (j_lo & ~15) + 16 * warp; j0 < j_hi; j0 += 16 * kSmallWarps) {
+        // K rows g and g + 8, pieces c; V rows 2c, 2c + 1, 2c + 8, 2c + 9, HD / 8 dims
+        // of g.  Rows behind the sequence's end are zeros.
+        uint4 kw[2][HD / 32], vw[4][HD / 64];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int j = j0 + g + 8 * r;
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) {
+                kw[r][e] = j < q.n_k ? __ldg(reinterpret_cast<const uint4 *>(kb + j * S.k_nb1 + 64 * e))
+                                     : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int j = j0 + 2 * c + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+            for (int e = 0; e < HD / 64; ++e) {
+                vw[r][e] = j < q.n_k ? __ldg(reinterpret_cast<const uint4 *>(vb + j * S.v_nb1 + 16 * e))
+                                     : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+        // ---- S^T: (key g, rows 2c 2c+1), (key g + 8, the same rows); even and odd k-steps apart
+        float s[NT][4], s2[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[nt][e] = s2[nt][e] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) {
+            const uint32_t a[4] = {kw[0][e].x, kw[1][e].x, kw[0][e].y, kw[1][e].y};
+            const uint32_t b[4] = {kw[0][e].z, kw[1][e].z, kw[0][e].w, kw[1][e].w};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma_16816<BF16>(s[nt], a, qf[nt][2 * e][0], qf[nt][2 * e][1]);
+                mma_16816<BF16>(s2[nt], b, qf[nt][2 * e + 1][0], qf[nt][2 * e + 1][1]);
+            }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int   j = j0 + g + 8 * (e >> 1);
+                const float v = (s[nt][e] + s2[nt][e]) * P.scale_log2;
+                s[nt][e]      = j >= lo[nt][e & 1] && j < hi[nt][e & 1] ? v : -INFINITY;
+                grow |= s[nt][e] > m[nt][e & 1] + kSlack;
+            }
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(s[nt][e], s[nt][2 + e]);
+                    top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float mn = fmaxf(m[nt][e], top), f = fast_exp2(m[nt][e] - mn);
+                    m[nt][e] = mn;
+                    l[nt][e] *= f;
+#pragma unroll
+                    for (int t = 0; t < KS; ++t) {
+                        acc[nt][t][e] *= f;
+                        acc[nt][t][2 + e] *= f;
+                    }
+                }
+            }
+        }
+        uint32_t ph[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = fast_exp2(s[nt][e] - m[nt][e & 1]);
+                l[nt][e & 1] += p[e];
+            }
+            ph[nt][0] = movmatrix_trans(pack2<BF16>(p[0], p[1]));
+            ph[nt][1] = movmatrix_trans(pack2<BF16>(p[2], p[3]));
+        }
+        // ---- O^T: m-tile t is dims g * HD / 8 + 2t (row g) and + 2t + 1 (row g + 8)
+        uint32_t vr[4][HD / 16];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int e = 0; e < HD / 64; ++e) {
+                vr[r][4 * e] = vw[r][e].x, vr[r][4 * e + 1] = vw[r][e].y;
+                vr[r][4 * e + 2] = vw[r][e].z, vr[r][4 * e + 3] = vw[r][e].w;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < KS; ++t) {
+            const uint32_t a[4] = {__byte_perm(vr[0][t], vr[1][t], 0x5410u), __byte_perm(vr[0][t], vr[1][t], 0x7632u),
+                                   __byte_perm(vr[2][t], vr[3][t], 0x5410u), __byte_perm(vr[2][t], vr[3][t], 0x7632u)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                mma_16816<BF16>(acc[nt][t], a, ph[nt][0], ph[nt][1]);
+            }
+        }
+    }
+    // ---- the warps' results together
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[nt][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            const int row = nt * 8 + 2 * c + e;
+            if (g == 0) {
+                s_m[warp][row] = m[nt][e];
+                s_l[warp][row] = sum;
+            }
+#pragma unroll
+            for (int t = 0; t < KS; t += 2) {
+                *reinterpret_cast<float4 *>(&s_o[warp][row][g * (HD / 8) + 2 * t]) =
+                    make_float4(acc[nt][t][e], acc[nt][t][2 + e], acc[nt][t + 1][e], acc[nt][t + 1][2 + e]);
+            }
+        }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < n_row * (HD / 4); x += 32 * kSmallWarps) {
+        const int r = x / (HD / 4), d = x % (HD / 4) * 4;
+        float     M = kNoMax, L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kSmallWarps; ++w) {
+            M = fmaxf(M, s_m[w][r]);
+        }
+#pragma unroll
+        for (int w = 0; w < kSmallWarps; ++w) {
+            const float  f = exp2f(s_m[w][r] - M);
+            const float4 v = *reinterpret_cast<const float4 *>(&s_o[w][r][d]);
+            L = fmaf(s_l[w][r], f, L);
+            o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[2] = fmaf(v.z, f, o[2]), o[3] = fmaf(v.w, f, o[3]);
+        }
+        const float inv = 1.0f / L;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            o[e] = L == 0.0f ? 0.0f : o[e] * inv;  // a row that saw nothing is 0
+        }
+        char *p = P.dst + h * P.d_nb1 + (int64_t) (q.q0 + row0 + r) * P.d_nb2;
+        if (P.dst_type == ACEFA_TYPE_F32) {
+            float *f = reinterpret_cast<float *>(p) + d;
+            if (P.vec) {
+                *reinterpret_cast<float4 *>(f) = make_float4(o[0], o[1], o[2], o[3]);
+            } else {
+                f[0] = o[0], f[1] = o[1], f[2] = o[2], f[3] = o[3];
+            }
+        } else {
+            const uint32_t w[2] = {pack2<BF16>(o[0], o[1]), pack2<BF16>(o[2], o[3])};
+            uint16_t      *f    = reinterpret_cast<uint16_t *>(p) + d;
+            if (P.vec) {
+                *reinterpret_cast<uint2 *>(f) = make_uint2(w[0], w[1]);
+            } else {
+                f[0] = (uint16_t) w[0], f[1] = (uint16_t) (w[0] >> 16);
+                f[2] = (uint16_t) w[1], f[3] = (uint16_t) (w[1] >> 16);
+            }
+        }
+    }
+}
+
 template <int HD, bool BF16>
 cudaError_t launch(const PackedParams &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int n_cta,
                    cudaStream_t s) {
@@ -910,6 +1158,16 @@ int encode_rows(CUtensorMap *map, const acefa_tensor *t) {
                       3, t->data, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return rc == CUDA_SUCCESS ? ACEFA_OK : ACEFA_ERR_LAYOUT;
+}
+
+// The few-rows kernel?  It reads the keys again for every 16 rows of a head, so
+// its time grows with rows x heads x D; the tensor-memory kernel starts slowly.
+// Measured, few-rows against the other (us): one sequence of 16 / 128 / 256 rows,
+// 16 heads, D = 128: 3.8 : 8.4, 4.9 : 8.5, 7.8 : 10.5; 512 rows, 8 / 16 heads: 11.4 : 14.0,
+// 17.9 : 14.1; 256 rows, 32 heads: 12.9 : 10.8; 8 sequences of 578 rows in all, 8 / 16
+// heads: 9.2 : 10.7, 13.4 : 11.0; 512 rows, 16 heads, D = 64: 11.1 : 12.6.
+bool use_small(int64_t rows_q, int64_t rows_kv, int64_t Hq, int64_t D, int n_seq) {
+    return rows_q * Hq * D <= 6000 * 128 && rows_kv <= 1024 && n_seq <= 1024;
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
@@ -965,18 +1223,6 @@ extern "C" ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const ac
         note_launches(0, 0);
         return ACEFA_OK;
     }
-    // no keys at all: nothing is loaded, but the kernel's parameters still want a map
-    CUtensorMap qm, km, vm;
-    int         mrc = encode_rows(&qm, q);
-    if (mrc == ACEFA_OK) {
-        mrc = encode_rows(&km, rows_kv ? k : q);
-    }
-    if (mrc == ACEFA_OK) {
-        mrc = encode_rows(&vm, rows_kv ? v : q);
-    }
-    if (mrc != ACEFA_OK) {
-        return mrc;
-    }
     PackedParams p;
     std::memset(&p, 0, sizeof(p));
     p.dst   = static_cast<char *>(dst->data);
@@ -992,14 +1238,44 @@ extern "C" ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const ac
     p.scale_log2    = scale * kLog2e;
     p.dev_err       = ctx.dev_err;
     p.wait_limit_ns = ctx.wait_limit_ns;
+    const bool bf     = q->type == ACEFA_TYPE_BF16;
+    auto       cs = static_cast<cudaStream_t>(stream);
+    if (use_small(rows_q, rows_kv, Hq, D, n_seq)) {
+        SmallParams sp;
+        sp.p = p;
+        sp.q = static_cast<const char *>(q->data), sp.k = static_cast<const char *>(k->data);
+        sp.v = static_cast<const char *>(v->data);
+        sp.q_nb1 = (int64_t) q->nb[1], sp.q_nb2 = (int64_t) q->nb[2];
+        sp.k_nb1 = (int64_t) k->nb[1], sp.k_nb2 = (int64_t) k->nb[2];
+        sp.v_nb1 = (int64_t) v->nb[1], sp.v_nb2 = (int64_t) v->nb[2];
+        const dim3 grid((unsigned) (rows_q / kSmallRows + n_seq), (unsigned) Hq);
+        auto       kern = D == 128 ? (bf ? fa_packed_small<128, true> : fa_packed_small<128, false>)
+                                   : (bf ? fa_packed_small<64, true> : fa_packed_small<64, false>);
+        kern<<<grid, 32 * kSmallWarps, 0, cs>>>(sp);
+        if (cudaGetLastError() != cudaSuccess) {
+            return ACEFA_ERR_CUDA;
+        }
+        note_launches(1, 3);
+        return ACEFA_OK;
+    }
+    // no keys at all: nothing is loaded, but the kernel's parameters still want a map
+    CUtensorMap qm, km, vm;
+    int         mrc = encode_rows(&qm, q);
+    if (mrc == ACEFA_OK) {
+        mrc = encode_rows(&km, rows_kv ? k : q);
+    }
+    if (mrc == ACEFA_OK) {
+        mrc = encode_rows(&vm, rows_kv ? v : q);
+    }
+    if (mrc != ACEFA_OK) {
+        return mrc;
+    }
     // units: at most (tiles of all sequences * G + 1 per sequence) / 2 per KV head
     const int64_t tiles = rows_q / kBM + n_seq;
     const int64_t units = (tiles * (Hq / Hkv) + n_seq) / 2 * Hkv;
     const int     n_cta = (int) std::min<int64_t>(std::max<int64_t>(units, 1), ctx.sm_count);
-    auto          s     = static_cast<cudaStream_t>(stream);
-    const bool    bf    = q->type == ACEFA_TYPE_BF16;
-    cudaError_t   e     = D == 128 ? (bf ? launch<128, true>(p, qm, km, vm, n_cta, s) : launch<128, false>(p, qm, km, vm, n_cta, s))
-                                   : (bf ? launch<64, true>(p, qm, km, vm, n_cta, s) : launch<64, false>(p, qm, km, vm, n_cta, s));
+    cudaError_t   e     = D == 128 ? (bf ? launch<128, true>(p, qm, km, vm, n_cta, cs) : launch<128, false>(p, qm, km, vm, n_cta, cs))
+                                   : (bf ? launch<64, true>(p, qm, km, vm, n_cta, cs) : launch<64, false>(p, qm, km, vm, n_cta, cs));
     if (e != cudaSuccess) {
         return ACEFA_ERR_CUDA;
     }

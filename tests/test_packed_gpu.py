@@ -49,6 +49,12 @@ def _check(got, q, k, v, cu_q, cu_k, mask, window, scale, kind, out_kind):
     return on, want
 
 
+def _rows(total, Hq, D, many):
+    """Rows of the tensors: more than the sequences have select the kernel for many rows (the few-rows kernel
+    takes rows x heads x D up to 768000)."""
+    return max(total, 768000 // (Hq * D) + 1) if many else total
+
+
 CASES = [
     ([1], 1, 1, 64), ([1, 1, 1], 2, 1, 128), ([128], 4, 2, 128), ([127, 129, 1, 0, 64], 4, 2, 128),
     ([300, 77], 3, 1, 64), ([5] * 40, 2, 2, 64), ([513, 256, 2], 8, 1, 128), ([640], 5, 5, 128),
@@ -56,39 +62,44 @@ CASES = [
 ]
 
 
+@pytest.mark.parametrize("many", [False, True])
 @pytest.mark.parametrize("mask,window", [(0, 0), (1, 0), (2, 0), (2, 63), (2, 300)])
 @pytest.mark.parametrize("kind,out_kind", [("f16", "f16"), ("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32")])
 @pytest.mark.parametrize("lens,Hq,H,D", CASES)
-def test_packed(lens, Hq, H, D, kind, out_kind, mask, window):
+def test_packed(lens, Hq, H, D, kind, out_kind, mask, window, many):
     total = sum(lens)
-    q, k, v = _inputs([len(lens), total, D], Hq, H, total, total, D, kind)
+    rows = _rows(total, Hq, D, many)
+    q, k, v = _inputs([len(lens), total, D], Hq, H, rows, rows, D, kind)
     cu = _cu(lens)
-    out = torch.full((total, Hq, D), 9.0, dtype=DT[out_kind], device="cuda")
+    out = torch.full((rows, Hq, D), 9.0, dtype=DT[out_kind], device="cuda")
     acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu.tolist()), mask=mask, window=window, out=out)
     assert acefa.last_path() == 3
-    _check(out, q, k, v, cu, cu, mask, window, D ** -0.5, kind, out_kind)
+    _check(out[:total], q[:, :total], k, v, cu, cu, mask, window, D ** -0.5, kind, out_kind)
+    assert (out[total:] == 9.0).all()
     assert acefa.device_error() == 0
 
 
+@pytest.mark.parametrize("many", [False, True])
 @pytest.mark.parametrize("mask", [0, 1])
 @pytest.mark.parametrize("lq,lk", [([5, 1, 130, 7], [200, 64, 130, 3]), ([1, 1], [1, 700]), ([64, 9], [0, 129]),
                                    ([300], [20])])
-def test_queries_behind_a_prefix(mask, lq, lk):
+def test_queries_behind_a_prefix(mask, lq, lk, many):
     """Other offsets for the keys: the last rows of a longer sequence, fewer keys than queries, none at all
     (rows that see nothing are 0)."""
     D, Hq, H = 128, 4, 2
-    q, k, v = _inputs([sum(lq), sum(lk)], Hq, H, sum(lq), sum(lk), D, "bf16")
+    q, k, v = _inputs([sum(lq), sum(lk)], Hq, H, _rows(sum(lq), Hq, D, many), sum(lk), D, "bf16")
     cu_q, cu_k = _cu(lq), _cu(lk)
-    out = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu_q.tolist()), _i32(cu_k.tolist()), mask=mask)
-    _check(out, q, k, v, cu_q, cu_k, mask, 0, D ** -0.5, "bf16", "bf16")
+    out = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu_q.tolist()), _i32(cu_k.tolist()), mask=mask)[:sum(lq)]
+    _check(out, q[:, :sum(lq)], k, v, cu_q, cu_k, mask, 0, D ** -0.5, "bf16", "bf16")
     if mask == 1 and lq == [300]:
         assert (out[:280] == 0).all() and (out[280:] != 0).any()
 
 
-def test_strides_gaps_and_poison_around_the_sequences():
+@pytest.mark.parametrize("rows", [420, 1200])
+def test_strides_gaps_and_poison_around_the_sequences(rows):
     """Rows of a (rows, Hq + 2H, D) projection, offsets that start late and end early, NaN and infinity in every
     row that belongs to no sequence: none of it reaches the output, whose other rows stay as they were."""
-    D, Hq, H, rows = 128, 6, 2, 420
+    D, Hq, H = 128, 6, 2
     r = np.random.default_rng(12)
     x = torch.from_numpy(r.standard_normal((rows, Hq + 2 * H, D)).astype(np.float32)).half()
     cu = np.array([40, 171, 171, 300, 377])
@@ -107,16 +118,18 @@ def test_strides_gaps_and_poison_around_the_sequences():
         assert (big[:40] == 3.0).all() and (big[377:] == 3.0).all() and (big[:, Hq] == 3.0).all()
 
 
-def test_a_sequence_never_reads_its_neighbour():
+@pytest.mark.parametrize("many", [False, True])
+def test_a_sequence_never_reads_its_neighbour(many):
     """NaN in every row of one sequence leaves the others bit for bit as they are."""
     D, Hq, H, lens = 64, 4, 2, [100, 50, 200]
-    q, k, v = _inputs([3, 3], Hq, H, 350, 350, D, "bf16")
+    rows = _rows(350, Hq, D, many)
+    q, k, v = _inputs([3, 3], Hq, H, rows, rows, D, "bf16")
     cu = _i32(_cu(lens).tolist())
     a = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), cu, mask=1)
     for t in (q, k, v):
         t[:, 100:150] = float("nan")
     b = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), cu, mask=1)
-    assert torch.equal(a[:100], b[:100]) and torch.equal(a[150:], b[150:]) and torch.isnan(b[100:150]).all()
+    assert torch.equal(a[:100], b[:100]) and torch.equal(a[150:350], b[150:350]) and torch.isnan(b[100:150]).all()
 
 
 @pytest.mark.parametrize("mask", [0, 1])
@@ -129,31 +142,37 @@ def test_thousands_of_short_sequences(mask):
     _check(out, q, k, v, cu, cu, mask, 0, D ** -0.5, "f16", "f16")
 
 
-def test_large_and_small_scales():
+@pytest.mark.parametrize("many", [False, True])
+def test_large_and_small_scales(many):
     D, lens = 128, [200, 129]
-    q, k, v = _inputs([7, 7], 2, 1, 329, 329, D, "f16")
+    rows = _rows(329, 2, D, many)
+    q, k, v = _inputs([7, 7], 2, 1, rows, rows, D, "f16")
     cu = _cu(lens)
     for scale in (1.0, 0.3, 1e-6):
-        out = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu.tolist()), mask=1, scale=scale)
-        _check(out, q, k, v, cu, cu, 1, 0, scale, "f16", "f16")
+        out = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu.tolist()), mask=1, scale=scale)[:329]
+        _check(out, q[:, :329], k, v, cu, cu, 1, 0, scale, "f16", "f16")
 
 
-def test_unaligned_output_rows():
+@pytest.mark.parametrize("out_kind", ["f16", "f32"])
+@pytest.mark.parametrize("many", [False, True])
+def test_unaligned_output_rows(many, out_kind):
     """Output rows at an odd element offset and stride."""
     D, lens = 64, [140, 3]
-    q, k, v = _inputs([8, 7], 2, 2, 143, 143, D, "f16")
+    rows = _rows(143, 2, D, many)
+    q, k, v = _inputs([8, 7], 2, 2, rows, rows, D, "f16")
     cu = _cu(lens)
-    buf = torch.zeros(143 * (2 * D + 5) + 1, dtype=torch.float16, device="cuda")
-    out = buf[1:].as_strided((143, 2, D), (2 * D + 5, D + 1, 1))
+    buf = torch.zeros(rows * (2 * D + 5) + 1, dtype=DT[out_kind], device="cuda")
+    out = buf[1:].as_strided((rows, 2, D), (2 * D + 5, D + 1, 1))
     acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu.tolist()), mask=1, out=out)
-    _check(out, q, k, v, cu, cu, 1, 0, D ** -0.5, "f16", "f16")
+    _check(out[:143], q[:, :143], k, v, cu, cu, 1, 0, D ** -0.5, "f16", out_kind)
 
 
-def test_bad_offsets_are_skipped_and_reported():
+@pytest.mark.parametrize("rows", [100, 6100])
+def test_bad_offsets_are_skipped_and_reported(rows):
     D = 64
-    q, k, v = _inputs([1, 9], 2, 1, 100, 100, D, "f16")
-    out = torch.full((100, 2, D), 5.0, dtype=torch.float16, device="cuda")
-    cu = [0, 30, 20, 200]  # decreasing, then past the rows
+    q, k, v = _inputs([1, 9], 2, 1, rows, rows, D, "f16")
+    out = torch.full((rows, 2, D), 5.0, dtype=torch.float16, device="cuda")
+    cu = [0, 30, 20, rows + 100]  # decreasing, then past the rows
     acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu), mask=1, out=out)
     _check(out[:30], q[:, :30], k, v, np.array([0, 30]), np.array([0, 30]), 1, 0, D ** -0.5, "f16", "f16")
     assert (out[30:] == 5.0).all()
@@ -167,8 +186,9 @@ def test_empty_calls_launch_nothing():
     assert acefa.last_launch_count() == 0
 
 
-def test_captured_with_new_offsets():
-    D, Hq, H, rows = 128, 4, 2, 400
+@pytest.mark.parametrize("rows", [400, 1600])
+def test_captured_with_new_offsets(rows):
+    D, Hq, H = 128, 4, 2
     q, k, v = _inputs([4, 9], Hq, H, rows, rows, D, "bf16")
     qd, kd, vd = q.cuda(), k.cuda(), v.cuda()
     cu = _i32([0, 100, 400, 400])
@@ -184,4 +204,4 @@ def test_captured_with_new_offsets():
         cu.copy_(_i32(offsets))
         graph.replay()
         torch.cuda.synchronize()
-        _check(call.out, q, k, v, np.array(offsets), np.array(offsets), 1, 0, D ** -0.5, "bf16", "bf16")
+        _check(call.out[:400], q[:, :400], k, v, np.array(offsets), np.array(offsets), 1, 0, D ** -0.5, "bf16", "bf16")
