@@ -1204,14 +1204,24 @@ extern "C" ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const ac
         if (t->ne[1] == 0) {
             continue;  // no rows: strides say nothing
         }
-        if (t->nb[0] != 2 || !aligned(t->data, 16) || (t->ne[1] > 1 && t->nb[1] % 16) ||
-            (t->ne[2] > 1 && t->nb[2] % 16)) {
+        if (t->nb[0] != 2 || !aligned(t->data, 16)) {
             return ACEFA_ERR_LAYOUT;
+        }
+        for (int i = 1; i < 3; ++i) {  // (no tensor map has a stride of 0)
+            if (t->ne[i] > 1 && (t->nb[i] % 16 || t->nb[i] == 0)) {
+                return ACEFA_ERR_LAYOUT;
+            }
         }
     }
     const size_t es = dst->type == ACEFA_TYPE_F32 ? 4 : 2;
     if ((rows_q && (dst->nb[0] != es || !aligned(dst->data, es))) || (Hq > 1 && dst->nb[1] % es) ||
         (rows_q > 1 && dst->nb[2] % es) || !aligned(cu_q, 4) || !aligned(cu_k, 4)) {
+        return ACEFA_ERR_LAYOUT;
+    }
+    // no two rows of dst on one another (its heads and rows in either order)
+    const size_t row = (size_t) D * es, heads = dst->nb[1], rows = dst->nb[2];
+    if ((Hq > 1 && heads < row) || (rows_q > 1 && rows < row) ||
+        (Hq > 1 && rows_q > 1 && rows < heads * (size_t) Hq && heads < rows * (size_t) rows_q)) {
         return ACEFA_ERR_LAYOUT;
     }
     DeviceCtx ctx;

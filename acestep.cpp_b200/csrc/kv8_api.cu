@@ -27,25 +27,37 @@ size_t extent(const acefa_tensor &t) {
     }
     return b;
 }
-bool overlap(const acefa_tensor &a, const acefa_tensor &b) {
-    const auto x = reinterpret_cast<uintptr_t>(a.data), y = reinterpret_cast<uintptr_t>(b.data);
-    return x < y + extent(b) && y < x + extent(a);
-}
-// No two elements at one address (so that kernels may write it in any order).
-bool disjoint(const acefa_tensor &t) {
-    int    order[4] = {0, 1, 2, 3};
+// No two elements at one address (so that kernels may write it in any order);
+// with `twin`, nor one with an element of the same tensor `twin` bytes further on.
+bool disjoint(const acefa_tensor &t, size_t twin = 0) {
+    size_t nb[5]    = {t.nb[0], t.nb[1], t.nb[2], t.nb[3], twin};
+    size_t ne[5]    = {(size_t) t.ne[0], (size_t) t.ne[1], (size_t) t.ne[2], (size_t) t.ne[3], twin ? 2u : 1u};
+    int    order[5] = {0, 1, 2, 3, 4};
     size_t next     = elem_size(t.type);
-    std::sort(order, order + 4, [&](int a, int b) { return t.nb[a] < t.nb[b]; });
+    std::sort(order, order + 5, [&](int a, int b) { return nb[a] < nb[b]; });
     for (int i : order) {
-        if (t.ne[i] == 1) {
+        if (ne[i] == 1) {
             continue;
         }
-        if (t.nb[i] < next) {
+        if (nb[i] < next) {
             return false;
         }
-        next = t.nb[i] * (size_t) t.ne[i];
+        next = nb[i] * ne[i];
     }
     return true;
+}
+// Whether a and b share an address, as far as their extents tell; two of the
+// same layout may be interleaved (K and V of one buffer).
+bool overlap(const acefa_tensor &a, const acefa_tensor &b) {
+    const auto x = reinterpret_cast<uintptr_t>(a.data), y = reinterpret_cast<uintptr_t>(b.data);
+    if (!(x < y + extent(b) && y < x + extent(a))) {
+        return false;
+    }
+    bool same = a.type == b.type && x != y;
+    for (int i = 0; i < 4; ++i) {
+        same = same && a.ne[i] == b.ne[i] && a.nb[i] == b.nb[i];
+    }
+    return !(same && disjoint(a, x < y ? y - x : x - y));
 }
 
 int check_shape(const acefa_tensor &t, int64_t n0, int64_t n1, int64_t n2, int64_t n3) {
@@ -87,9 +99,13 @@ int check_cache(const acefa_kv8_cache *c, bool written, Kv8Dev *d) {
         }
     }
     for (const acefa_tensor *t : {&c->k, &c->v}) {
-        if (t->nb[0] != 1 || !aligned(t->data, 16) || (t->ne[1] > 1 && t->nb[1] % 16) ||
-            (t->ne[2] > 1 && t->nb[2] % 16) || (t->ne[3] > 1 && t->nb[3] % 16) || (written && !disjoint(*t))) {
+        if (t->nb[0] != 1 || !aligned(t->data, 16) || (written && !disjoint(*t))) {
             return ACEFA_ERR_LAYOUT;
+        }
+        for (int i = 1; i < 4; ++i) {  // (no tensor map has a stride of 0)
+            if (t->ne[i] > 1 && (t->nb[i] % 16 || t->nb[i] == 0)) {
+                return ACEFA_ERR_LAYOUT;
+            }
         }
     }
     if (written) {

@@ -325,7 +325,7 @@ ACEFA_API int acefa_cfg_logit_combine(const float *cond, const float *uncond, in
  * a little over half the bytes.  Row j of (head h, set s) stands for the values
  *   k[d, j, h, s] * k_scale[j / 64, h, s]         (each product rounded to F32)
  * and likewise for v.  k, v: I8 [D, n_max, Hkv, Bk], D 64 or 128, nb[0] == 1,
- * data and nb[1..3] multiples of 16 bytes; k_scale, v_scale: F32
+ * data and nb[1..3] multiples of 16 bytes, not 0; k_scale, v_scale: F32
  * [ceil(n_max / 64), Hkv, Bk], nb[0] == 4.  1 <= Bk <= ACEFA_KV8_MAX_SETS,
  * Hkv <= 4096.  A cache needs no initialisation: rows at or past a set's
  * length are never read as values.
@@ -447,8 +447,9 @@ ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *
  * they hold.  Offsets must not decrease: a sequence whose offsets do, or leave
  * the tensors, is left unwritten and raises device error 5
  * (acefa_device_error()).  nb[0] = the element size; data and nb[1..2] of q, k and
- * v multiples of 16 bytes; dst aligned to its elements.  rows_q and
- * rows_kv up to 2^24, n_seq <= 65535, Hq <= 4096.  No workspace.
+ * v multiples of 16 bytes, not 0; dst aligned to its elements, its rows apart, and
+ * apart from q, k and v.  rows_q and rows_kv up to 2^24, n_seq <= 65535,
+ * Hq <= 4096.  No workspace.
  */
 ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const acefa_tensor *k, const acefa_tensor *v,
                                       const acefa_tensor *dst, const int32_t *cu_q, const int32_t *cu_k, int n_seq,

@@ -73,6 +73,18 @@ def test_store_refusals(lib):
     assert _store(lib, k=inside, v=_t(f32, (128, 6, 2), 4, 1 << 29)) == -4  # overlaps the cache
 
 
+def test_keys_and_values_of_one_buffer_are_accepted(lib):
+    """k and v interleaved per set, per head or per row are no overlap; shifted by less than a row they are."""
+    sets = [1, 128, 128 * 200, 2 * 2 * 128 * 200]
+    heads = [1, 128, 2 * 128 * 200, 2 * 2 * 128 * 200]
+    rows = [1, 256, 256 * 200, 2 * 256 * 200]
+    for nb, step in ((sets, 2 * 128 * 200), (heads, 128 * 200), (rows, 128)):
+        k, v = (_t(acefa.GGML_I8, (128, 200, 2, 3), 1, x, nb=nb) for x in (1 << 24, (1 << 24) + step))
+        assert _store(lib, cache=_cache(k=k, v=v)) in NO_DEVICE
+        v = _t(acefa.GGML_I8, (128, 200, 2, 3), 1, (1 << 24) + step - 16, nb=nb)
+        assert _store(lib, cache=_cache(k=k, v=v)) == -4
+
+
 @pytest.mark.parametrize("change,want", [
     ({"D": 96}, -3), ({"D": 256}, -3), ({"B": 1025}, -3), ({"H": 5000}, -3), ({"n": 0}, -3),
     ({"k": _t(acefa.GGML_F16, (128, 200, 2, 3), 2, 1 << 24)}, -2),
@@ -187,6 +199,10 @@ def test_packed_refusals(lib):
     assert packed(k=_t(f16, (128, 50, 2), 2, 1 << 27, nb=[2, 264, 13200, 13200])) == -4
     assert packed(q=_t(f16, (128, 1, 4), 2, 1 << 26), dst=_t(f16, (128, 4, 1), 2, (1 << 29) + 1)) == -4
     assert packed(cu=ctypes.c_void_p(257)) == -4
+    assert packed(k=_t(f16, (128, 50, 2), 2, 1 << 27, nb=[2, 256, 0, 0])) == -4
+    q = _t(f16, (128, 7, 4), 2, 1 << 26)
+    for nb in ([2, 256, 512, 0], [2, 128, 1024, 0], [2, 0, 256, 0], [2, 1024, 512, 0]):
+        assert packed(q=q, dst=_t(f16, (128, 4, 7), 2, 1 << 29, nb=nb)) == -4, nb
 
 
 def test_python_refusals():

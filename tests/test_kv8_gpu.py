@@ -197,6 +197,8 @@ def _attend_tol(q, k, v, scale, D, kind):
     (128, 3, 1, 3, [5000], 5000, "f32"),
     (128, 16, 1, 1, [4500], 5000, "f16"),
     (64, 6, 1, 2, [6001], 6001, "f32"),
+    (64, 32, 1, 2, [300, 77], 300, "bf16"),
+    (128, 32, 1, 2, [7000], 7000, "f16"),
     (64, 2, 1, 1, [(37 * i) % 131 for i in range(400)], 130, "f32"),
 ])
 @pytest.mark.parametrize("weigh", [False, True])
