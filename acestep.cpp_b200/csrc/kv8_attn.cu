@@ -567,7 +567,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], phase, abort_f, P.dev_err, DEVERR_TIMEOUT_FULL,
                                                        P.wait_limit_ns)) && ok;
         if (ok && j0 < at.len) {  // uniform over the warp
-            const float kd = s_sc[2 * stage], vd = s_sc[2 * stage + 1];
+            const float kd = s_sc[2 * stage];
+            float       vd = s_sc[2 * stage + 1];
             // ---- S^T = K Q^T
             // (two sums per product, of the even and the odd k-steps: half as long a chain)
             float s[NT][4], s2[NT][MODE == kSplit ? 3 : 1][4];
@@ -632,6 +633,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     for (int e = 0; e < 4; ++e) {
                         s[nt][e] = j0 + g + 8 * (e >> 1) < lim[nt][e & 1] ? s[nt][e] : -INFINITY;
                     }
+                }
+                if (!(fabsf(vd) < INFINITY)) {
+                    // V's scale is no number, and 0 * NaN would reach the rows that see
+                    // nothing of the chunk: the others' sums become NaN here
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                            for (int t = 0; t < KS; ++t) {
+                                acc_o[nt][t][e] = j0 < lim[nt][e & 1] ? NAN : acc_o[nt][t][e];
+                            }
+                        }
+                    }
+                    vd = 0.0f;
                 }
             }
 #pragma unroll

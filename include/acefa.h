@@ -384,7 +384,8 @@ ACEFA_API int acefa_kv8_load(const acefa_kv8_cache *cache, const int32_t *len, c
  *   dst     [D, Hq, n_q, Bk] F32, F16 or BF16, nb[0] = the element size
  *   weight  F32 [n_max, Hkv, Bk], nb[0] == 4, or NULL
  * Query i sees rows j < len - (n_q - 1 - i) of its set.  dst = softmax(scale *
- * q k^T) v; a query that sees nothing gives 0.  With `weight`, weight[j, h, s]
+ * q k^T) v; a query that sees nothing gives 0, and a block whose scale is NaN
+ * reaches only the queries that see one of its rows.  With `weight`, weight[j, h, s]
  * grows by the softmax weights of row j summed over the n_q * Hq / Hkv
  * queries of its head -- what acefa_kv8_evict goes by; rows at or past
  * len[s] are left alone.  Q, the weights and the sums are held in F32
@@ -444,7 +445,8 @@ ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *
  * dst = softmax(scale * q k^T) v per sequence, scale > 0, sums in F32; a query
  * that sees nothing gives 0.  Rows of dst outside every sequence are left as
  * they were, and rows of k and v outside a sequence never reach it, whatever
- * they hold.  Offsets must not decrease: a sequence whose offsets do, or leave
+ * they hold; a NaN or an infinity in a sequence's own v may reach every query of
+ * that sequence and head.  Offsets must not decrease: a sequence whose offsets do, or leave
  * the tensors, is left unwritten and raises device error 5
  * (acefa_device_error()).  nb[0] = the element size; data and nb[1..2] of q, k and
  * v multiples of 16 bytes, not 0; dst aligned to its elements, its rows apart, and

@@ -245,6 +245,64 @@ def test_attend_large_scores_and_small_queries():
     assert np.abs(out - want).max() <= tol + half * np.abs(want).max()
 
 
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("D,Hq,H,n_q,sets,n_max,kind", [
+    (128, 4, 4, 4, 1, 130, "f32"), (128, 8, 4, 4, 2, 130, "f32"), (64, 16, 4, 4, 1, 130, "bf16"),
+    (128, 4, 1, 4, 1, 5000, "f16"), (64, 1, 1, 4, 3, 5000, "f32"), (128, 2, 1, 20, 1, 130, "f32")])
+def test_a_nan_row_reaches_only_the_queries_that_see_its_block(D, Hq, H, n_q, sets, n_max, kind, side):
+    """The last drafted row opens a block, and its K or V holds a NaN: the queries before it give what
+    they gave without it, the last one NaN."""
+    r = _rng(D, Hq, n_q, n_max, 7)
+    ln = 65 + 64 * ((n_max - 66) // 64)
+    cache, cq, cs = _cache(r, sets, H, n_max, D)
+    bad = [_rows(r, H, sets, D) for _ in range(2)]
+    bad["kv".index(side)][:, :, 3] = np.nan
+    acefa.kv8_store(cache, *(torch.from_numpy(x).cuda() for x in bad), _i32([ln - 1] * sets))
+    block = (ln - 1) // 64
+    assert torch.isnan((cache.k_scale if side == "k" else cache.v_scale)[:, :, block]).all()
+    q = torch.from_numpy(r.standard_normal((sets, Hq, n_q, D)).astype(np.float32)).to(DT[kind])
+    out = acefa.kv8_attn(q.cuda(), cache, _i32([ln] * sets)).cpu()
+    assert torch.isnan(out[:, -1]).all()
+    # the others saw the same rows before the last one was there
+    qn = q.float().numpy().astype(np.float64)
+    k, v = ref.values(cq[0], cs[0]), ref.values(cq[1], cs[1])
+    want, _ = ref.attend(qn[:, :, :-1], k, v, [ln - 1] * sets, D ** -0.5)
+    tol, _, half = _attend_tol(qn, k, v, D ** -0.5, D, kind)
+    assert np.abs(out[:, :-1].double().numpy() - want).max() <= tol + half * np.abs(want).max()
+
+
+@pytest.mark.parametrize("order", ["sets", "heads", "rows"])
+def test_keys_and_values_interleaved_in_one_buffer(order):
+    """Store, load, attention and eviction give the bits of a cache whose K and V lie apart."""
+    r = _rng(4, 5, len(order))
+    D, H, sets, n, keep = 128, 2, 3, 200, 90
+    lens = [200, 64, 131]
+    new = [torch.from_numpy(_rows(r, H, sum(lens), D)).cuda() for _ in range(2)]
+    q = torch.from_numpy(r.standard_normal((sets, 4, 1, D)).astype(np.float32)).cuda()
+
+    def build(rows):
+        scales = [torch.zeros((sets, H, -(-rows // 64)), device="cuda") for _ in range(2)]
+        shape = {"sets": (sets, 2, H, rows, D), "heads": (sets, H, 2, rows, D), "rows": (sets, H, rows, 2, D)}[order]
+        at = {"sets": 1, "heads": 2, "rows": 3}[order]
+        both = torch.zeros(shape, dtype=torch.int8, device="cuda")
+        return acefa.Kv8Cache(both.select(at, 0), both.select(at, 1), *scales)
+
+    def run(cache, out):
+        for c in (cache, out):
+            for t in c.tensors:
+                t.zero_()
+        weight = torch.zeros((sets, H, n), device="cuda")
+        kept, lo = torch.zeros((sets, H, keep), dtype=torch.int32, device="cuda"), _i32([0] * sets)
+        acefa.kv8_store(cache, *new, _i32([0] * sets), _cu(lens))
+        o = acefa.kv8_attn(q, cache, _i32(lens), weight=weight)
+        acefa.Kv8Evict(cache, weight, _i32(lens), out, kept, lo, n_first=4, n_recent=20)()
+        return [*cache.tensors, *acefa.kv8_load(cache, _i32(lens)), o, weight, *out.tensors, kept, lo]
+
+    for a, b in zip(run(build(n), build(keep)),
+                    run(acefa.Kv8Cache.empty(n, H, sets, D), acefa.Kv8Cache.empty(keep, H, sets, D))):
+        assert torch.equal(a, b)
+
+
 def test_attend_repeats_bit_for_bit_and_other_stream():
     r = _rng(3, 1, 4)
     cache, *_ = _cache(r, 5, 2, 900, 128)
