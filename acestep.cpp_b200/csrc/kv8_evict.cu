@@ -5,13 +5,14 @@
 // largest key is found by a radix descent (11 + 11 + 10 bits, one histogram
 // each, counts only, so the atomics' order changes nothing; it ends early where
 // a whole bin stays), and a scan in row order writes the rows above it and
-// the first of those equal to it.  One CTA per (head, set), the keys in shared
-// memory: bound by the latency of its passes.
+// the first of those equal to it.  One CTA per (head, set), the keys in registers
+// up to 8192 rows (9 us for 64 CTAs of 8192 rows; from shared memory 13): bound by
+// the latency of its passes.
 // Move.  One CTA per 64 destination rows of K and V of a (head, set): it reads the
 // rows' source blocks' scales, takes the largest, and copies the rows, rounding
 // those of another scale once more.  Every source row and destination byte is
 // touched once, 2 bytes per value kept.  Measured (B200), 8 sets x 8 heads, 8192
-// rows to 4000: selection 13 us, move 25 us (5.2 TB/s); 2 sets, 2048 to 1024: 7 and 6 us.
+// rows to 4000: selection 9 us, move 25 us (5.2 TB/s); 2 sets, 2048 to 1024: 7 and 6 us.
 #include "kv8_internal.h"
 #include "ptx.cuh"
 
@@ -22,6 +23,8 @@ constexpr int kSelThreads  = 1024;
 constexpr int kSelWarps    = kSelThreads / 32;
 constexpr int kBins        = 2048;
 constexpr int kSelMaxKeys  = 49152;  // keys held in shared memory; more are read again from L2
+constexpr int kSelRegs     = 8;      // of a thread: keys held in registers up to 8192 rows
+constexpr int kShared = 0, kAgain = -1;
 constexpr int kMoveThreads = 256;
 
 // Orders like the weight: larger weight, larger key; -0 as 0, NaN below all.
@@ -33,11 +36,13 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// One CTA per (head, set).  KEPT: the keys of [0, len) stay in shared memory.
-template <bool KEPT>
-__global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_constant__ Kv8EvictParams P) {
+// One CTA per (head, set); each warp owns a run of consecutive rows and a thread
+// every 32nd of them.  Where its keys wait between the passes: K > 0, in K
+// registers (up to 1024 K rows); kShared, in shared memory; kAgain, read again from L2.
+template <int K>
+__global__ void __launch_bounds__(kSelThreads, 1) kv8_select_kernel(const __grid_constant__ Kv8EvictParams P) {
     extern __shared__ uint32_t s_key[];
-    __shared__ int      hist[kBins];
+    __shared__ int      s_hist[3][kBins];
     __shared__ int      s_eq[kSelWarps], s_sure[kSelWarps];
     __shared__ uint32_t s_prefix;
     __shared__ int      s_need, s_done;
@@ -66,48 +71,78 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         }
         return;
     }
-    auto key_of = [&](int x) { return KEPT ? s_key[x] : order_key(__ldg(w + x)); };
     // candidates: rows [lo, hi); the others stay.  len > keep >= n_first + n_recent.
     const int  lo = P.n_first, hi = len - P.n_recent;
     const bool none = P.keep == P.n_first + P.n_recent;  // no candidate stays
-    if (KEPT) {
-        for (int x = tid; x < len; x += 4 * kSelThreads) {  // four loads on their way
+    const int  steps = (len + kSelThreads - 1) / kSelThreads;  // rows of a thread, K at most
+    const int  r0 = min(len, warp * steps * 32), r1 = min(len, r0 + steps * 32);  // the warp's run
+    uint32_t   reg[K > 0 ? K : 1];
+    if constexpr (K > 0) {
+        float v[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {  // all on their way together
+            v[i] = r0 + 32 * i + lane < r1 ? __ldg(w + r0 + 32 * i + lane) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            reg[i] = order_key(v[i]);
+        }
+    } else if constexpr (K == kShared) {
+        for (int x = r0 + lane; x < r1; x += 4 * 32) {  // four loads on their way
             float v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[e] = x + e * kSelThreads < len ? __ldg(w + x + e * kSelThreads) : 0.0f;
+                v[e] = x + e * 32 < r1 ? __ldg(w + x + e * 32) : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (x + e * kSelThreads < len) {
-                    s_key[x + e * kSelThreads] = order_key(v[e]);
+                if (x + e * 32 < r1) {
+                    s_key[x + e * 32] = order_key(v[e]);  // read by this thread alone
                 }
             }
         }
+    }
+    // f(row, key) for the rows of this thread; rows at or past r1 are none.  All
+    // threads take the same number of steps, so f may vote.
+    auto each_row = [&](auto f) {
+        if constexpr (K > 0) {
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                if (i < steps) {
+                    f(r0 + 32 * i + lane, reg[i]);
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < steps; ++i) {
+                const int x = r0 + 32 * i + lane;
+                f(x, x < r1 ? (K == kShared ? s_key[x] : order_key(__ldg(w + x))) : 0u);
+            }
+        }
+    };
+    for (int x = tid; x < 3 * kBins; x += kSelThreads) {
+        s_hist[0][x] = 0;
     }
     if (tid == 0) {
         s_prefix = 0u;
         s_need   = P.keep - P.n_first - P.n_recent;  // of the candidates
         s_done   = 0;
     }
+    __syncthreads();
     // ---- the need-th largest key, and how many of those equal to it are kept
     const int shifts[3] = {21, 10, 0};
     uint32_t  mask      = 0u;  // bits of the key settled so far
 #pragma unroll 1
     for (int pass = 0; pass < 3 && !none; ++pass) {
-        const int shift = shifts[pass], bins = pass == 2 ? 1024 : 2048;
-        for (int x = tid; x < kBins; x += kSelThreads) {
-            hist[x] = 0;
-        }
-        __syncthreads();
+        const int      shift = shifts[pass], bins = pass == 2 ? 1024 : 2048;
+        int           *hist   = s_hist[pass];
         const uint32_t prefix = s_prefix;
         const int      need   = s_need;
-        for (int x = lo + tid; x < hi; x += kSelThreads) {
-            const uint32_t key = key_of(x);
-            if ((key & mask) == prefix) {
+        each_row([&](int x, uint32_t key) {
+            if (x >= lo && x < min(hi, r1) && (key & mask) == prefix) {
                 atomicAdd(&hist[(key >> shift) & (uint32_t) (bins - 1)], 1);
             }
-        }
+        });
         __syncthreads();
         // suffix sums from the largest bin; the bin where they reach `need`
         const int b0 = kBins - 2 - 2 * tid;  // this thread: bins b0 + 1, b0, from the top
@@ -145,37 +180,25 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
             break;  // uniform
         }
     }
-    if (none) {
-        __syncthreads();
-    }
     // a candidate stays with a key above `top`, or as one of the first `need` equal
     // to it.  (A bin that starts at key 0 and stays whole keeps every candidate:
     // len > keep rules that out, so top - 1 does not wrap.)
     const uint32_t top  = s_done ? s_prefix - 1u : s_prefix;
     const int      need = s_need;
-    // ---- rows in order: each warp owns a contiguous run, 32 rows at a time
-    const int per = (len + kSelThreads - 1) / kSelThreads * 32;
-    const int r0 = min(len, warp * per), r1 = min(len, r0 + per);
-    auto look = [&](int x, bool &sure, bool &eq) {
-        sure = eq = false;
-        if (x < r1) {
-            if (x < lo || x >= hi) {
-                sure = true;
-            } else if (!none) {
-                const uint32_t key = key_of(x);
-                sure               = key > top;
-                eq                 = !s_done && key == top;
-            }
-        }
+    // ---- rows in order
+    auto look = [&](int x, uint32_t key, bool &sure, bool &eq) {
+        const bool candidate = x >= lo && x < hi;
+        sure = x < r1 && (!candidate || (!none && key > top));
+        eq   = x < r1 && candidate && !none && !s_done && key == top;
     };
     int n_eq = 0, n_sure = 0;
-    for (int x = r0; x < r1; x += 32) {
+    each_row([&](int x, uint32_t key) {
         bool sure, eq;
-        look(x + lane, sure, eq);
+        look(x, key, sure, eq);
         n_sure += __popc(__ballot_sync(0xffffffffu, sure));
         n_eq += __popc(__ballot_sync(0xffffffffu, eq));
-    }
-    __syncthreads();  // s_eq is free
+    });
+    // (s_eq is free: every pass ends with a barrier)
     if (lane == 0) {
         s_eq[warp]   = n_eq;
         s_sure[warp] = n_sure;
@@ -184,10 +207,9 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
     int eq_before = (int) __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0);  // before this run
     int at = (int) __reduce_add_sync(0xffffffffu, lane < warp ? s_sure[lane] : 0) + min(eq_before, need);
     const unsigned below = (1u << lane) - 1u;
-    for (int x0 = r0; x0 < r1; x0 += 32) {
-        const int x = x0 + lane;
-        bool      sure, eq;
-        look(x, sure, eq);
+    each_row([&](int x, uint32_t key) {
+        bool sure, eq;
+        look(x, key, sure, eq);
         const unsigned m_eq = __ballot_sync(0xffffffffu, eq);
         const bool     stay = sure || (eq && eq_before + __popc(m_eq & below) < need);
         const unsigned m    = __ballot_sync(0xffffffffu, stay);
@@ -200,7 +222,7 @@ __global__ void __launch_bounds__(kSelThreads) kv8_select_kernel(const __grid_co
         }
         eq_before += __popc(m_eq);
         at += __popc(m);
-    }
+    });
 }
 
 // grid (64-row blocks of `keep`, Hkv, B); K and V of the block
@@ -287,21 +309,23 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const __grid_con
 
 cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s) {
     const dim3 sel((unsigned) p.c.Hkv, (unsigned) p.c.B);
-    if (p.c.n_max <= kSelMaxKeys) {
+    if (p.c.n_max <= kSelRegs * kSelThreads) {
+        kv8_select_kernel<kSelRegs><<<sel, kSelThreads, 0, s>>>(p);
+    } else if (p.c.n_max <= kSelMaxKeys) {
         static thread_local int configured = -1;
         int                     dev        = 0;
         cudaGetDevice(&dev);
         if (configured != dev) {
-            const cudaError_t e = cudaFuncSetAttribute(kv8_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            const cudaError_t e = cudaFuncSetAttribute(kv8_select_kernel<kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                        kSelMaxKeys * (int) sizeof(uint32_t));
             if (e != cudaSuccess) {
                 return e;
             }
             configured = dev;
         }
-        kv8_select_kernel<true><<<sel, kSelThreads, (size_t) p.c.n_max * sizeof(uint32_t), s>>>(p);
+        kv8_select_kernel<kShared><<<sel, kSelThreads, (size_t) p.c.n_max * sizeof(uint32_t), s>>>(p);
     } else {
-        kv8_select_kernel<false><<<sel, kSelThreads, 0, s>>>(p);
+        kv8_select_kernel<kAgain><<<sel, kSelThreads, 0, s>>>(p);
     }
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {

@@ -424,7 +424,9 @@ def _check_evict(cache, cq, cs, weight, lens, keep, n_first, n_recent):
 @pytest.mark.parametrize("D,H,n,lens,keep,first,recent", [
     (128, 2, 300, [300, 299, 100, 0, 129], 128, 4, 30), (64, 3, 200, [200, 65], 64, 0, 0), (64, 1, 70, [70], 69, 0, 69),
     (128, 1, 1500, [1500, 1400], 700, 4, 100), (128, 1, 130, [130], 1, 0, 0), (64, 2, 100, [100, 90], 20, 10, 10),
-    (64, 1, 5000, [5000, 2049], 2050, 1, 7), (64, 1, 90, [90], 200, 3, 9)])
+    (64, 1, 5000, [5000, 2049], 2050, 1, 7), (64, 1, 90, [90], 200, 3, 9),
+    # around the longest cache whose keys fit the registers
+    (64, 1, 8192, [8192, 1025, 8161, 700], 600, 0, 3), (64, 2, 8193, [8193, 1024, 4097], 1000, 40, 0)])
 def test_evict(D, H, n, lens, keep, first, recent):
     r = _rng(D, n, keep)
     cache, cq, cs = _cache(r, len(lens), H, n, D, n_alloc=n + 2)
