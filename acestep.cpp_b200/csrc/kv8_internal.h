@@ -94,6 +94,26 @@ inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows 
 // ------------------------------------------------------------------ device helpers
 #ifdef __CUDACC__
 
+// Launches a kernel that begins with pdl_wait_primary(): its blocks are set up
+// while the stream's previous kernel ends, and wait there until it has.  Measured,
+// back to back: 0.2 us of a call of few rows, 0.3 of a store and of an eviction's
+// kernels each.  (Letting the next kernel start earlier, behind that wait, cost time:
+// store + load of one token 4.6 -> 5.2 us, eviction 15.7 -> 16.7, packed prompts 78 -> 81.)
+template <class... K, class... A>
+cudaError_t launch_pdl(void (*kernel)(K...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A &...args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim            = grid;
+    cfg.blockDim           = dim3((unsigned) threads);
+    cfg.dynamicSmemBytes   = smem;
+    cfg.stream             = s;
+    cfg.attrs              = attr;
+    cfg.numAttrs           = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Finds item x among the items of n segments, count(i) of segment i in their
 // order (fewer than 2^31 in all).  The whole warp calls it with the same arguments
 // and gets the same answer: the segment and the item's number in it, or false
