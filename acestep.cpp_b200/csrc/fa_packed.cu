@@ -1,5 +1,6 @@
 // fa_packed.cu -- attention of whole sequences packed behind one another
-// (acefa_flash_attn_packed) on the tensor cores (tcgen05 / TMEM / TMA).
+// (acefa_flash_attn_packed) on the tensor cores: a persistent tcgen05 / TMEM / TMA
+// kernel, described here, and one on mma.sync for few rows further down.
 //
 // Mathematics: the online softmax in log2 units, S = Q K^T and O += P V on
 // 128-row x 128-key tiles with F32 accumulators in tensor memory; P is rounded to
@@ -883,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // 16 keys of every 64 and loads exactly its fragments' 16-B pieces of rows to
 // registers, products run transposed (S^T = K Q^T, O^T = V^T P^T; P changes layout by
 // movmatrix), and the warps' results meet once in shared memory.  Bound by latency:
-// 3-5 us up to 128 rows of 16 heads against 8.5 us of the kernel above.
+// 2.7-4.5 us up to 128 rows of 16 heads, where the kernel above takes 8.2.
 constexpr int   kSmallRows = 16;
 constexpr int   kSmallWarps = 4;
 constexpr float kNoMax = -1.7e38f;  // below every score, finite

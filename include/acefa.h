@@ -499,7 +499,7 @@ ACEFA_API int acefa_last_launch_count(void);
 
 /* Which kernel family served the last successful call on this thread:
  * 1 = split-KV decode (mma.sync), 2 = dense tcgen05/TMEM, 3 = packed sequences
- * (tcgen05/TMEM), 4 = decode over an 8-bit block-scaled cache. */
+ * (tcgen05/TMEM, few rows mma.sync), 4 = decode over an 8-bit block-scaled cache. */
 ACEFA_API int acefa_last_path(void);
 
 /* ABI version: major*10000 + minor*100 + patch. */
