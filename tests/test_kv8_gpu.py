@@ -521,3 +521,62 @@ def test_prompt_decode_evict_decode():
         tol, wtol, half = _attend_tol(qn, k, v, D ** -0.5, D, "f32")
         assert np.abs(got - want).max() <= tol + half * np.abs(want).max()
     assert np.all(np.abs(weight.cpu().numpy() - total_w) <= total_w * (2 * wtol + 2.0 ** -18))
+
+
+def test_captured_behind_copies_and_other_streams():
+    """One graph of every entry behind a memset, a copy or a join of two streams; replayed with new inputs
+    it gives what eager calls give."""
+    r = _rng(6, 6, 6)
+    D, H, sets, n, keep, total = 64, 2, 2, 150, 70, 210
+    lens = _i32([150, 60])
+    cu = _cu([150, 60])
+    src = [torch.from_numpy(_rows(r, H, total, D)).half().cuda() for _ in range(3)]
+    qkv = [torch.empty_like(x) for x in src]
+    cache, small = acefa.Kv8Cache.empty(n, H, sets, D), acefa.Kv8Cache.empty(keep, H, sets, D)
+    q = torch.empty((sets, 2 * H, 1, D), dtype=torch.float16, device="cuda")
+    weight = torch.empty((sets, H, n), device="cuda")
+    kept, lo, pos = torch.empty((sets, H, keep), dtype=torch.int32, device="cuda"), _i32([0, 0]), _i32([0, 0])
+    packed = acefa.PackedAttn(*qkv, cu, mask=acefa.MASK_CAUSAL)
+    store, attn = acefa.Kv8Store(cache, qkv[1], qkv[2], pos, cu), acefa.Kv8Attn(q, cache, lens, weight=weight)
+    evict = acefa.Kv8Evict(cache, weight, lens, small, kept, lo, n_recent=5)
+    back = [torch.empty((sets, H, keep, D), device="cuda") for _ in range(2)]
+    load = acefa.Kv8Load(small, lo, *back)
+    outs = (packed.out, *cache.tensors, attn.out, weight, *small.tensors, kept, lo, *back)
+    side = torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        for a, b in zip(qkv, src):
+            a.copy_(b)
+        side.wait_stream(main)
+        packed(side)  # behind a fork
+        for t in cache.tensors:
+            t.zero_()
+        store()  # behind a memset
+        q.copy_(src[0][:, :2 * sets].reshape(sets, 2 * H, 1, D))
+        main.wait_stream(side)
+        weight.zero_()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            back[0].zero_()
+        main.wait_stream(side)
+        attn()  # behind a join
+        evict()
+        load()
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for step in range(3):
+        for x in src:
+            x.copy_(torch.from_numpy(_rows(r, H, total, D)).half())
+        graph.replay()
+        got = [t.clone() for t in outs]
+        for t in outs:
+            t.zero_()
+        run()
+        for a, b in zip(got, outs):
+            assert torch.equal(a, b)
+    assert acefa.device_error() == 0
