@@ -20,7 +20,7 @@ import torch
 GGML_F32, GGML_F16, GGML_Q8_0, GGML_I8, GGML_I32, GGML_BF16 = 0, 1, 8, 24, 26, 30
 PREC_DEFAULT, PREC_F32 = 0, 10
 
-OK = 0
+OK, ERR_DEVICE = 0, -7
 STATUS_NAMES = {
     0: "ACEFA_OK", -1: "ACEFA_ERR_NULL", -2: "ACEFA_ERR_TYPE", -3: "ACEFA_ERR_SHAPE",
     -4: "ACEFA_ERR_LAYOUT", -5: "ACEFA_ERR_WORKSPACE", -6: "ACEFA_ERR_CUDA",
@@ -520,20 +520,23 @@ class _Call:
         for t in tensors:
             if t.device != dev:
                 raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-        # a CUDA tensor's device always has an index; CPU tensors reach the ABI only in its argument checks
         self._what, self._keep, self._head, self._tail = what, tensors, head, tail
+        # a CUDA tensor's device always has an index; the entries cannot tell a host address from one of the
+        # device, so other tensors never reach them
         self._index = dev.index if dev.type == "cuda" else None
         self._fn = getattr(load_library(), what)
 
     def _launch(self, stream):
         index = self._index
+        if index is None:
+            raise AcefaError(ERR_DEVICE, f"{self._what}: tensors on {self._keep[0].device}")
         if stream is None:
-            handle = _current_stream(index) if index is not None else 0
-        elif index is not None and stream.device.index != index:
+            handle = _current_stream(index)
+        elif stream.device.index != index:
             raise ValueError(f"{self._what}: a stream of {stream.device} for tensors on cuda:{index}")
         else:
             handle = stream.cuda_stream
-        if index is None or index == torch.cuda.current_device():
+        if index == torch.cuda.current_device():
             st = self._fn(*self._head, handle, *self._tail)
         else:
             with torch.cuda.device(index):
