@@ -6,13 +6,17 @@
 //   s_rj = scale * kd_j * (q_r . k8_j),   p_rj = exp(s_rj - m_r),
 //   o_r  = sum_j vd_j p_rj v8_j / sum_j p_rj.
 // k8 and v8 are integers below 128, exact in F16.  An F32 q_r (scaled by a power
-// of two into F16's range) and the p_rj of an F32 output are split into two F16
-// numbers each, which together keep 22 bits, so that the F16 tensor-core
-// products with F32 sums lose nothing beside F32 arithmetic (a 16-bit q_r is
-// exact in one, and one rounding of p_rj to 11 bits is below a 16-bit output's
-// own); the scales multiply in F32: kd on the finished score, vd on the 16-key
-// partial product of V.  Up to four rows, the two halves of a split operand
-// ride in one product as columns r and r + 4 of its eight.
+// of two into F16's range) and, unless Q and the output both have 16 bits, the
+// p_rj are split into two F16 numbers each, which together keep 22 bits, so that
+// the F16 tensor-core products with F32 sums lose nothing beside F32 arithmetic
+// (a 16-bit q_r is exact in one, and one rounding of p_rj to 11 bits is below a
+// 16-bit output's own).  F16's steps end at 2^-24; m_r is therefore kept 2^kLift
+// below the running maximum, and p_rj reaches from 2^15 down: what its halves
+// cannot hold is below 2^-32 of the row's largest weight, so that thousands of
+// keys far below one early key still count.  The scales multiply in F32: kd on
+// the finished score, vd on the 16-key partial product of V.  Up to four rows,
+// the two halves of a split operand ride in one product as columns r and r + 4
+// of its eight.
 //
 // Work.  The (set, KV head, row block) units' 64-key tiles, numbered one after
 // another over all sets' actual lengths, are cut into equal runs, one per CTA:
@@ -35,8 +39,8 @@
 // CTA); 2 sets of 700 rows: 6 us, bound by the latencies of launch, Q and merge.
 // Products run transposed (keys or dims are the MMA's M, the rows its N = 8):
 // S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
-// operand layout by four movmatrix.  The running maximum moves only when a
-// score exceeds it by more than 2^8 (a warp vote), as in the other kernels.
+// operand layout by four movmatrix.  m_r moves only when a score exceeds the
+// maximum that it was taken from by more than 2^8 (a warp vote), as in the other kernels.
 #include <algorithm>
 #include <type_traits>
 
@@ -50,6 +54,7 @@ constexpr int   kWarps   = 4;  // consumers
 constexpr int   kThreads = 32 * (kWarps + 1);
 constexpr int   kChunk   = 16;  // keys of one warp and tile
 constexpr float kSlack   = 8.0f;
+constexpr float kLift    = 7.0f;  // kSlack + kLift = 15: the largest weight is 2^15, F16 holds 2^16
 constexpr int   kUnitCost = 2;
 // "No maximum yet": below every score, finite so that differences stay numbers
 // (2^(anything - it) only meets weights and sums that are 0).
@@ -654,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    grow |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + kSlack;
+                    grow |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + (kSlack + kLift);
                 }
             }
             if (P.scores) {
@@ -678,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                         top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        const float mn = fmaxf(m[nt][e], top);
+                        const float mn = fmaxf(m[nt][e], top - kLift);
                         const float f  = fast_exp2(m[nt][e] - mn);
                         m[nt][e]       = mn;
                         l[nt][e] *= f;

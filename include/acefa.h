@@ -388,8 +388,10 @@ ACEFA_API int acefa_kv8_load(const acefa_kv8_cache *cache, const int32_t *len, c
  * reaches only the queries that see one of its rows.  With `weight`, weight[j, h, s]
  * grows by the softmax weights of row j summed over the n_q * Hq / Hkv
  * queries of its head -- what acefa_kv8_evict goes by; rows at or past
- * len[s] are left alone.  Q, the weights and the sums are held in F32
- * precision throughout: the cache's rounding is the only one in 8 bits.
+ * len[s] are left alone.  Q enters whole and all sums are F32.  The softmax
+ * weights that multiply V are rounded to 22 bits, or to 11 (F16) where q and dst
+ * both have 16-bit types, and to steps of 2^-32 of the row's largest; those that
+ * `weight` receives are F32.
  * Results do not depend on the order in which the GPU runs the blocks.
  * workspace: acefa_kv8_attn_workspace_bytes(), 256-B aligned, no
  * initialisation; a function of shapes and the device only.  Calls that may

@@ -1,0 +1,72 @@
+"""GPU tests of the packed and 8-bit-cache entries at the edges of what they
+accept, against the plain 64-bit statements of kv8_ref.py."""
+import numpy as np
+import pytest
+import torch
+
+import acefa
+import kv8_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+LOG2E = 1.4426950408889634
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------ small weights beside a large one
+# Four sinks of weight 1 (the first key of every 16 of the first 64, whose values are 0) and thousands of keys
+# 2^-20 .. 2^-27 below them: what the output consists of are the small weights alone.
+#
+# Tolerance.  A score is off by at most e absolute (below), so a weight by a factor within exp(+-e) and twice
+# that after the normalisation, plus 2^-20 for the exponential and u for the weight's rounding (11 bits where
+# Q and the output have 16, else 22): a share r = 2e + 2^-20 + u of the mean of |v|, which is the output, all v
+# being positive; F32 sums add 2^-18 of it.  A weight that is too small for the rounding's exponents is off by
+# at most 2^-32 of the largest, and there are n of them over a sum of at least 4.  The output's own rounding:
+# half a step of its type, 2^-25 where F16 is subnormal.
+def _sink_values(r, n, low, high):
+    t = r.integers(4 * low, 4 * high + 1, n)  # quarters of a power of two
+    t[[0, 16, 32, 48]] = 0
+    v = r.integers(1, 128, n)
+    v[[0, 16, 32, 48]] = 0
+    return t, v
+
+
+def _sink_want(score, v):
+    p = np.exp2(score - score.max())
+    return float(p @ v / p.sum())
+
+
+def _sink_tol(want, n, e, u, kind):
+    return (2 * e + 2.0 ** -20 + u + 2.0 ** -18) * want + n * 2.0 ** -34 + torch.finfo(DT[kind]).eps / 2 * want + 2.0 ** -25
+
+
+@pytest.mark.parametrize("low,high", [(25.25, 27), (20, 27)])
+@pytest.mark.parametrize("D,G,n_q,kind", [(128, 1, 1, "f32"), (64, 4, 1, "f32"), (64, 8, 1, "f32"), (64, 3, 4, "f32"),
+                                          (128, 2, 1, "bf16"), (64, 16, 1, "f16"), (128, 6, 4, "bf16")])
+@pytest.mark.parametrize("sets,H", [(37, 1), (40, 8)])  # a cluster per unit; units of their own CTAs
+def test_small_weights_of_the_8_bit_cache(sets, H, D, G, n_q, kind, low, high):
+    n = 8192
+    r = np.random.default_rng([sets, D, G, n_q])
+    t, v = _sink_values(r, n, low, high)
+    k8 = torch.from_numpy(r.integers(-127, 128, (n, D), dtype=np.int8))  # (dims that Q does not look at)
+    k8[:, 0] = torch.from_numpy(-t)
+    v8 = torch.from_numpy(np.repeat(v.astype(np.int8)[:, None], D, 1))
+    tile = lambda x: x.cuda().expand(sets, H, n, D).contiguous()  # noqa: E731
+    scales = [torch.full((sets, H, n // 64), x, device="cuda") for x in (1.0, 1.0 / 127.0)]
+    cache = acefa.Kv8Cache(tile(k8), tile(v8), *scales)
+    scale = D ** -0.5
+    q = torch.zeros((sets, G * H, n_q, D), dtype=DT[kind], device="cuda")
+    q[..., 0] = 0.25 / (scale * LOG2E)
+    out = acefa.kv8_attn(q, cache, _i32([n] * sets), scale=scale).double().cpu().numpy()
+    q0 = float(q[0, 0, 0, 0])
+    for iq in range(n_q):
+        ln = n - (n_q - 1 - iq)
+        want = _sink_want(-t[:ln] * q0 * scale * LOG2E, v[:ln] * float(np.float32(1.0 / 127.0)))
+        A = scale * q0 * 4 * high
+        tol = _sink_tol(want, n, (2.0 ** -21 + D / 8 * 2.0 ** -23) * A, 2.0 ** -22 if kind == "f32" else 2.0 ** -11, kind)
+        assert np.abs(out[:, iq] - want).max() <= tol, (iq, np.abs(out[:, iq] - want).max(), want, tol)
+
