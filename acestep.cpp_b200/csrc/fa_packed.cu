@@ -5,7 +5,10 @@
 // Mathematics: the online softmax in log2 units, S = Q K^T and O += P V on
 // 128-row x 128-key tiles with F32 accumulators in tensor memory; P is rounded to
 // the operands' type (F16 or BF16), its row sum is not.  A row's maximum only
-// moves when it grows by more than 2^8, and O is rescaled only then.
+// moves when it grows by more than 2^8, and O is rescaled only then.  What is
+// subtracted lies kLift below that maximum: F16's steps end at 2^-24, and with P from
+// 2^15 down only weights below 2^-32 of the row's largest are lost in them (BF16
+// has F32's exponents).
 //
 // Work.  An item is a 128-token tile of one query head; the items of a
 // (sequence, KV head), tokens slowest, go two by two to one CTA, which streams
@@ -74,6 +77,8 @@ constexpr int      kSmemBytes = kOffStage + 8 * 4096 + 1024;  // + alignment of 
 static_assert(kSmemBytes <= 232448, "more than the 227 KB of a CTA");
 constexpr uint32_t kTmemCols  = 512;
 constexpr float    kSlack     = 8.0f;
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.0f : 7.0f;  // with kSlack: P is 2^15 at most, F16 holds 2^16
 // Register split (setmaxnreg): the sum must stay within what the block was
 // launched with, 384 x 168 = 64512, or setmaxnreg.inc would wait forever.
 constexpr uint32_t kRegsControl = 112;
@@ -717,10 +722,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     top = max_chunk<true>(x3, bit_range(vlo - j0 - 96, vhi - j0 - 96), top);
                 }
                 top *= c;
-                const bool grew = top > m_run + kSlack;  // the first visible key counts: any number is above -inf
+                // the first visible key counts: any number is above -inf
+                const bool grew = top > m_run + (kSlack + kLift<BF16>);
                 if (__any_sync(0xffffffffu, grew)) {
-                    const float f = grew ? fast_exp2(m_run - top) : 1.0f;
-                    m_run         = grew ? top : m_run;
+                    const float mn = top - kLift<BF16>;
+                    const float f  = grew ? fast_exp2(m_run - mn) : 1.0f;
+                    m_run          = grew ? mn : m_run;
                     l_run *= f;
                     if (j > ja) {
 #pragma unroll 1
@@ -1009,7 +1016,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid
                 const int   j = j0 + g + 8 * (e >> 1);
                 const float v = (s[nt][e] + s2[nt][e]) * P.scale_log2;
                 s[nt][e]      = j >= lo[nt][e & 1] && j < hi[nt][e & 1] ? v : -INFINITY;
-                grow |= s[nt][e] > m[nt][e & 1] + kSlack;
+                grow |= s[nt][e] > m[nt][e & 1] + (kSlack + kLift<BF16>);
             }
         }
         if (__any_sync(0xffffffffu, grow)) {
@@ -1021,7 +1028,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid
                     top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top       = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float mn = fmaxf(m[nt][e], top), f = fast_exp2(m[nt][e] - mn);
+                    const float mn = fmaxf(m[nt][e], top - kLift<BF16>), f = fast_exp2(m[nt][e] - mn);
                     m[nt][e] = mn;
                     l[nt][e] *= f;
 #pragma unroll

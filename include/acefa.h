@@ -444,7 +444,9 @@ ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *
  *   mask  0: every query sees every key of its sequence; ACEFA_MASK_CAUSAL:
  *         query i of n_q sees key j <= i + n_k - n_q (a prompt, or the last
  *         n_q tokens of one); ACEFA_MASK_WINDOW: |i - j| <= window
- * dst = softmax(scale * q k^T) v per sequence, scale > 0, sums in F32; a query
+ * dst = softmax(scale * q k^T) v per sequence, scale > 0, sums in F32; the weights
+ * that multiply v are rounded to the operands' type (11 bits, in steps of 2^-32 of
+ * the row's largest, or BF16's 8), their sum takes them whole.  A query
  * that sees nothing gives 0.  Rows of dst outside every sequence are left as
  * they were, and rows of k and v outside a sequence never reach it, whatever
  * they hold; a NaN or an infinity in a sequence's own v may reach every query of

@@ -70,3 +70,23 @@ def test_small_weights_of_the_8_bit_cache(sets, H, D, G, n_q, kind, low, high):
         tol = _sink_tol(want, n, (2.0 ** -21 + D / 8 * 2.0 ** -23) * A, 2.0 ** -22 if kind == "f32" else 2.0 ** -11, kind)
         assert np.abs(out[:, iq] - want).max() <= tol, (iq, np.abs(out[:, iq] - want).max(), want, tol)
 
+
+@pytest.mark.parametrize("low,high", [(25.25, 27), (20, 27)])
+@pytest.mark.parametrize("n,D,Hq,kind,out_kind", [(1024, 64, 2, "f16", "f32"), (1024, 128, 1, "f16", "f16"),
+                                                  (8192, 64, 2, "f16", "f32"), (8192, 128, 3, "f16", "f16"),
+                                                  (8192, 128, 2, "bf16", "f32"), (1000, 64, 1, "bf16", "bf16")])
+def test_small_weights_of_packed_sequences(n, D, Hq, kind, out_kind, low, high):
+    r = np.random.default_rng([n, D, Hq])
+    t, v = _sink_values(r, n, low, high)
+    scale, rows = D ** -0.5, 200
+    q = torch.zeros((Hq, rows, D), dtype=DT[kind])
+    q[..., 0] = 0.25 / (scale * LOG2E)
+    k = torch.from_numpy(r.standard_normal((1, n, D)).astype(np.float32)).to(DT[kind])
+    k[..., 0] = torch.from_numpy(-t).to(DT[kind])
+    v1 = torch.from_numpy(np.repeat(v[None, :, None] / 128.0, D, 2)).to(DT[kind])
+    out = acefa.PackedAttn(q.cuda(), k.cuda(), v1.cuda(), _i32([0, rows]), _i32([0, n]), scale=scale,
+                           out=torch.empty((rows, Hq, D), dtype=DT[out_kind], device="cuda"))().double().cpu().numpy()
+    q0 = float(q[0, 0, 0])
+    want = _sink_want(k[0, :, 0].double().numpy() * q0 * scale * LOG2E, v1[0, :, 0].double().numpy())
+    tol = _sink_tol(want, n, 2.0 ** -17 * scale * q0 * 4 * high, torch.finfo(DT[kind]).eps / 2, out_kind)
+    assert np.abs(out - want).max() <= tol, (np.abs(out - want).max(), want, tol)
