@@ -85,16 +85,18 @@ constexpr uint32_t kRegsControl = 112;
 constexpr uint32_t kRegsSoftmax = 192;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= 384 * 168, "register split exceeds the launch pool");
 
-// The rows of sequence s; empty and bad for offsets that are none.
+// The rows of sequence s; empty and bad for offsets that are none.  Where the
+// offsets of Q fall, the sequences behind could meet the rows of those before:
+// they end there.
 struct Seq {
     int  q0, n_q, k0, n_k;
-    bool bad;
+    bool bad, end;
 };
 __device__ __forceinline__ Seq seq_of(const PackedParams &P, int s) {
     const int a = __ldg(P.cu_q + s), b = __ldg(P.cu_q + s + 1), c = __ldg(P.cu_k + s), d = __ldg(P.cu_k + s + 1);
-    Seq       r = {a, b - a, c, d - c, false};
+    Seq       r = {a, b - a, c, d - c, false, false};
     if (a < 0 || b < a || b > P.rows_q || c < 0 || d < c || d > P.rows_kv) {
-        r = {0, 0, 0, 0, true};
+        r = {0, 0, 0, 0, true, b < a};
     }
     return r;
 }
@@ -175,7 +177,9 @@ __device__ __forceinline__ void find_unit(const PackedParams &P, int u, const Se
             if (from >= P.n_seq) {
                 return;
             }
-            np   = from + lane < P.n_seq ? n_pairs(P, seq_of(P, from + lane).n_q) : 0;
+            const Seq      s   = from + lane < P.n_seq ? seq_of(P, from + lane) : Seq{};
+            const unsigned end = __ballot_sync(0xffffffffu, s.end);
+            np   = end && lane >= __ffs(end) - 1 ? 0 : n_pairs(P, s.n_q);
             incl = np;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -185,6 +189,9 @@ __device__ __forceinline__ void find_unit(const PackedParams &P, int u, const Se
             hit = __ballot_sync(0xffffffffu, x < before + incl);
             if (hit) {
                 break;
+            }
+            if (end) {
+                return;
             }
             before += __shfl_sync(0xffffffffu, incl, 31);
         }
@@ -356,9 +363,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         setmaxnreg_dec<kRegsControl>();
         if (warp == 3) {
             // ============================ units ====================================
-            Seq mine = {0, 0, 0, 0, false};
-            if (P.n_seq <= 32 && lane < P.n_seq) {
-                mine = seq_of(P, lane);
+            Seq mine = {};
+            if (P.n_seq <= 32) {
+                mine               = lane < P.n_seq ? seq_of(P, lane) : mine;
+                const unsigned end = __ballot_sync(0xffffffffu, mine.end);
+                mine               = end && lane >= __ffs(end) - 1 ? Seq{} : mine;
             }
             Unit t;
             bool ok   = true;
@@ -671,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (row0 >= t.n_q) {
                 continue;
             }
-            const Seq  q        = {t.q0, t.n_q, t.k0, t.n_k, false};
+            const Seq  q        = {t.q0, t.n_q, t.k0, t.n_k, false, false};
             const int  row      = row0 + r;
             const bool mine_row = row < q.n_q;
             int        vlo = 0, vhi = 0;
@@ -925,7 +934,11 @@ __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid
         }
     }
     int si, item;
-    if (!find_item(P.n_seq, blockIdx.x, [&](int i) { return (seq_of(P, i).n_q + kSmallRows - 1) / kSmallRows; }, si, item)) {
+    auto tiles = [&](int i) {
+        const Seq s = seq_of(P, i);
+        return s.end ? -1 : (s.n_q + kSmallRows - 1) / kSmallRows;
+    };
+    if (!find_item(P.n_seq, blockIdx.x, tiles, si, item)) {
         return;
     }
     const Seq q    = seq_of(P, si);

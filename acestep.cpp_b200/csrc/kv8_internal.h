@@ -115,15 +115,17 @@ cudaError_t launch_pdl(void (*kernel)(K...), dim3 grid, int threads, size_t smem
 }
 
 // Finds item x among the items of n segments, count(i) of segment i in their
-// order (fewer than 2^31 in all).  The whole warp calls it with the same arguments
-// and gets the same answer: the segment and the item's number in it, or false
-// behind the last.
+// order (fewer than 2^31 in all); a negative count ends them.  The whole warp calls
+// it with the same arguments and gets the same answer: the segment and the item's
+// number in it, or false behind the last.
 template <class F>
 __device__ __forceinline__ bool find_item(int n, int x, F count, int &seg, int &item) {
     const int lane = threadIdx.x & 31;
     for (int base = 0; base < n; base += 32) {
-        const int mine = base + lane < n ? count(base + lane) : 0;
-        int       incl = mine;
+        int            mine = base + lane < n ? count(base + lane) : 0;
+        const unsigned end  = __ballot_sync(0xffffffffu, mine < 0);
+        mine                = end && lane >= __ffs(end) - 1 ? 0 : mine;
+        int incl            = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, off);
@@ -135,6 +137,9 @@ __device__ __forceinline__ bool find_item(int n, int x, F count, int &seg, int &
             seg         = base + l;
             item        = x - __shfl_sync(0xffffffffu, incl - mine, l);
             return true;
+        }
+        if (end) {
+            return false;
         }
         x -= __shfl_sync(0xffffffffu, incl, 31);
     }

@@ -451,8 +451,8 @@ ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *
  * they were, and rows of k and v outside a sequence never reach it, whatever
  * they hold; a NaN or an infinity in a sequence's own v may reach every query of
  * that sequence and head.  Offsets must not decrease: a sequence whose offsets do, or leave
- * the tensors, is left unwritten and raises device error 5
- * (acefa_device_error()).  nb[0] = the element size; data and nb[1..2] of q, k and
+ * the tensors, is left unwritten and raises device error 5 (acefa_device_error());
+ * where cu_q decreases, so are all sequences behind.  nb[0] = the element size; data and nb[1..2] of q, k and
  * v multiples of 16 bytes, not 0; dst aligned to its elements, its rows apart, and
  * apart from q, k and v.  rows_q and rows_kv up to 2^24, n_seq <= 65535,
  * Hq <= 4096.  No workspace.

@@ -90,3 +90,38 @@ def test_small_weights_of_packed_sequences(n, D, Hq, kind, out_kind, low, high):
     want = _sink_want(k[0, :, 0].double().numpy() * q0 * scale * LOG2E, v1[0, :, 0].double().numpy())
     tol = _sink_tol(want, n, 2.0 ** -17 * scale * q0 * 4 * high, torch.finfo(DT[kind]).eps / 2, out_kind)
     assert np.abs(out - want).max() <= tol, (np.abs(out - want).max(), want, tol)
+
+
+# ------------------------------------------------------------------ offsets that fall back
+@pytest.mark.parametrize("rows", [512, 6100])  # few rows, many rows
+@pytest.mark.parametrize("empty", [0, 31, 40, 100])  # sequences ahead, of no rows
+def test_packed_sequences_behind_falling_offsets_are_left_out(rows, empty):
+    """Offsets that fall and rise again would give rows to two sequences: the first keeps them, whole."""
+    D, a = 64, 500
+    r = np.random.default_rng([rows, empty])
+    q, k, v = (torch.from_numpy(r.standard_normal((h, n, D)).astype(np.float32)).half()
+               for h, n in ((2, rows), (1, 900), (1, 900)))
+    out = torch.full((rows, 2, D), 5.0, dtype=torch.float16, device="cuda")
+    cu_q = [0] * empty + [0, a, 0, a, a + 9]
+    cu_k = [0] * empty + [0, 300, 300, 900, 900]  # (the third sequence has keys of its own)
+    acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu_q), _i32(cu_k), out=out)
+    assert acefa.device_error() == 5 and acefa.device_error() == 0
+    alone = acefa.flash_attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32([0, a]), _i32([0, 300]))
+    assert torch.equal(out[:a], alone[:a]) and (out[a:] == 5.0).all()
+    qn, kn, vn = (x.double().numpy() for x in (q, k, v))
+    want = ref.packed(qn, kn, vn, [0, a], [0, 300], 0, 0, D ** -0.5)[:a]
+    A = D ** -0.5 * float(np.abs(qn).max((0, 1)) @ np.abs(kn).max((0, 1)))
+    u = torch.finfo(torch.float16).eps / 2  # of the weights, and of the output
+    tol = (u + 2 * (2.0 ** -17 * A + 2.0 ** -20)) * np.abs(vn).max() + u * np.abs(want)
+    assert (np.abs(out[:a].double().cpu().numpy() - want) <= tol).all()
+
+
+def test_packed_sequence_whose_key_offsets_fall_is_the_only_one_left_out():
+    D, cu_q, cu_k = 64, [0, 10, 30, 60], [50, 40, 90, 100]
+    r = np.random.default_rng(3)
+    q, k, v = (torch.from_numpy(r.standard_normal((1, 100, D)).astype(np.float32)).half().cuda() for _ in range(3))
+    out = torch.full((100, 1, D), 5.0, dtype=torch.float16, device="cuda")
+    acefa.flash_attn_packed(q, k, v, _i32(cu_q), _i32(cu_k), out=out)
+    assert acefa.device_error() == 5
+    good = acefa.flash_attn_packed(q[:, 10:], k, v, _i32([0, 20, 50]), _i32([40, 90, 100]))
+    assert torch.equal(out[10:60], good[:50]) and (out[:10] == 5.0).all() and (out[60:] == 5.0).all()
