@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv8_move_kernel(const __grid_con
         for (int p = 0; p < kPass; ++p) {
             const int   r = r0 + p * kRows;
             const float d = i ? s_d[r].y : s_d[r].x;
-            if (d != d_new[i]) {
+            if (d < d_new[i]) {  // (not beside a NaN scale: its block's rows keep their bytes, places without a row 0)
                 const float ratio = i ? s_ratio[r].y : s_ratio[r].x;
                 w[i][p].x = requant4(w[i][p].x, d, d_new[i], ratio);
                 w[i][p].y = requant4(w[i][p].y, d, d_new[i], ratio);

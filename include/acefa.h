@@ -421,9 +421,10 @@ ACEFA_API size_t acefa_kv8_attn_workspace_bytes(const acefa_tensor *q, const ace
  * (-0 equals 0; a NaN ranks below every number).  A set of at most keep rows
  * keeps them all.  A block of `out` takes the largest scale of the rows that
  * come into it; rows of that scale move unchanged, the others become
- * q * d_old / d rounded once to the nearest integer, ties to even.  Behind
- * len_out, up to keep, `kept` is -1 and rows, their blocks' scales and
- * weight_out are 0.
+ * q * d_old / d rounded once to the nearest integer, ties to even.  A NaN scale
+ * counts as the largest, and all rows that meet it move unchanged.  Behind
+ * len_out, up to keep, `kept` is -1 and rows, scales of blocks without a row
+ * and weight_out are 0.
  */
 ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *weight, const int32_t *len,
                               int64_t n_first, int64_t n_recent, const acefa_kv8_cache *out,

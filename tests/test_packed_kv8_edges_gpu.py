@@ -125,3 +125,25 @@ def test_packed_sequence_whose_key_offsets_fall_is_the_only_one_left_out():
     assert acefa.device_error() == 5
     good = acefa.flash_attn_packed(q[:, 10:], k, v, _i32([0, 20, 50]), _i32([40, 90, 100]))
     assert torch.equal(out[10:60], good[:50]) and (out[:10] == 5.0).all() and (out[60:] == 5.0).all()
+
+
+# ------------------------------------------------------------------ eviction beside blocks that are no number
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_evict_moves_rows_of_a_nan_block_unchanged_and_zeros_the_rest(D, side):
+    """A block of the smaller cache that takes a row whose scale is NaN gets that scale; its rows keep their
+    integers, and rows behind the length are 0 like in any other block."""
+    r = np.random.default_rng([D, len(side)])
+    sets, H, n, keep = 2, 2, 200, 128
+    q = [r.integers(-127, 128, (sets, H, n, D), dtype=np.int8) for _ in range(2)]
+    s = [r.random((sets, H, 4)).astype(np.float32) + 0.1 for _ in range(2)]
+    s["kv".index(side)][:, :, 1] = np.nan
+    w = r.random((sets, H, n)).astype(np.float32)
+    lens = [100, 200]
+    cache = acefa.Kv8Cache(*(torch.from_numpy(x).cuda() for x in (*q, *s)))
+    out, kept, lo, _ = acefa.kv8_evict(cache, torch.from_numpy(w).cuda(), _i32(lens), keep, 3, 20)
+    for i, (tq, ts) in enumerate(((out.k, out.k_scale), (out.v, out.v_scale))):
+        wq, ws, wk, wl, _ = ref.evict(q[i], s[i], w, lens, keep, 3, 20)
+        assert np.array_equal(kept.cpu().numpy(), wk) and np.array_equal(lo.cpu().numpy(), wl)
+        assert np.array_equal(ts.cpu().numpy(), ws, equal_nan=True)
+        assert np.array_equal(tq.cpu().numpy(), wq)
