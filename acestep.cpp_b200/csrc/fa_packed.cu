@@ -1193,6 +1193,41 @@ bool use_small(int64_t rows_q, int64_t rows_kv, int64_t Hq, int64_t D, int n_seq
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// The rows of a tensor on the host: `rows` x `heads` pieces of `bytes`.
+struct Pieces {
+    int64_t at, bytes, rows, row_nb, heads, head_nb;
+
+    int64_t end() const { return at + (rows - 1) * row_nb + (heads - 1) * head_nb + bytes; }
+};
+
+// Whether a and b share an address.  Tensors whose rows are the same distance
+// apart may lie in one buffer (the projections of a row and its output behind one
+// another); with other distances their extents have to be apart.
+bool meet(Pieces a, Pieces b) {
+    if (!a.rows || !b.rows || a.at >= b.end() || b.at >= a.end()) {
+        return false;
+    }
+    a.row_nb = a.rows > 1 ? a.row_nb : b.row_nb;
+    b.row_nb = b.rows > 1 ? b.row_nb : a.row_nb;
+    if (a.row_nb != b.row_nb) {
+        return true;
+    }
+    const int64_t step = a.rows > 1 || b.rows > 1 ? a.row_nb : 1ll << 62;
+    auto          floor_div = [](int64_t n, int64_t d) { return n / d - (n % d < 0); };
+    for (int64_t i = 0; i < a.heads; ++i) {
+        for (int64_t j = 0; j < b.heads; ++j) {
+            // row r of a meets row r + d of b where d * step lies in (gap - b.bytes, gap + a.bytes)
+            const int64_t gap = a.at + i * a.head_nb - b.at - j * b.head_nb;
+            const int64_t lo  = std::max(floor_div(gap - b.bytes, step) + 1, 1 - a.rows);
+            const int64_t hi  = std::min(-floor_div(-(gap + a.bytes), step) - 1, b.rows - 1);
+            if (lo <= hi) {
+                return true;
+            }
+        }
+    }
+    return false;
+}
+
 }  // namespace
 }  // namespace acefa
 
@@ -1244,6 +1279,13 @@ extern "C" ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const ac
     if ((Hq > 1 && heads < row) || (rows_q > 1 && rows < row) ||
         (Hq > 1 && rows_q > 1 && rows < heads * (size_t) Hq && heads < rows * (size_t) rows_q)) {
         return ACEFA_ERR_LAYOUT;
+    }
+    // nor on the rows of q, k and v
+    const Pieces out = {(int64_t) (uintptr_t) dst->data, (int64_t) row, rows_q, (int64_t) rows, Hq, (int64_t) heads};
+    for (const acefa_tensor *t : {q, k, v}) {
+        if (meet(out, {(int64_t) (uintptr_t) t->data, 2 * D, t->ne[1], (int64_t) t->nb[1], t->ne[2], (int64_t) t->nb[2]})) {
+            return ACEFA_ERR_LAYOUT;
+        }
     }
     DeviceCtx ctx;
     const int rc = device_ctx(&ctx);

@@ -455,7 +455,8 @@ ACEFA_API int acefa_kv8_evict(const acefa_kv8_cache *cache, const acefa_tensor *
  * the tensors, is left unwritten and raises device error 5 (acefa_device_error());
  * where cu_q decreases, so are all sequences behind.  nb[0] = the element size; data and nb[1..2] of q, k and
  * v multiples of 16 bytes, not 0; dst aligned to its elements, its rows apart, and
- * apart from q, k and v.  rows_q and rows_kv up to 2^24, n_seq <= 65535,
+ * apart from q, k and v (in one buffer with them only where all rows are the same
+ * distance apart).  rows_q and rows_kv up to 2^24, n_seq <= 65535,
  * Hq <= 4096.  No workspace.
  */
 ACEFA_API int acefa_flash_attn_packed(const acefa_tensor *q, const acefa_tensor *k, const acefa_tensor *v,

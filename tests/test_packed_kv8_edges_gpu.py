@@ -147,3 +147,18 @@ def test_evict_moves_rows_of_a_nan_block_unchanged_and_zeros_the_rest(D, side):
         assert np.array_equal(kept.cpu().numpy(), wk) and np.array_equal(lo.cpu().numpy(), wl)
         assert np.array_equal(ts.cpu().numpy(), ws, equal_nan=True)
         assert np.array_equal(tq.cpu().numpy(), wq)
+
+
+# ------------------------------------------------------------------ one buffer
+@pytest.mark.parametrize("rows", [100, 3100])
+def test_packed_output_beside_the_projections_in_one_buffer(rows):
+    """(rows, Hq + 2 Hkv + Hq, D): the output's heads behind the row's projections."""
+    D, Hq, H = 64, 4, 2
+    r = np.random.default_rng(rows)
+    x = torch.from_numpy(r.standard_normal((rows, 2 * Hq + 2 * H, D)).astype(np.float32)).half().cuda()
+    q, k, v = (x[:, a:b].transpose(0, 1) for a, b in ((0, Hq), (Hq, Hq + H), (Hq + H, Hq + 2 * H)))
+    before, cu = x.clone(), _i32([0, 37, 100])
+    want = acefa.flash_attn_packed(*(t.contiguous() for t in (q, k, v)), cu, mask=1)
+    acefa.flash_attn_packed(q, k, v, cu, mask=1, out=x[:, Hq + 2 * H:])
+    assert torch.equal(x[:100, Hq + 2 * H:], want[:100])
+    assert torch.equal(x[:, :Hq + 2 * H], before[:, :Hq + 2 * H]) and torch.equal(x[100:], before[100:])
