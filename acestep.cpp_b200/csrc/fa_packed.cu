@@ -93,7 +93,7 @@ struct Seq {
     bool bad, end;
 };
 __device__ __forceinline__ Seq seq_of(const PackedParams &P, int s) {
-    const int a = __ldg(P.cu_q + s), b = __ldg(P.cu_q + s + 1), c = __ldg(P.cu_k + s), d = __ldg(P.cu_k + s + 1);
+    const int a = P.cu_q[s], b = P.cu_q[s + 1], c = P.cu_k[s], d = P.cu_k[s + 1];
     Seq       r = {a, b - a, c, d - c, false, false};
     if (a < 0 || b < a || b > P.rows_q || c < 0 || d < c || d > P.rows_kv) {
         r = {0, 0, 0, 0, true, b < a};
@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid
         const char *p = S.q + (int64_t) (q.q0 + row0 + r) * S.q_nb1 + h * S.q_nb2 + 16 * c;
 #pragma unroll
         for (int e = 0; e < HD / 32; ++e) {
-            const uint4 w = r < n_row ? __ldg(reinterpret_cast<const uint4 *>(p + 64 * e)) : make_uint4(0u, 0u, 0u, 0u);
+            const uint4 w = r < n_row ? *reinterpret_cast<const uint4 *>(p + 64 * e) : make_uint4(0u, 0u, 0u, 0u);
             qf[nt][2 * e][0] = w.x, qf[nt][2 * e][1] = w.y, qf[nt][2 * e + 1][0] = w.z, qf[nt][2 * e + 1][1] = w.w;
         }
     }
@@ -989,7 +989,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid
             const int j = j0 + g + 8 * r;
 #pragma unroll
             for (int e = 0; e < HD / 32; ++e) {
-                kw[r][e] = j < q.n_k ? __ldg(reinterpret_cast<const uint4 *>(kb + j * S.k_nb1 + 64 * e))
+                kw[r][e] = j < q.n_k ? *reinterpret_cast<const uint4 *>(kb + j * S.k_nb1 + 64 * e)
                                      : make_uint4(0u, 0u, 0u, 0u);
             }
         }
@@ -998,7 +998,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid
             const int j = j0 + 2 * c + (r & 1) + 8 * (r >> 1);
 #pragma unroll
             for (int e = 0; e < HD / 64; ++e) {
-                vw[r][e] = j < q.n_k ? __ldg(reinterpret_cast<const uint4 *>(vb + j * S.v_nb1 + 16 * e))
+                vw[r][e] = j < q.n_k ? *reinterpret_cast<const uint4 *>(vb + j * S.v_nb1 + 16 * e)
                                      : make_uint4(0u, 0u, 0u, 0u);
             }
         }

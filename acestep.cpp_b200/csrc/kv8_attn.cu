@@ -214,7 +214,7 @@ __device__ __forceinline__ void tile_table(int *base, int *lens, const int32_t *
     if (threadIdx.x < 32) {
         int acc = 0;
         for (int b0 = 0; b0 < B; b0 += 32) {
-            const int n = b0 + lane < B ? clamp_len(__ldg(len + b0 + lane), n_max) : 0;
+            const int n = b0 + lane < B ? clamp_len(len[b0 + lane], n_max) : 0;
             int       v = n ? (n + kKv8Block - 1) / kKv8Block + kUnitCost : 0;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         const int unit = (int) blockIdx.x / P.cluster, rank = (int) blockIdx.x - unit * P.cluster;
         at.b   = unit / HU;
         at.ub  = unit - at.b * HU;
-        at.len = clamp_len(__ldg(P.len + at.b), P.c.n_max);
+        at.len = clamp_len(P.len[at.b], P.c.n_max);
         at.nt  = (at.len + kKv8Block - 1) / kKv8Block;
         at.t = at.at = run_start(at.nt, P.cluster, rank);
         x1           = run_start(at.nt, P.cluster, rank + 1);

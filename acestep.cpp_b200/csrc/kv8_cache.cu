@@ -29,10 +29,10 @@ struct SetRows {
 };
 __device__ __forceinline__ SetRows set_rows(const Kv8StoreParams &P, int s) {
     SetRows r;
-    r.pos = __ldg(P.pos + s);
+    r.pos = P.pos[s];
     if (P.cu) {
-        r.first         = __ldg(P.cu + s);
-        const int end   = __ldg(P.cu + s + 1);
+        r.first         = P.cu[s];
+        const int end   = P.cu[s + 1];
         r.bad           = r.first < 0 || end < r.first || end > (int) P.rows;
         r.count         = r.bad ? 0 : end - r.first;
     } else {
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kThreads) kv8_load_kernel(const __grid_constan
     const int      blk = blockIdx.x, h = blockIdx.y, s = blockIdx.z >> 1;
     const Kv8Rows &dst  = (blockIdx.z & 1) ? P.v : P.k;
     const Kv8Side &side = (blockIdx.z & 1) ? P.c.v : P.c.k;
-    const int      len  = min(clamp_len(__ldg(P.len + s), P.c.n_max), P.n);
+    const int      len  = min(clamp_len(P.len[s], P.c.n_max), P.n);
     const int      lo   = blk * kKv8Block;
     const int      r0 = threadIdx.x / kLanes, e0 = 4 * (threadIdx.x % kLanes);
     const int8_t  *qb = side.q + (int64_t) lo * side.nb1 + h * side.nb2 + s * side.nb3;

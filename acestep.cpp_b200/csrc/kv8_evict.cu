@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) kv8_select_kernel(const __grid
     pdl_wait_primary();
     const int    h = blockIdx.x, b = blockIdx.y;
     const int    tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int    len  = clamp_len(__ldg(P.len + b), P.c.n_max);
+    const int    len  = clamp_len(P.len[b], P.c.n_max);
     const int    kept = min(len, P.keep);
     const float *w    = reinterpret_cast<const float *>(P.weight + h * P.w_nb2 + b * P.w_nb3);
     int32_t     *out  = reinterpret_cast<int32_t *>(P.kept + h * P.k_nb2 + b * P.k_nb3);
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) kv8_select_kernel(const __grid
         float v[K];
 #pragma unroll
         for (int i = 0; i < K; ++i) {  // all on their way together
-            v[i] = r0 + 32 * i + lane < r1 ? __ldg(w + r0 + 32 * i + lane) : 0.0f;
+            v[i] = r0 + 32 * i + lane < r1 ? w[r0 + 32 * i + lane] : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < K; ++i) {
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) kv8_select_kernel(const __grid
             float v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[e] = x + e * 32 < r1 ? __ldg(w + x + e * 32) : 0.0f;
+                v[e] = x + e * 32 < r1 ? w[x + e * 32] : 0.0f;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) kv8_select_kernel(const __grid
 #pragma unroll 4
             for (int i = 0; i < steps; ++i) {
                 const int x = r0 + 32 * i + lane;
-                f(x, x < r1 ? (K == kShared ? s_key[x] : order_key(__ldg(w + x))) : 0u);
+                f(x, x < r1 ? (K == kShared ? s_key[x] : order_key(w[x])) : 0u);
             }
         }
     };

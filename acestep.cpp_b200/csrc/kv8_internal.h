@@ -95,7 +95,9 @@ inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows 
 #ifdef __CUDACC__
 
 // Launches a kernel that begins with pdl_wait_primary(): its blocks are set up
-// while the stream's previous kernel ends, and wait there until it has.  Measured,
+// while the stream's previous kernel ends, and wait there until it has.  What they
+// read may still be written while they wait, so no load of theirs may go the
+// read-only way (__ldg), which wants data that is constant from the kernel's start.  Measured,
 // back to back: 0.2 us of a call of few rows, 0.3 of a store and of an eviction's
 // kernels each.  (Letting the next kernel start earlier, behind that wait, cost time:
 // store + load of one token 4.6 -> 5.2 us, eviction 15.7 -> 16.7, packed prompts 78 -> 81.)

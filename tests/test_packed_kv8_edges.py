@@ -1,7 +1,9 @@
 """CPU tests of the packed and 8-bit-cache entries at the edges of what they accept."""
 import ctypes
 import itertools
+import os
 import random
+import re
 
 import pytest
 import torch
@@ -128,3 +130,16 @@ def test_packed_output_of_any_layout_against_every_address():
         assert (got == -4) == meets and (meets or got in ACCEPTED), (rows, kv_rows, H, step, head)
         seen[meets] += 1
     assert min(seen.values()) > 50
+
+
+# ------------------------------------------------------------------ launches beside the previous kernel
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "acestep.cpp_b200", "csrc")
+
+
+@pytest.mark.parametrize("name", ["fa_packed.cu", "kv8_attn.cu", "kv8_cache.cu", "kv8_evict.cu", "kv8_internal.h"])
+def test_kernels_set_up_early_read_nothing_as_constant(name):
+    """They run while the previous kernel may still write their inputs and wait for its end; a read-only load
+    (__ldg, ld.global.nc, a const __restrict__ argument) says that its data does not change in all that time."""
+    with open(os.path.join(CSRC, name)) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert not re.search(r"__ldg\s*\(|ld\.global[.\w]*\.nc|__restrict__", code)
