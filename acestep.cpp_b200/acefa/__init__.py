@@ -646,7 +646,8 @@ class Kv8Attn(_Call):
 class Kv8Evict(_Call):
     """acefa_kv8_evict: kept.shape[2] rows of each (set, head) of cache move to out, the first n_first, the last
     n_recent and the largest of weight (sets, Hkv, n_max) f32.  kept (sets, Hkv, keep) int32, lens_out (sets) int32
-    and weight_out (sets, Hkv, keep) f32 or None are written."""
+    and weight_out (sets, Hkv, keep) f32 or None are written.  out may have more than keep rows and weight_out be
+    the first of a longer array: what lies behind stays as it is (sets that go on growing there want weights of 0)."""
 
     def __init__(self, cache, weight, lens, out, kept, lens_out, weight_out=None, n_first=0, n_recent=0):
         n = cache.k.shape[0]
@@ -707,15 +708,18 @@ def kv8_attn(q, cache, lens, scale=None, weight=None, out=None, stream=None):
         return Kv8Attn(q, cache, lens, scale=scale, weight=weight, out=out)(stream)
 
 
-def kv8_evict(cache, weight, lens, keep, n_first=0, n_recent=0, stream=None):
-    """Returns (cache of keep rows, kept, lens, weights) of the rows that stay."""
+def kv8_evict(cache, weight, lens, keep, n_first=0, n_recent=0, stream=None, n_max=None):
+    """Returns (cache, kept, lens, weights) of the rows that stay.  The cache and the weights have n_max rows
+    (default: keep, so that a set which was shrunk is full); kv8_store goes on at lens, and the weights
+    behind keep are 0."""
     B, H, _, D = cache.k.shape
+    n_max = keep if n_max is None else n_max
     with _on(stream):
-        out = Kv8Cache.empty(keep, H, B, D, device=cache.k.device)
+        out = Kv8Cache.empty(n_max, H, B, D, device=cache.k.device)
         kept = torch.empty((B, H, keep), dtype=torch.int32, device=cache.k.device)
-        weight_out = torch.empty((B, H, keep), device=cache.k.device)
+        weight_out = (torch.zeros if n_max > keep else torch.empty)((B, H, n_max), device=cache.k.device)
         lens_out = torch.empty(B, dtype=torch.int32, device=cache.k.device)
-        Kv8Evict(cache, weight, lens, out, kept, lens_out, weight_out=weight_out, n_first=n_first,
+        Kv8Evict(cache, weight, lens, out, kept, lens_out, weight_out=weight_out[..., :keep], n_first=n_first,
                  n_recent=n_recent)(stream)
     return out, kept, lens_out, weight_out
 

@@ -412,10 +412,14 @@ ACEFA_API size_t acefa_kv8_attn_workspace_bytes(const acefa_tensor *q, const ace
  *   len         int32 [Bk], device: rows in each set
  *   n_first, n_recent  the first and the last rows that are kept whatever
  *               their weight (n_first + n_recent <= keep)
- *   out         the smaller cache, keep <= its n_max, same D, Hkv and Bk; must
- *               not overlap `cache`
+ *   out         the cache of the rows that stay, keep <= its n_max, same D, Hkv
+ *               and Bk; must not overlap `cache`.  Rows behind keep stay as they
+ *               are: with a longer n_max acefa_kv8_store goes on at len_out (with
+ *               n_max == keep a set that was shrunk is full)
  *   kept        I32 [keep, Hkv, Bk], nb[0] == 4: the kept rows, ascending
- *   weight_out  F32 [keep, Hkv, Bk], nb[0] == 4, or NULL: their weights
+ *   weight_out  F32 [keep, Hkv, Bk], nb[0] == 4, or NULL: their weights (also as
+ *               the first rows of an [n_max, Hkv, Bk] array for acefa_kv8_attn,
+ *               whose rows behind keep the caller clears before it goes on)
  *   len_out     int32 [Bk], device: min(len, keep)
  * The other places go to the largest weights, equal ones to the lower row
  * (-0 equals 0; a NaN ranks below every number).  A set of at most keep rows

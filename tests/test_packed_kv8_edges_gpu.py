@@ -162,3 +162,55 @@ def test_packed_output_beside_the_projections_in_one_buffer(rows):
     acefa.flash_attn_packed(q, k, v, cu, mask=1, out=x[:, Hq + 2 * H:])
     assert torch.equal(x[:100, Hq + 2 * H:], want[:100])
     assert torch.equal(x[:, :Hq + 2 * H], before[:, :Hq + 2 * H]) and torch.equal(x[100:], before[100:])
+
+
+# ------------------------------------------------------------------ a loop that goes on behind evictions
+@pytest.mark.parametrize("D,keep,n_max", [(128, 100, 150), (64, 64, 130), (64, 70, 71)])
+def test_decode_goes_on_in_the_evicted_cache(D, keep, n_max):
+    """Steps of store + attend with weights; whenever a set is full, an eviction to a cache of the same length."""
+    r = np.random.default_rng([D, keep, n_max])
+    sets, H, G, evictions = 3, 2, 2, 0
+    cache = acefa.Kv8Cache.empty(n_max, H, sets, D)
+    weight = torch.zeros((sets, H, n_max), device="cuda")
+    lens = [n_max - 2, 5, n_max - 6]  # (prompts: the second stays below keep)
+    cq = [np.zeros((sets, H, n_max, D), np.int8) for _ in range(2)]
+    cs = [np.zeros((sets, H, -(-n_max // 64)), np.float32) for _ in range(2)]
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    x = [r.standard_normal((H, cu[-1], D)).astype(np.float32) for _ in range(2)]
+    acefa.kv8_store(cache, *(torch.from_numpy(t).cuda() for t in x), _i32([0] * sets), _i32(cu.tolist()))
+    for i in range(2):
+        cq[i], cs[i] = ref.store(cq[i], cs[i], x[i], [0] * sets, cu)
+    total = np.zeros((sets, H, n_max))
+    for _ in range(2 * (n_max - keep) + 6 if n_max - keep < 50 else 60):
+        if max(lens) == n_max:
+            evictions += 1
+            w32 = weight.cpu().numpy()
+            cache, kept, lo, weight = acefa.kv8_evict(cache, weight, _i32(lens), keep, 2, 10, n_max=n_max)
+            assert cache.k.shape[2] == n_max and weight.shape == (sets, H, n_max) and (weight[..., keep:] == 0).all()
+            for i in range(2):
+                cq[i], cs[i], wk, wl, ww = ref.evict(cq[i], cs[i], w32, lens, keep, 2, 10)
+                cq[i] = np.pad(cq[i], ((0, 0), (0, 0), (0, n_max - keep), (0, 0)))
+                cs[i] = np.pad(cs[i], ((0, 0), (0, 0), (0, -(-n_max // 64) - cs[i].shape[2])))
+            assert np.array_equal(kept.cpu().numpy(), wk) and np.array_equal(weight[..., :keep].cpu().numpy(), ww)
+            lens = wl.tolist()
+            assert lo.tolist() == lens
+            total = weight.double().cpu().numpy()
+        x = [r.standard_normal((H, sets, D)).astype(np.float32) for _ in range(2)]
+        acefa.kv8_store(cache, *(torch.from_numpy(t).cuda() for t in x), _i32(lens))
+        for i in range(2):
+            cq[i], cs[i] = ref.store(cq[i], cs[i], x[i], lens, np.arange(sets + 1))
+        lens = [a + 1 for a in lens]
+        qn = r.standard_normal((sets, H * G, 1, D)).astype(np.float32)
+        got = acefa.kv8_attn(torch.from_numpy(qn).cuda(), cache, _i32(lens), weight=weight).double().cpu().numpy()
+        k, v = ref.values(cq[0], cs[0]), ref.values(cq[1], cs[1])
+        want, w = ref.attend(qn.astype(np.float64), k, v, lens, D ** -0.5)
+        total += w
+        # a score is off by e, a weight by 2e + 2^-20 of itself, F32 sums of V by 2^-18, of weights by 2^-24 a step
+        A = D ** -0.5 * max(float(np.abs(qn[b]).reshape(-1, D).max(0) @ np.abs(k[b]).reshape(-1, D).max(0)) for b in range(sets))
+        e = (2.0 ** -21 + D / 8 * 2.0 ** -23) * A
+        assert np.abs(got - want).max() <= (2 * e + 2.0 ** -18) * np.abs(v).max()
+    # the first set is full after 2 steps and again n_max - keep later (66 of 60 steps in the second case)
+    assert acefa.device_error() == 0 and evictions >= (2 if n_max - keep < 58 else 1)
+    rows = (np.arange(n_max) < np.array(lens)[:, None])[:, None]  # (64 sums of two weights at most)
+    gw = weight.double().cpu().numpy()
+    assert (np.abs(gw - total) <= (2 * e * 4 + 2.0 ** -20 + 128 * 2.0 ** -24) * total)[np.broadcast_to(rows, gw.shape)].all()
