@@ -214,3 +214,35 @@ def test_decode_goes_on_in_the_evicted_cache(D, keep, n_max):
     rows = (np.arange(n_max) < np.array(lens)[:, None])[:, None]  # (64 sums of two weights at most)
     gw = weight.double().cpu().numpy()
     assert (np.abs(gw - total) <= (2 * e * 4 + 2.0 ** -20 + 128 * 2.0 ** -24) * total)[np.broadcast_to(rows, gw.shape)].all()
+
+
+# ------------------------------------------------------------------ Q and output of different types
+# Tolerance: a score is off by at most e = (2^-21 + D / 8 * 2^-23) * A, a weight by 2e + 2^-20 of itself, where Q and
+# the output both have 16 bits by its rounding to 11 too (2^-11); sums lose 2^-18; then half a step of the output.
+@pytest.mark.parametrize("weigh", [False, True])
+@pytest.mark.parametrize("kind,out_kind", [(a, b) for a in DT for b in DT if a != b])
+@pytest.mark.parametrize("D,Hq,H,n_q,lens,n_max", [
+    (128, 4, 2, 1, [300, 0, 77], 320), (64, 8, 1, 1, [130], 130), (128, 16, 1, 1, [500, 64], 512), (64, 6, 2, 5, [65, 700], 704),
+    (128, 2, 1, 1, [4000], 4096), (128, 24, 1, 2, [5000], 5000), (64, 12, 1, 1, [6001, 3], 6001)])
+def test_attend_with_mixed_types(D, Hq, H, n_q, lens, n_max, kind, out_kind, weigh):
+    r = np.random.default_rng([D, Hq, n_q, n_max])
+    sets, nb = len(lens), -(-n_max // 64)
+    q8 = [r.integers(-127, 128, (sets, H, n_max, D), dtype=np.int8) for _ in range(2)]
+    s = [(r.random((sets, H, nb)).astype(np.float32) + 0.5) / 64 for _ in range(2)]
+    cache = acefa.Kv8Cache(*(torch.from_numpy(x).cuda() for x in (*q8, *s)))
+    q = torch.from_numpy(r.standard_normal((sets, Hq, n_q, D)).astype(np.float32)).to(DT[kind])
+    out = torch.empty((sets, n_q, Hq, D), dtype=DT[out_kind], device="cuda")
+    weight = torch.zeros((sets, H, n_max), device="cuda") if weigh else None
+    acefa.kv8_attn(q.cuda(), cache, _i32(lens), weight=weight, out=out)
+    qn, k, v = q.double().numpy(), ref.values(q8[0], s[0]), ref.values(q8[1], s[1])
+    want, ww = ref.attend(qn, k, v, lens, D ** -0.5)
+    A = D ** -0.5 * max(float(np.abs(qn[b]).reshape(-1, D).max(0) @ np.abs(k[b]).reshape(-1, D).max(0)) for b in range(sets))
+    e = (2.0 ** -21 + D / 8 * 2.0 ** -23) * A
+    u = 0.0 if "f32" in (kind, out_kind) else 2.0 ** -11
+    tol = (2 * e + 2.0 ** -18 + u) * np.abs(v).max() + torch.finfo(DT[out_kind]).eps / 2 * np.abs(want)
+    got = out.double().cpu().numpy()
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) - tol).max()
+    if weigh:
+        rows = Hq // H * n_q
+        gw = weight.double().cpu().numpy()
+        assert (np.abs(gw - ww) <= (2 * e + 2.0 ** -20 + (rows + 1) * 2.0 ** -24) * ww).all()
