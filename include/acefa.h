@@ -326,7 +326,10 @@ ACEFA_API int acefa_cfg_logit_combine(const float *cond, const float *uncond, in
  *   k[d, j, h, s] * k_scale[j / 64, h, s]         (each product rounded to F32)
  * and likewise for v.  k, v: I8 [D, n_max, Hkv, Bk], D 64 or 128, nb[0] == 1,
  * data and nb[1..3] multiples of 16 bytes, not 0; k_scale, v_scale: F32
- * [ceil(n_max / 64), Hkv, Bk], nb[0] == 4.  1 <= Bk <= ACEFA_KV8_MAX_SETS,
+ * [ceil(n_max / 64), Hkv, Bk], nb[0] == 4.  A value is off by at most half its
+ * block's scale when it is stored, and by half the new scale whenever that
+ * grows: coarser than Q8_0 with its scale per 32 values (a root mean square of 0.9 %
+ * of normal rows stored at once and 1.2 % one by one, Q8_0 0.5 %).  1 <= Bk <= ACEFA_KV8_MAX_SETS,
  * Hkv <= 4096.  A cache needs no initialisation: rows at or past a set's
  * length are never read as values.
  *
@@ -354,7 +357,8 @@ typedef struct acefa_kv8_cache {
  * values become x / d rounded to the nearest integer, ties to even (0 where
  * d is 0); where d grew, the rows that stay are rounded again: q * d_old / d.
  * Both quotients are rounded once, exactly.  A NaN or an infinity among the
- * new rows makes their block's scale NaN.  Rows of the last block behind the
+ * new rows makes their block's scale NaN, which it stays while a row of the
+ * block stays.  Rows of the last block behind the
  * new length are left as they are.  A set whose rows are no rows of the
  * cache or of k_new (a negative pos, an end past n_max, offsets that
  * decrease or leave [0, rows]) is left unwritten and raises device error 5

@@ -246,3 +246,64 @@ def test_attend_with_mixed_types(D, Hq, H, n_q, lens, n_max, kind, out_kind, wei
         rows = Hq // H * n_q
         gw = weight.double().cpu().numpy()
         assert (np.abs(gw - ww) <= (2 * e + 2.0 ** -20 + (rows + 1) * 2.0 ** -24) * ww).all()
+
+
+# ------------------------------------------------------------------ against the K and V that were stored
+@pytest.mark.parametrize("D,grow", [(64, False), (128, True)])
+def test_attention_over_the_cache_against_unquantised_keys_and_values(D, grow):
+    """Prompts at once, then 40 rows one by one.  A value is off by at most half a step of its scale when it is
+    stored and of the new scale whenever that grows: (1 + g) / 2 times the block's last scale after g growths.  A
+    score is then off by at most E = scale * sum_d |q_d| times that of K, the weights' ratios by exp(2E), and
+    the output by V's own error and (exp(2E) - 1) * max|v|; the kernel adds 2^-16 of max|v| (scores below 2)."""
+    r = np.random.default_rng([D, grow])
+    sets, H, n_max, steps, lens = 2, 2, 320, 40, [150, 230]
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    x = [r.standard_normal((H, cu[-1], D)).astype(np.float32) for _ in range(2)]
+    cache = acefa.Kv8Cache.empty(n_max, H, sets, D)
+    acefa.kv8_store(cache, *(torch.from_numpy(t).cuda() for t in x), _i32([0] * sets), _i32(cu.tolist()))
+    full = [np.zeros((sets, H, n_max, D)) for _ in range(2)]
+    for i in range(2):
+        for b, ln in enumerate(lens):
+            full[i][b, :, :ln] = x[i][:, cu[b]:cu[b + 1]]
+    growths = [np.zeros((sets, H, n_max // 64)) for _ in range(2)]
+    scales = lambda: [t.cpu().numpy().astype(np.float64) for t in (cache.k_scale, cache.v_scale)]  # noqa: E731
+    old = scales()
+    for t in range(steps):
+        y = [(r.standard_normal((H, sets, D)) * (1 + 0.05 * t * grow)).astype(np.float32) for _ in range(2)]
+        acefa.kv8_store(cache, *(torch.from_numpy(z).cuda() for z in y), _i32([ln + t for ln in lens]))
+        new = scales()
+        for i in range(2):
+            for b, ln in enumerate(lens):
+                full[i][b, :, ln + t] = y[i][:, b]
+                blk = (ln + t) // 64
+                growths[i][b, :, blk] += (new[i][b, :, blk] > old[i][b, :, blk]) & ((ln + t) % 64 != 0)
+        old = new
+    lens = [ln + steps for ln in lens]
+    assert not grow or max(g.max() for g in growths) > 3
+    off = [np.repeat((1 + growths[i]) / 2 * old[i] * (1 + 2.0 ** -20), 64, -1) for i in range(2)]
+    values = [t.double().cpu().numpy() for t in acefa.kv8_load(cache, _i32(lens))]
+    for i in range(2):
+        for b, ln in enumerate(lens):
+            assert (np.abs(values[i] - full[i])[b, :, :ln] <= off[i][b, :, :ln, None]).all()
+    q = (0.1 * r.standard_normal((sets, 2 * H, 1, D))).astype(np.float32)
+    got = acefa.kv8_attn(torch.from_numpy(q).cuda(), cache, _i32(lens)).double().cpu().numpy()
+    want, _ = ref.attend(q.astype(np.float64), *full, lens, D ** -0.5)
+    for b, ln in enumerate(lens):
+        E = D ** -0.5 * np.abs(q[b]).sum(-1).max() * off[0][b, :, :ln].max()
+        top = np.abs(full[1][b, :, :ln]).max() + off[1][b, :, :ln].max()
+        assert np.abs(got[b] - want[b]).max() <= off[1][b, :, :ln].max() + (np.expm1(2 * E) + 2.0 ** -16) * top
+
+
+def test_a_nan_scale_stays_while_rows_of_its_block_stay():
+    D, r = 64, np.random.default_rng(8)
+    cache = acefa.Kv8Cache.empty(128, 1, 1, D)
+    x = torch.from_numpy(r.standard_normal((1, 10, D)).astype(np.float32)).cuda()
+    bad = x.clone()
+    bad[0, 3, 5] = float("nan")
+    acefa.kv8_store(cache, bad, x, _i32([0]))
+    acefa.kv8_store(cache, x * 9, x, _i32([10]))
+    k, v = acefa.kv8_load(cache, _i32([20]))
+    assert torch.isnan(k[0, 0, :20]).all() and not torch.isnan(v).any()
+    acefa.kv8_store(cache, x, x, _i32([0]))  # the block anew: no row stays
+    k, _ = acefa.kv8_load(cache, _i32([10]))
+    assert not torch.isnan(k).any()
