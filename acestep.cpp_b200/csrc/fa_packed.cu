@@ -911,12 +911,6 @@ struct SmallParams {
     int64_t      q_nb1, q_nb2, k_nb1, k_nb2, v_nb1, v_nb2;  // row, head
 };
 
-__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(32 * kSmallWarps) fa_packed_small(const __grid_constant__ SmallParams S) {
     constexpr int NT = kSmallRows / 8, KS = HD / 16, kOut = HD + 4;

@@ -102,13 +102,6 @@ __device__ __forceinline__ uint2 lds_v2(uint32_t a) {
     asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
     return v;
 }
-// 8x8 b16 matrix spread over the warp (row = lane / 4, two columns each), transposed
-__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
 // Two bytes of `biased` (int8 + 128, picked by sel) as f16: 0x6400 | b is
 // 1024 + b, and subtracting 1152 leaves the int8 value exactly.
 __device__ __forceinline__ uint32_t i8x2_f16(uint32_t biased, uint32_t sel) {

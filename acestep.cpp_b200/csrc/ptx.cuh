@@ -227,6 +227,13 @@ __device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
     return d;
 }
 
+// 8x8 b16 matrix spread over the warp (row = lane / 4, two columns each), transposed
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 // Named barrier over a subset of warps (id 1..15; 0 is __syncthreads).
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
