@@ -31,10 +31,10 @@
 // dropped.  Every wait is bounded (error word and drain on expiry).
 //
 // Measured (B200): 4096 + 2751 + 1201 causal rows, 16 / 8 heads, D = 128, BF16:
-// 106-119 us, 890-1000 TFLOP/s of visible pairs, tensor pipe 53 % -- bound by the
+// 119-121 us, 870-890 TFLOP/s of visible pairs, tensor pipe 53 % -- bound by the
 // chain S -> softmax -> P -> O of each tile and the issuing thread's waits
 // (shared memory feeds the S products at its full 128 B per clock); 16 prompts of
-// 64 .. 1024 rows, 32 / 8 heads: 79 us, a third of it the units' beginnings and ends.
+// 64 .. 1024 rows, 32 / 8 heads: 88 us, a third of it the units' beginnings and ends.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -900,7 +900,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // 16 keys of every 64 and loads exactly its fragments' 16-B pieces of rows to
 // registers, products run transposed (S^T = K Q^T, O^T = V^T P^T; P changes layout by
 // movmatrix), and the warps' results meet once in shared memory.  Bound by latency:
-// 2.7-4.5 us up to 128 rows of 16 heads, where the kernel above takes 8.2.
+// 2.7-4.4 us up to 128 rows of 16 heads, where the kernel above takes 7.9.
 constexpr int   kSmallRows = 16;
 constexpr int   kSmallWarps = 4;
 constexpr float kNoMax = -1.7e38f;  // below every score, finite
@@ -1177,10 +1177,11 @@ int encode_rows(CUtensorMap *map, const acefa_tensor *t) {
 
 // The few-rows kernel?  It reads the keys again for every 16 rows of a head, so
 // its time grows with rows x heads x D; the tensor-memory kernel starts slowly.
-// Measured, few-rows against the other (us): one sequence of 16 / 128 / 256 rows,
-// 16 heads, D = 128: 3.8 : 8.4, 4.9 : 8.5, 7.8 : 10.5; 512 rows, 8 / 16 heads: 11.4 : 14.0,
-// 17.9 : 14.1; 256 rows, 32 heads: 12.9 : 10.8; 8 sequences of 578 rows in all, 8 / 16
-// heads: 9.2 : 10.7, 13.4 : 11.0; 512 rows, 16 heads, D = 64: 11.1 : 12.6.
+// Measured, few-rows against the other (us, causal, BF16, 100 calls in a graph): one
+// sequence of 1 / 16 / 128 / 256 rows, 16 heads, D = 128: 2.7 : 7.9, 3.3 : 7.8, 4.4 : 7.9, 7.4 : 9.9;
+// 512 rows, 8 / 16 heads: 10.9 : 13.4, 18.0 : 13.4; 256 rows, 32 heads: 12.5 : 10.1; 8 sequences of 578
+// rows in all, 8 / 16 heads: 7.7 : 9.7, 11.3 : 10.4; 512 rows, 16 heads, D = 64: 10.4 : 12.0; at the
+// rule's edge, 375 rows of 16 heads: 12.6 : 11.8.
 bool use_small(int64_t rows_q, int64_t rows_kv, int64_t Hq, int64_t D, int n_seq) {
     return rows_q * Hq * D <= 6000 * 128 && rows_kv <= 1024 && n_seq <= 1024;
 }

@@ -34,9 +34,9 @@
 // an equal share of its tiles, and the partial results meet in distributed shared
 // memory -- one launch, no table of the sets, no partials in HBM.
 // Measured (B200): 16 sets of up to 8192 rows, 8 KV heads, D = 128, BF16 rows:
-// 46 us, 5.4 TB/s in all and 6.9 TB/s between the first and the last tile (bound by
-// HBM and, closely, by the four warps' instructions: 0.70 us per tile and
-// CTA); 2 sets of 700 rows: 6 us, bound by the latencies of launch, Q and merge.
+// 47-51 us with the second launch, 4.9-5.2 TB/s in all and 6.9 TB/s between the first and
+// the last tile (bound by HBM and, closely, by the four warps' instructions: 0.70 us per
+// tile and CTA); 2 sets of 700 rows: 6 us, bound by the latencies of launch, Q and merge.
 // Products run transposed (keys or dims are the MMA's M, the rows its N = 8):
 // S^T = K Q^T and O^T = V^T P^T; P moves from the accumulator layout to the
 // operand layout by four movmatrix.  m_r moves only when a score exceeds the
@@ -296,6 +296,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         tile_table(s_base, s_len, P.len, P.c.B, P.c.n_max);
         const int T = s_base[P.c.B] * HU;
         const int C = min((int) gridDim.x, T);
+        // The sum kernel, always the next in the stream, may be set up from here on.  It reads the
+        // lengths before its own wait, which is sound only behind this one's pdl_wait_primary():
+        // whatever wrote them is complete.
         pdl_launch_dependents();
         if ((int) blockIdx.x >= C) {
             return;

@@ -12,7 +12,7 @@
 // F32, with 16 B or 4 B per lane and whole lines per warp.  Measured (B200): 8086
 // rows x 8 heads x 128 of K and V from F32 stored in 18-21 us (4.0-4.6 TB/s, bound by
 // instruction issue, 62 %), 16384 rows read back in 22.5 us (7.4 TB/s); both together
-// 40.7 us with 256 threads per block of rows, 42.5 with 128 and 48.6 with 512.
+// 40.9 us with 256 threads per block of rows (128: 42.5, 512: 48.6 against 40.7 then).
 #include "kv8_internal.h"
 #include "ptx.cuh"
 

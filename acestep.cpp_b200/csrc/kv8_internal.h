@@ -85,7 +85,10 @@ cudaError_t launch_kv8_evict(const Kv8EvictParams &p, cudaStream_t s);
 // Rows of a unit of the attention kernel and the CTAs that it may keep
 // resident on one SM; functions of the operands alone.  More than eight F32
 // rows go in units of eight that read the keys again (from L2): split Q
-// fragments of sixteen rows do not fit the registers of two CTAs per SM.
+// fragments of sixteen rows do not fit the registers of two CTAs per SM.  The
+// output's type is not known where the workspace is sized, so 16-bit rows with an
+// F32 output, which split too, stay in units of sixteen and spill (4 sets of 8192 rows,
+// 8 heads of 16 rows, D = 128: 36 us, from F32 rows 30, with a 16-bit output 23).
 inline int kv8_unit_rows(int rows, int q_type) { return rows <= 8 || q_type == ACEFA_TYPE_F32 ? 8 : 16; }
 int        kv8_attn_ctas_per_sm();
 int        kv8_attn_cluster(const Kv8AttnParams &p, int64_t units, int sm_count);
@@ -97,7 +100,9 @@ inline size_t kv8_slot_floats(int D, int unit_rows) { return (size_t) unit_rows 
 // Launches a kernel that begins with pdl_wait_primary(): its blocks are set up
 // while the stream's previous kernel ends, and wait there until it has.  What they
 // read may still be written while they wait, so no load of theirs may go the
-// read-only way (__ldg), which wants data that is constant from the kernel's start.  Measured,
+// read-only way (__ldg), which wants data that is constant from the kernel's start.  One
+// exception reads before its wait: kv8_attn_sum_kernel takes the lengths, which the kernel
+// ahead of it (kv8_attn_kernel, which lets it start) has waited for.  Measured,
 // back to back: 0.2 us of a call of few rows, 0.3 of a store and of an eviction's
 // kernels each.  (Letting the next kernel start earlier, behind that wait, cost time:
 // store + load of one token 4.6 -> 5.2 us, eviction 15.7 -> 16.7, packed prompts 78 -> 81.)

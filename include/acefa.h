@@ -87,7 +87,9 @@ typedef struct acefa_tensor {
  *
  * scale, max_bias (ALiBi) and logit_softcap have ggml's meaning.  prec is
  * accepted for either value; accumulation is always F32.  stream is a
- * cudaStream_t (NULL = legacy default stream).  workspace must hold
+ * cudaStream_t (NULL = legacy default stream); a kernel directly ahead on it
+ * that lets its dependents start early (programmatic launch) writes q, masks and
+ * positions before it does so.  workspace must hold
  * acefa_workspace_bytes() bytes, 256-B aligned, caller-owned; its contents need
  * no initialisation and are dead after the call's kernels finish.
  * Returns ACEFA_OK or a negative acefa_status; launches nothing on error.
@@ -389,13 +391,14 @@ ACEFA_API int acefa_kv8_load(const acefa_kv8_cache *cache, const int32_t *len, c
  *   weight  F32 [n_max, Hkv, Bk], nb[0] == 4, or NULL
  * Query i sees rows j < len - (n_q - 1 - i) of its set.  dst = softmax(scale *
  * q k^T) v; a query that sees nothing gives 0, and a block whose scale is NaN
- * reaches only the queries that see one of its rows.  With `weight`, weight[j, h, s]
+ * reaches only the queries that see one of its rows.  dst and weight lie apart
+ * from one another, from q and from the cache.  With `weight`, weight[j, h, s]
  * grows by the softmax weights of row j summed over the n_q * Hq / Hkv
  * queries of its head -- what acefa_kv8_evict goes by; rows at or past
  * len[s] are left alone.  Q enters whole and all sums are F32.  The softmax
  * weights that multiply V are rounded to 22 bits, or to 11 (F16) where q and dst
  * both have 16-bit types, and to steps of 2^-32 of the row's largest; those that
- * `weight` receives are F32.
+ * `weight` receives are F32 (a NaN in q makes those of its head NaN).
  * Results do not depend on the order in which the GPU runs the blocks.
  * workspace: acefa_kv8_attn_workspace_bytes(), 256-B aligned, no
  * initialisation; a function of shapes and the device only.  Calls that may
@@ -507,11 +510,14 @@ ACEFA_API int acefa_device_error(void *stream);
 /* Human-readable name of an acefa_status. */
 ACEFA_API const char *acefa_status_string(int status);
 
-/* Kernel-launch count of the last successful acefa_flash_attn_ext call on this
- * host thread (1 to 3: mask classification, attention, split-KV combine). */
+/* Kernel-launch count of the last successful call on this host thread:
+ * acefa_flash_attn_ext 1 to 3 (mask classification, attention, split-KV
+ * combine), acefa_flash_attn_packed, acefa_kv8_store and acefa_kv8_load 1,
+ * acefa_kv8_attn 1 or 2, acefa_kv8_evict 2; calls without rows 0. */
 ACEFA_API int acefa_last_launch_count(void);
 
-/* Which kernel family served the last successful call on this thread:
+/* Which kernel family served the last successful attention call on this thread
+ * (acefa_kv8_store, _load, _evict and calls without rows leave it as it was):
  * 1 = split-KV decode (mma.sync), 2 = dense tcgen05/TMEM, 3 = packed sequences
  * (tcgen05/TMEM, few rows mma.sync), 4 = decode over an 8-bit block-scaled cache. */
 ACEFA_API int acefa_last_path(void);
