@@ -307,3 +307,59 @@ def test_a_nan_scale_stays_while_rows_of_its_block_stay():
     acefa.kv8_store(cache, x, x, _i32([0]))  # the block anew: no row stays
     k, _ = acefa.kv8_load(cache, _i32([10]))
     assert not torch.isnan(k).any()
+
+
+# ------------------------------------------------------------------ the same bits again
+@pytest.mark.parametrize("lens,Hq,H,D,kind", [([1200, 700, 41], 6, 2, 128, "bf16"), ([70, 9, 130], 4, 4, 64, "f16"),
+                                              ([65 + i for i in range(40)], 3, 1, 64, "f16")])
+@pytest.mark.parametrize("mask", [0, 1, 2])
+def test_packed_repeats_bit_for_bit(lens, Hq, H, D, kind, mask):
+    r = np.random.default_rng([len(lens), mask])
+    q, k, v = (torch.from_numpy(r.standard_normal((h, sum(lens), D)).astype(np.float32)).to(DT[kind]).cuda()
+               for h in (Hq, H, H))
+    call = acefa.PackedAttn(q, k, v, _i32(np.concatenate([[0], np.cumsum(lens)]).tolist()), mask=mask, window=50)
+    first = call().clone()
+    for _ in range(10):
+        call.out.fill_(7.0)
+        assert torch.equal(call(), first)
+
+
+@pytest.mark.parametrize("D,Hq,H,n_q,lens,n_max,kind", [
+    (128, 8, 2, 1, [700, 3, 64], 768, "f32"), (64, 16, 4, 4, [3000], 6001, "f16"), (128, 16, 1, 2, [900, 5000], 5000, "f32")])
+def test_attend_with_weights_repeats_bit_for_bit(D, Hq, H, n_q, lens, n_max, kind):
+    r = np.random.default_rng([D, Hq, n_max])
+    sets = len(lens)
+    q8 = [torch.from_numpy(r.integers(-127, 128, (sets, H, n_max, D), dtype=np.int8)).cuda() for _ in range(2)]
+    s = [torch.from_numpy(r.random((sets, H, -(-n_max // 64))).astype(np.float32) / 64).cuda() for _ in range(2)]
+    q = torch.from_numpy(r.standard_normal((sets, Hq, n_q, D)).astype(np.float32)).to(DT[kind]).cuda()
+    weight = torch.zeros((sets, H, n_max), device="cuda")
+    call = acefa.Kv8Attn(q, acefa.Kv8Cache(*q8, *s), _i32(lens), weight=weight)
+    first = call().clone(), weight.clone()
+    for _ in range(10):
+        call.out.fill_(7.0), weight.zero_()
+        call()
+        assert torch.equal(call.out, first[0]) and torch.equal(weight, first[1])
+
+
+def test_packed_longest_sequence():
+    """2^24 keys under 200 queries: one pair of row tiles streams them all, inside the bound of every wait."""
+    n, D, rows = 1 << 24, 64, 200
+    g = torch.Generator(device="cuda").manual_seed(24)
+    q, k, v = (torch.randn((1, m, D), device="cuda", generator=g, dtype=torch.float16) for m in (rows, n, n))
+    out = acefa.PackedAttn(q, k, v, _i32([0, rows]), _i32([0, n]), scale=0.5,
+                           out=torch.empty((rows, 1, D), dtype=torch.float32, device="cuda"))()
+    assert acefa.device_error() == 0
+    num, size, den = (torch.zeros((rows, x), dtype=torch.float64, device="cuda") for x in (D, D, 1))
+    top = torch.full((rows, 1), -float("inf"), dtype=torch.float64, device="cuda")
+    for a in range(0, n, 1 << 18):
+        s = q[0].double() @ k[0, a:a + (1 << 18)].double().T * 0.5
+        new = torch.maximum(top, s.amax(-1, keepdim=True))
+        f, p = torch.exp(top - new), torch.exp(s - new)
+        vv = v[0, a:a + (1 << 18)].double()
+        num, size, den, top = num * f + p @ vv, size * f + p @ vv.abs(), den * f + p.sum(-1, keepdim=True), new
+    want = num / den
+    # weights rounded to 11 bits, scores off by 2^-17 * A, and F32 sums of 2^17 tiles in a row: 2^-24 of their running
+    # magnitude each, 2^-7 of the mean of |v| in all
+    A = 0.5 * float(q[0].abs().amax(0).float() @ k[0].abs().amax(0).float())
+    tol = (2.0 ** -11 + 2 * (2.0 ** -17 * A + 2.0 ** -20) + 2 * 2.0 ** -7) * size / den
+    assert ((out[:, 0].double() - want).abs() <= tol).all()
